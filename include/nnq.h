@@ -724,6 +724,81 @@ NNQ_API nnq_status nnq_decoder_set_head_options(nnq_decoder *d, const nnq_head_o
 NNQ_API nnq_status nnq_decoder_extend(nnq_decoder *d, const int32_t *tokens_host, int count, int start_pos, const int32_t *want,
                                       int n_want, float *logits_host, void *stream);
 
+/* ---- serving a batch of requests: a paged cache of keys and values in 8 bits ------------------------- */
+
+/* Keys and values of one layer in blocks of `block` tokens (16, 32, 64, 128 or 256): codes [blocks, kv_heads, block, dim]
+ * of one byte and one exponent byte per block and head, value = code * 2^(byte - 127), bytes 1 .. 253. dim 64, 128, 192
+ * or 256. All memory is the caller's (device, codes 16-byte aligned) and needs no clearing. Slot s of a cache is token
+ * s mod block of block s / block; blocks * block must fit 31 bits.
+ * The reference keeps one sequence's keys and values in f32 (KvCacheLayer,
+ * crates/nn-core/src/layers/generation/kv_cache.rs:132) and attends to them with sdpa
+ * (crates/nn-core/src/layers/attention/sdpa.rs:42-118); it has no counterpart of the tables and the 8-bit form. */
+typedef enum nnq_kv_format {
+    NNQ_KV_INT8 = 0,   /* two's complement */
+    NNQ_KV_E4M3 = 1    /* sign, four exponent bits (bias 7), three mantissa bits; the codes 0x7F and 0xFF read as +-480 */
+} nnq_kv_format;
+typedef struct nnq_kv_cache {
+    int32_t format;    /* nnq_kv_format */
+    int32_t kv_heads, dim, block;
+    int64_t blocks;
+    void *k, *v;
+    uint8_t *k_exp, *v_exp;
+} nnq_kv_cache;
+
+/* Block tables and slot maps of a step: request r held past[r] tokens and gets count[r] new ones (0 or more). In request
+ * order each takes the blocks that its new tokens need beyond those it has from free_dev [n_free], the first
+ * *skip_dev (NULL: none) of which are taken already, and appends them to its row of table_dev [requests, table_ld]; the
+ * rest of a table is read where a token falls into a block held before and otherwise left as it was. Written:
+ * length[r] = past[r] + count[r]; row_start [requests + 1], the sums of count (the packed rows of request r are
+ * row_start[r] .. row_start[r + 1] - 1); for each of `rows` packed rows its slot and position, -1 for rows behind the last
+ * request; *used_dev (may be NULL) = *skip_dev + blocks taken. Where the list or a table's row ends, the entry and the slots of
+ * its tokens are -1 and *used_dev says more than n_free. length_dev may be past_dev, used_dev may be
+ * skip_dev: a captured step then advances the batch. Negative counts are taken as 0. One launch; neither
+ * allocates nor synchronises, as all calls of this section. */
+NNQ_API nnq_status nnq_kv_tables(nnq_ctx *ctx, const int32_t *past_dev, const int32_t *count_dev, int64_t requests, const int32_t *free_dev, int64_t n_free,
+                                 const int32_t *skip_dev, int block, int32_t *table_dev, int64_t table_ld, int32_t *length_dev, int32_t *row_start_dev,
+                                 int32_t *slot_dev, int32_t *position_dev, int64_t rows, int32_t *used_dev, void *stream);
+
+/* Quantizes rows of keys and values ([rows, kv_heads, dim], rows k_ld / v_ld elements apart, 16-byte aligned) into their
+ * slots; rows of slot -1 are skipped. The exponent of a block and head is the least under which the largest new value does not
+ * pass the largest code (127, 448), and not below the block's old one where the block held tokens before the first new one;
+ * where it grew, the codes held before are rounded again. The tokens of one block must be consecutive rows with consecutive slots;
+ * a block in two separate runs of one call is not defined. NaN is stored as 0 and values beyond the range as the largest
+ * code; nnq_device_status then reports NNQ_ERR_VALUE_OUT_OF_RANGE for NaN and infinities. A slot beyond the cache is skipped and
+ * reported as NNQ_ERR_INVALID_ARG. */
+NNQ_API nnq_status nnq_kv_append(nnq_ctx *ctx, const nnq_kv_cache *cache, const void *k_dev, int64_t k_ld, const void *v_dev, int64_t v_ld, nnq_dtype dt,
+                                 const int32_t *slot_dev, int64_t rows, void *stream);
+
+/* The values of given slots, k and v [rows, kv_heads, dim] f32 or bf16 (exact in both); zeros for slot -1. */
+NNQ_API nnq_status nnq_kv_read(nnq_ctx *ctx, const nnq_kv_cache *cache, const int32_t *slot_dev, int64_t rows, void *k_dev, void *v_dev, nnq_dtype dt, void *stream);
+
+/* The batch as attention reads it: what nnq_kv_tables writes. max_rows: rows of the request with the most, as far as the
+ * host knows; it decides which kernels run, not what they compute. */
+typedef struct nnq_kv_batch {
+    const int32_t *length, *row_start, *table;
+    int64_t requests, table_ld, rows, max_rows;
+} nnq_kv_batch;
+
+/* Softmax attention over the cache: row i of request r stands at position length[r] - (rows of r) + i and sees the positions up to
+ * its own, with window > 0 the last `window` of them; query head h reads key / value head h / (heads / kv_heads).
+ * q [rows, heads, dim] and y in the same layout, f32 or bf16, rows q_ld / y_ld elements apart, 16-byte aligned. A row that sees
+ * nothing is zero; rows behind the last request are left as they were. Scores, softmax and sums are f32, codes exact, queries
+ * and weights enter the products with 22 bits or more (bf16 queries exactly). A block number outside the cache is not read: its positions
+ * count as unseen, and nnq_device_status reports NNQ_ERR_INVALID_ARG. The workspace (nnq_kv_attention_workspace; 16-byte
+ * aligned, contents arbitrary) must not be shared by calls that can overlap. */
+NNQ_API nnq_status nnq_kv_attention_workspace(nnq_ctx *ctx, const nnq_kv_cache *cache, const nnq_kv_batch *batch, int heads, size_t *bytes);
+NNQ_API nnq_status nnq_kv_attention(nnq_ctx *ctx, const nnq_kv_cache *cache, const nnq_kv_batch *batch, const void *q_dev, nnq_dtype q_dt, int64_t q_ld, int heads,
+                                    float scale, int window, void *y_dev, nnq_dtype y_dt, int64_t y_ld, void *workspace, size_t workspace_bytes, void *stream);
+
+/* Log probabilities from rows of logits [rows, vocab] (f32 or bf16, rows ld elements apart): logprob[r] of token[r] (0 for a
+ * negative token; NaN and NNQ_ERR_INVALID_ARG from nnq_device_status beyond the vocabulary), the entropy of the row in nats, and its `top`
+ * (0 .. 32) most probable tokens, [rows, top], in descending order, of equal ones the lowest first. Outputs that are not wanted may be
+ * NULL (token_dev too, without logprob). Logits of -inf have probability 0; a row of nothing else has entropy 0 and log probabilities of
+ * -inf; with a NaN or +inf the row's numbers are NaN, and a NaN ranks highest. f32 throughout. The reference's samplers
+ * do this on the host (crates/nn-core/src/layers/generation/autoregressive_sampling.rs:14-21). */
+NNQ_API nnq_status nnq_token_logprobs(nnq_ctx *ctx, const void *logits_dev, nnq_dtype dt, int64_t rows, int64_t vocab, int64_t ld, const int32_t *token_dev, int top,
+                                      float *logprob_dev, float *entropy_dev, int32_t *top_token_dev, float *top_logprob_dev, void *stream);
+
 /* Number of kernels this library has launched on this context since creation. */
 NNQ_API int64_t nnq_launch_count(const nnq_ctx *ctx);
 

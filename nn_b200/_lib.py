@@ -115,6 +115,15 @@ SIGNATURES = {
     "nnq_moe_forward_routed": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_int64, c_int, c_void_p, c_void_p, c_void_p, c_void_p]),
     "nnq_moe_gather_rows": (c_int, [c_void_p, c_void_p, c_int, c_void_p, c_int64, c_int64, c_void_p, c_void_p]),
     "nnq_moe_combine_rows": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int, c_int, c_void_p, c_void_p]),
+    "nnq_kv_tables": (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int, c_void_p, c_int64, c_void_p, c_void_p,
+                              c_void_p, c_void_p, c_int64, c_void_p, c_void_p]),
+    "nnq_kv_append": (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_int64, c_int, c_void_p, c_int64, c_void_p]),
+    "nnq_kv_read": (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_int, c_void_p]),
+    "nnq_kv_attention_workspace": (c_int, [c_void_p, c_void_p, c_void_p, c_int, ctypes.POINTER(c_size_t)]),
+    "nnq_kv_attention": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int64, c_int, ctypes.c_float, c_int, c_void_p, c_int, c_int64,
+                                 c_void_p, c_size_t, c_void_p]),
+    "nnq_token_logprobs": (c_int, [c_void_p, c_void_p, c_int, c_int64, c_int64, c_int64, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p,
+                                   c_void_p]),
     "nnq_moe_route": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_int64, c_void_p, c_void_p, c_void_p]),
 }
 

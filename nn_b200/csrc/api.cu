@@ -203,6 +203,8 @@ nnq_status nnq_device_status(nnq_ctx *ctx, void *stream) {
     cudaStreamSynchronize(st);
     if (v == 1) return fail(ctx, NNQ_ERR_TIMEOUT, "a bounded device wait ran out (device status word = 1)");
     if (v == 2) return fail(ctx, NNQ_ERR_UNSUPPORTED, "a decoder was stepped past its last position (max_seq): its context is full, reset it");
+    if (v == 3) return fail(ctx, NNQ_ERR_VALUE_OUT_OF_RANGE, "a key or value appended to a cache was not finite");
+    if (v == 4) return fail(ctx, NNQ_ERR_INVALID_ARG, "a slot, block number, row or token outside its range reached a kernel");
     return fail(ctx, NNQ_ERR_OTHER, "device status word = %d", v);
 }
 

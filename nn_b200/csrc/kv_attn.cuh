@@ -1,0 +1,85 @@
+// Attention over the paged 8-bit cache: what its kernels share (layout of the cache: kv_cache.cuh).
+#pragma once
+#include "kv_cache.cuh"
+
+namespace nnq {
+
+struct KvAttn {
+    const uint8_t *k, *v, *k_exp, *v_exp;
+    const int32_t *length, *row_start, *table;
+    const void *q;
+    void *y;
+    int64_t blocks, table_ld, requests, q_ld, y_ld, rows;
+    int kv_heads, group, dim, shift, window;   // window 0: every earlier position
+    int q_dt, y_dt;
+    float scale;
+    int *status;
+};
+
+// One request of the batch as the kernels take it: numbers outside their range are brought inside (the results of such a request are
+// undefined, its reads and writes are not).
+struct KvRequest {
+    int row0, rows;       // its rows of q and y
+    int64_t length;       // positions held, the rows' own included
+};
+__device__ __forceinline__ KvRequest kv_request(const KvAttn &a, int64_t r) {
+    KvRequest q;
+    const int s0 = (int)min(max((int64_t)a.row_start[r], (int64_t)0), a.rows), s1 = (int)min(max((int64_t)a.row_start[r + 1], (int64_t)s0), a.rows);
+    q.row0 = s0;
+    q.rows = s1 - s0;
+    q.length = min(max((int64_t)a.length[r], (int64_t)0), a.table_ld << a.shift);
+    if (q.length < a.length[r] || s0 != a.row_start[r] || s1 != a.row_start[r + 1]) atomicExch(a.status, kStatusIndex);
+    return q;
+}
+// position of row i, and the first position it sees
+__device__ __forceinline__ int64_t row_pos(const KvRequest &q, int i) { return q.length - q.rows + i; }
+__device__ __forceinline__ int64_t row_first(const KvAttn &a, int64_t pos) { return a.window > 0 ? max(pos - a.window + 1, (int64_t)0) : 0; }
+
+// Two f16 numbers of two codes that lie in the bytes of a 16-bit half each: int8 exactly, e4m3 times 2^-8 (its bits moved to their
+// place in an f16 number, subnormal ones included).
+template <int FMT>
+struct CodePairs;
+template <>
+struct CodePairs<NNQ_KV_INT8> {
+    static constexpr float unscale = 1.0f;
+    // codes + 128 in the low bits of 1024: exact
+    static __device__ __forceinline__ uint32_t word(uint32_t w) { return w ^ 0x80808080u; }
+    static __device__ __forceinline__ uint32_t half(uint32_t biased) {
+        const __half2 h = __hsub2(*reinterpret_cast<const __half2 *>(&biased), __half2half2(__ushort_as_half(0x6480)));   // 1152
+        return *reinterpret_cast<const uint32_t *>(&h);
+    }
+    // bytes 0, 1 (2, 3) of a word
+    static __device__ __forceinline__ uint32_t low(uint32_t w) { return half(__byte_perm(w, 0x64646464u, 0x4140)); }
+    static __device__ __forceinline__ uint32_t high(uint32_t w) { return half(__byte_perm(w, 0x64646464u, 0x4342)); }
+};
+template <>
+struct CodePairs<NNQ_KV_E4M3> {
+    static constexpr float unscale = 256.0f;
+    static __device__ __forceinline__ uint32_t word(uint32_t w) { return w; }
+    static __device__ __forceinline__ uint32_t half(uint32_t x) { return (x & 0x80008000u) | ((x >> 1) & 0x3F803F80u); }
+    static __device__ __forceinline__ uint32_t low(uint32_t w) { return half(__byte_perm(w, 0, 0x1404)); }
+    static __device__ __forceinline__ uint32_t high(uint32_t w) { return half(__byte_perm(w, 0, 0x3424)); }
+};
+
+__device__ __forceinline__ float kv_ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// The power of two that brings the largest absolute value of a query vector (its bits) to 2^14 .. 2^15, and its inverse. Elements
+// from 2^-28 of the largest on keep all of an f16 number's bits. Largest values below 2^-112 are scaled like that one.
+__device__ __forceinline__ uint32_t kv_top(uint32_t bits) { return min(max(bits >> 23, 15u), 254u); }
+__device__ __forceinline__ float kv_top_scale(uint32_t bits) { return __uint_as_float((268u - kv_top(bits)) << 23); }
+__device__ __forceinline__ float kv_top_unscale(uint32_t bits) { return __uint_as_float((kv_top(bits) - 14u) << 23); }
+
+__device__ __forceinline__ uint32_t half_bits(__half2 h) { return *reinterpret_cast<const uint32_t *>(&h); }
+// x and y as f16 pairs: the nearest values, and the nearest values of what they leave
+__device__ __forceinline__ void kv_split(float x, float y, uint32_t &hi, uint32_t &lo) {
+    const __half2 h = __floats2half2_rn(x, y);
+    const float2 f = __half22float2(h);
+    hi = half_bits(h);
+    lo = half_bits(__floats2half2_rn(x - f.x, y - f.y));
+}
+
+}  // namespace nnq

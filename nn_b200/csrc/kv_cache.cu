@@ -1,0 +1,402 @@
+// Block tables and slot maps of a batch of requests, and what writes and reads the codes of the paged 8-bit cache (kv_cache.cuh).
+// The reference keeps one sequence's keys and values in f32 and doubles the buffer as it grows
+// (crates/nn-core/src/layers/generation/kv_cache.rs:132).
+#include <algorithm>
+
+#include "kv_cache.cuh"
+#include "tcgen05.cuh"
+
+namespace nnq {
+
+// ---- tables ---------------------------------------------------------------------------------------------------------------------
+
+// One launch of one cluster: every CTA sums the counts of all requests, in portions of kTabChunk that lie in shared memory, and writes
+// its share of the tables: entry i of the portion's new blocks, row i of its rows, found by bisection of the sums. The cluster meets
+// between the reading of a portion and the writing, so lengths may be written where the old ones lie. What bounds it is latency:
+// the requests' loads, the sums, the bisection, one dependent load for a block that was there before.
+constexpr int kTabChunk = 2048;
+
+struct TableArgs {
+    const int32_t *past, *count, *free_list, *skip;
+    int32_t *table, *length, *row_start, *slot, *position, *used;
+    int64_t requests, n_free, table_ld, rows;
+    int shift;
+};
+
+// exclusive sums of two numbers over the block's threads; returns the totals
+__device__ __forceinline__ longlong2 block_scan2(longlong2 &v, longlong2 *warp_sums) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
+    longlong2 x = v;
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+        const long long a = __shfl_up_sync(0xFFFFFFFFu, x.x, off), b = __shfl_up_sync(0xFFFFFFFFu, x.y, off);
+        if (lane >= off) {
+            x.x += a;
+            x.y += b;
+        }
+    }
+    __syncthreads();
+    if (lane == 31) warp_sums[warp] = x;
+    __syncthreads();
+    longlong2 before = make_longlong2(0, 0), all = make_longlong2(0, 0);
+    for (int w = 0; w < nw; w++) {
+        if (w == warp) before = all;
+        all.x += warp_sums[w].x;
+        all.y += warp_sums[w].y;
+    }
+    v = make_longlong2(before.x + x.x - v.x, before.y + x.y - v.y);
+    return all;
+}
+
+// the last of `n` ascending sums that is not above x (sums[0] <= x)
+__device__ __forceinline__ int find_sum(const long long *sums, int n, long long x) {
+    int lo = 0, hi = n - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (sums[mid] <= x) lo = mid;
+        else hi = mid - 1;
+    }
+    return lo;
+}
+
+__global__ void __launch_bounds__(1024) kv_tables_kernel(const TableArgs a) {
+    __shared__ long long row0[kTabChunk], new0[kTabChunk];   // first row and first new block of every request of the portion
+    __shared__ int held[kTabChunk];
+    __shared__ longlong2 warp_sums[32];
+    pdl_prologue();
+    const int tid = threadIdx.x, nt = blockDim.x;
+    const int64_t me = (int64_t)blockIdx.x * nt + tid, all = (int64_t)gridDim.x * nt;
+    const int64_t block = (int64_t)1 << a.shift;
+    const int64_t skip = a.skip ? max(*a.skip, 0) : 0;
+    longlong2 done = make_longlong2(0, 0);   // rows and new blocks of the portions before
+    for (int64_t r0 = 0; r0 < a.requests; r0 += kTabChunk) {
+        const int n = (int)min((int64_t)kTabChunk, a.requests - r0);
+        longlong2 sum = make_longlong2(0, 0);
+        for (int i0 = 0; i0 < n; i0 += nt) {
+            const int i = i0 + tid;
+            longlong2 v = make_longlong2(0, 0);
+            int64_t past = 0;
+            if (i < n) {
+                past = max(a.past[r0 + i], 0);
+                v.x = max(a.count[r0 + i], 0);
+                v.y = ((past + v.x + block - 1) >> a.shift) - ((past + block - 1) >> a.shift);
+            }
+            const longlong2 part = block_scan2(v, warp_sums);
+            if (i < n) {
+                held[i] = (int)past;
+                row0[i] = sum.x + v.x;
+                new0[i] = sum.y + v.y;
+            }
+            sum.x += part.x;
+            sum.y += part.y;
+        }
+        __syncthreads();
+        if (gridDim.x > 1) cluster_sync();
+        auto count_of = [&](int i) { return (i + 1 < n ? row0[i + 1] : sum.x) - row0[i]; };
+        for (int64_t i = me; i < n; i += all) {
+            a.length[r0 + i] = (int32_t)min((long long)held[i] + count_of((int)i), (long long)INT32_MAX);
+            a.row_start[r0 + i] = (int32_t)min(done.x + row0[i], (long long)INT32_MAX);
+        }
+        // the block a request's new block number j (from its first) gets
+        auto fresh = [&](int i, int64_t j) {
+            const int64_t at = skip + done.y + new0[i] + j;
+            return at < a.n_free ? a.free_list[at] : -1;
+        };
+        for (int64_t e = me; e < sum.y; e += all) {
+            const int i = find_sum(new0, n, e);
+            const int64_t col = (((int64_t)held[i] + block - 1) >> a.shift) + e - new0[i];
+            if (col < a.table_ld) a.table[(r0 + i) * a.table_ld + col] = fresh(i, e - new0[i]);
+        }
+        const int64_t last = min((int64_t)sum.x, a.rows - (int64_t)done.x);
+        for (int64_t t = me; t < last; t += all) {
+            const int i = find_sum(row0, n, t);
+            const int64_t pos = held[i] + t - row0[i], col = pos >> a.shift, first = ((int64_t)held[i] + block - 1) >> a.shift;
+            int64_t b = -1;
+            if (col < a.table_ld) b = col < first ? a.table[(r0 + i) * a.table_ld + col] : fresh(i, col - first);
+            const int64_t s = (b << a.shift) + (pos & (block - 1));
+            a.slot[done.x + t] = b >= 0 && s <= INT32_MAX ? (int32_t)s : -1;
+            a.position[done.x + t] = (int32_t)min(pos, (int64_t)INT32_MAX);
+        }
+        done.x += sum.x;
+        done.y += sum.y;
+        __syncthreads();   // the portion's sums have been read
+    }
+    for (int64_t t = done.x + me; t < a.rows; t += all) a.slot[t] = a.position[t] = -1;
+    if (gridDim.x > 1) cluster_sync();   // (every CTA has read *skip)
+    if (me == 0) {
+        a.row_start[a.requests] = (int32_t)min(done.x, (long long)INT32_MAX);
+        if (a.used) *a.used = (int32_t)min(skip + done.y, (long long)INT32_MAX);
+    }
+}
+
+// ---- append ---------------------------------------------------------------------------------------------------------------------
+
+// Rows whose slots run on inside one block are a run; its first row is the leader. A CTA has kAppRows rows of one head, keys or values.
+// With one leader among them all warps work on its run (which may reach beyond the CTA's rows); with several a warp takes each.
+// A run: largest absolute value (bits compare like the numbers; non-finite ones are left out), exponent byte, codes; codes the block
+// held before are rounded again where the exponent grew.
+constexpr int kAppRows = 8, kAppWarps = 8;
+
+struct AppendArgs {
+    struct Part {
+        const void *x;
+        int64_t ld;
+        uint8_t *codes, *exps;
+    } keys, values;
+    const int32_t *slot;
+    int64_t rows, slots;
+    int kv_heads, dim, shift;
+    int *status;
+};
+
+template <bool F32>
+__device__ __forceinline__ void load8(const void *p, int64_t at, float (&v)[8]) {
+    if constexpr (F32) {
+        const float4 a = __ldg(reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(p) + at));
+        const float4 b = __ldg(reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(p) + at) + 1);
+        v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+    } else {
+        const uint4 a = __ldg(reinterpret_cast<const uint4 *>(reinterpret_cast<const __nv_bfloat16 *>(p) + at));
+        const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            v[2 * i] = __uint_as_float(w[i] << 16);
+            v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+        }
+    }
+}
+
+// A run of `n` rows from row `t` on, by `threads` threads of which this is number `me`; sync and reduce are theirs.
+template <int FMT, bool F32, typename Reduce, typename Sync>
+__device__ __forceinline__ void append_run(const AppendArgs &a, const AppendArgs::Part &p, int head, int64_t t, int n, int me, int threads, Reduce reduce, Sync sync) {
+    const int units = a.dim >> 3, first = a.slot[t];
+    const int64_t blk = first >> a.shift;
+    const int off = first & ((1 << a.shift) - 1);
+    const int64_t base = t * p.ld + (int64_t)head * a.dim;
+    uint8_t *codes = p.codes + (((blk * a.kv_heads + head) << a.shift) * a.dim), *exp_at = p.exps + blk * a.kv_heads + head;
+    const int old = off ? min(max((int)*exp_at, 0), kExpMax) : 0;
+    uint32_t top = 0;
+    bool bad = false;
+    for (int u = me; u < n * units; u += threads) {
+        const int row = u / units, d = (u - row * units) * 8;
+        float v[8];
+        load8<F32>(p.x, base + row * p.ld + d, v);
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const uint32_t b = __float_as_uint(v[i]) & 0x7FFFFFFFu;
+            if (b >= 0x7F800000u) bad = true;
+            else top = max(top, b);
+        }
+    }
+    if (bad) atomicExch(a.status, kStatusValue);
+    top = reduce(top);
+    const int e = max(exponent_byte<FMT>(top), old);
+    const float inv = pow2_byte(254 - e);
+    for (int u = me; u < n * units; u += threads) {
+        const int row = u / units, d = (u - row * units) * 8;
+        float v[8];
+        load8<F32>(p.x, base + row * p.ld + d, v);
+        uint32_t w[2] = {0, 0};
+#pragma unroll
+        for (int i = 0; i < 8; i++) w[i >> 2] |= kv_encode<FMT>(v[i] * inv) << (8 * (i & 3));
+        *reinterpret_cast<uint2 *>(codes + (int64_t)(off + row) * a.dim + d) = make_uint2(w[0], w[1]);
+    }
+    if (off && e > old) {
+        const float again = pow2_byte(max(127 + old - e, 0));
+        for (int u = me; u < off * units; u += threads) {
+            uint2 *at = reinterpret_cast<uint2 *>(codes) + u;
+            const uint2 c = *at;
+            uint32_t in[2] = {c.x, c.y}, w[2] = {0, 0};
+#pragma unroll
+            for (int i = 0; i < 8; i++) w[i >> 2] |= kv_encode<FMT>(kv_decode<FMT>(in[i >> 2] >> (8 * (i & 3)) & 0xFFu) * again) << (8 * (i & 3));
+            *at = make_uint2(w[0], w[1]);
+        }
+    }
+    sync();   // everybody has read the old byte
+    if (me == 0) *exp_at = (uint8_t)e;
+}
+
+template <int FMT, bool F32>
+__global__ void __launch_bounds__(kAppWarps * 32) kv_append_kernel(const AppendArgs a) {
+    __shared__ uint32_t red[kAppWarps];
+    pdl_prologue();
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, head = blockIdx.y;
+    const AppendArgs::Part part = blockIdx.z ? a.values : a.keys;
+    const int64_t t0 = (int64_t)blockIdx.x * kAppRows;
+    const int block = 1 << a.shift;
+    // leaders among the CTA's rows (every warp finds them for itself)
+    const int64_t t = t0 + lane;
+    int s = -1, before = -1;
+    if (lane < kAppRows && t < a.rows) {
+        s = a.slot[t];
+        if (t > 0) before = a.slot[t - 1];
+    }
+    if (s >= a.slots) {
+        if (tid < kAppRows) atomicExch(a.status, kStatusIndex);
+        s = -1;
+    }
+    const bool leads = s >= 0 && (before < 0 || before != s - 1 || (s & (block - 1)) == 0);
+    uint32_t leaders = __ballot_sync(0xFFFFFFFFu, leads);
+    auto run_length = [&](int64_t from) {
+        const int first = a.slot[from], most = block - (first & (block - 1));
+        for (int i0 = 0; i0 < most; i0 += 32) {
+            const int i = i0 + lane;
+            const bool on = i < most && from + i < a.rows && a.slot[from + i] == first + i;
+            const uint32_t m = __ballot_sync(0xFFFFFFFFu, on);
+            if (m != 0xFFFFFFFFu) return i0 + __ffs(~m) - 1;
+        }
+        return most;
+    };
+    if (__popc(leaders) == 1) {
+        const int64_t from = t0 + __ffs(leaders) - 1;
+        append_run<FMT, F32>(a, part, head, from, run_length(from), tid, kAppWarps * 32,
+                             [&](uint32_t v) {
+                                 v = __reduce_max_sync(0xFFFFFFFFu, v);
+                                 if (lane == 0) red[warp] = v;
+                                 __syncthreads();
+                                 uint32_t m = 0;
+#pragma unroll
+                                 for (int w = 0; w < kAppWarps; w++) m = max(m, red[w]);
+                                 return m;
+                             },
+                             [] { __syncthreads(); });
+    } else {
+        for (int i = 0; leaders; i++) {
+            const int64_t from = t0 + __ffs(leaders) - 1;
+            leaders &= leaders - 1;
+            if (i % kAppWarps == warp)
+                append_run<FMT, F32>(a, part, head, from, run_length(from), lane, 32, [](uint32_t v) { return __reduce_max_sync(0xFFFFFFFFu, v); }, [] { __syncwarp(); });
+        }
+    }
+}
+
+// ---- read -----------------------------------------------------------------------------------------------------------------------
+
+struct ReadArgs {
+    struct Part {
+        const uint8_t *codes, *exps;
+        void *y;
+    } keys, values;
+    const int32_t *slot;
+    int64_t rows, slots;
+    int kv_heads, dim, shift;
+    int *status;
+};
+
+// A thread has 16 values of a row: one load, two or four stores. Rows of no slot are zeros.
+template <int FMT, bool F32>
+__global__ void __launch_bounds__(256) kv_read_kernel(const ReadArgs a) {
+    pdl_prologue();
+    const ReadArgs::Part part = blockIdx.y ? a.values : a.keys;
+    const int units = a.kv_heads * (a.dim >> 4);
+    const int64_t total = a.rows * units;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+        const int64_t row = i / units;
+        const int u = (int)(i - row * units), head = u / (a.dim >> 4), d = (u - head * (a.dim >> 4)) * 16;
+        const int s = a.slot[row];
+        float v[16];
+#pragma unroll
+        for (int k = 0; k < 16; k++) v[k] = 0.0f;
+        if (s >= a.slots) atomicExch(a.status, kStatusIndex);
+        else if (s >= 0) {
+            const int64_t bh = (int64_t)(s >> a.shift) * a.kv_heads + head;
+            const uint4 c = __ldg(reinterpret_cast<const uint4 *>(part.codes + ((bh << a.shift) + (s & ((1 << a.shift) - 1))) * a.dim + d));
+            const float f = pow2_byte(part.exps[bh]);
+            const uint32_t w[4] = {c.x, c.y, c.z, c.w};
+#pragma unroll
+            for (int k = 0; k < 16; k++) v[k] = kv_decode<FMT>(w[k >> 2] >> (8 * (k & 3)) & 0xFFu) * f;
+        }
+        const int64_t at = (row * a.kv_heads + head) * a.dim + d;
+        if constexpr (F32) {
+            float4 *y = reinterpret_cast<float4 *>(reinterpret_cast<float *>(part.y) + at);
+#pragma unroll
+            for (int k = 0; k < 4; k++) y[k] = make_float4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]);
+        } else {
+            uint4 *y = reinterpret_cast<uint4 *>(reinterpret_cast<__nv_bfloat16 *>(part.y) + at);
+#pragma unroll
+            for (int k = 0; k < 2; k++)
+                y[k] = make_uint4(pack_bf16(v[8 * k], v[8 * k + 1]), pack_bf16(v[8 * k + 2], v[8 * k + 3]), pack_bf16(v[8 * k + 4], v[8 * k + 5]), pack_bf16(v[8 * k + 6], v[8 * k + 7]));
+        }
+    }
+}
+
+}  // namespace nnq
+
+using namespace nnq;
+
+extern "C" {
+
+nnq_status nnq_kv_tables(nnq_ctx *ctx, const int32_t *past_dev, const int32_t *count_dev, int64_t requests, const int32_t *free_dev, int64_t n_free,
+                         const int32_t *skip_dev, int block, int32_t *table_dev, int64_t table_ld, int32_t *length_dev, int32_t *row_start_dev,
+                         int32_t *slot_dev, int32_t *position_dev, int64_t rows, int32_t *used_dev, void *stream) {
+    if (!ctx) return NNQ_ERR_INVALID_ARG;
+    if (requests < 1 || n_free < 0 || table_ld < 1 || rows < 0) return fail(ctx, NNQ_ERR_INVALID_ARG, "bad sizes of a batch");
+    if (requests > INT32_MAX / 2 || rows > INT32_MAX) return fail(ctx, NNQ_ERR_UNSUPPORTED, "a batch of %lld requests and %lld rows", (long long)requests, (long long)rows);
+    if (block < 16 || block > 256 || (block & (block - 1))) return fail(ctx, NNQ_ERR_UNSUPPORTED, "blocks must hold 16, 32, 64, 128 or 256 tokens (got %d)", block);
+    if (!past_dev || !count_dev || (n_free && !free_dev) || !table_dev || !length_dev || !row_start_dev || (rows && (!slot_dev || !position_dev)))
+        return fail(ctx, NNQ_ERR_INVALID_ARG, "NULL tensor in a batch");
+    nnq_status s = check_cuda(ctx, cudaSetDevice(ctx->device), "cudaSetDevice");
+    if (s != NNQ_OK) return s;
+    const TableArgs a = {past_dev, count_dev, free_dev, skip_dev, table_dev, length_dev, row_start_dev, slot_dev, position_dev, used_dev, requests, n_free, table_ld, rows, log2_of(block)};
+    const bool small = requests <= 256 && rows <= 1024;
+    cudaLaunchConfig_t cfg = {};
+    cfg.blockDim = dim3(small ? 256 : 1024);
+    cfg.gridDim = dim3(small ? 1 : (unsigned)std::min<int64_t>(8, (std::max(rows, requests) + 2047) / 2048));
+    cfg.stream = (cudaStream_t)stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim = {cfg.gridDim.x, 1, 1};
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    s = check_cuda(ctx, cudaLaunchKernelEx(&cfg, kv_tables_kernel, a), "block tables launch");
+    if (s == NNQ_OK) ctx->launches++;
+    return s;
+}
+
+nnq_status nnq_kv_append(nnq_ctx *ctx, const nnq_kv_cache *c, const void *k_dev, int64_t k_ld, const void *v_dev, int64_t v_ld, nnq_dtype dt,
+                         const int32_t *slot_dev, int64_t rows, void *stream) {
+    if (!ctx) return NNQ_ERR_INVALID_ARG;
+    nnq_status s = check_kv_cache(ctx, c);
+    if (s != NNQ_OK) return s;
+    if (dt != NNQ_F32 && dt != NNQ_BF16) return fail(ctx, NNQ_ERR_INVALID_ARG, "unknown dtype %d", (int)dt);
+    if (rows < 0 || rows > INT32_MAX) return fail(ctx, NNQ_ERR_INVALID_ARG, "%lld rows", (long long)rows);
+    if (rows == 0) return NNQ_OK;
+    if (!k_dev || !v_dev || !slot_dev) return fail(ctx, NNQ_ERR_INVALID_ARG, "NULL tensor");
+    const int64_t width = (int64_t)c->kv_heads * c->dim;
+    if (k_ld < width || v_ld < width) return fail(ctx, NNQ_ERR_SHAPE_MISMATCH, "rows of keys and values must be %lld wide or further apart", (long long)width);
+    if (!rows_aligned(k_dev, k_ld, dt) || !rows_aligned(v_dev, v_ld, dt)) return fail(ctx, NNQ_ERR_INVALID_ARG, "rows of keys and values must start at multiples of 16 bytes");
+    if ((s = check_cuda(ctx, cudaSetDevice(ctx->device), "cudaSetDevice")) != NNQ_OK) return s;
+    const AppendArgs a = {{k_dev, k_ld, (uint8_t *)c->k, c->k_exp}, {v_dev, v_ld, (uint8_t *)c->v, c->v_exp}, slot_dev, rows, c->blocks * c->block, c->kv_heads, c->dim,
+                          log2_of(c->block), ctx->d_status};
+    const dim3 grid((unsigned)((rows + kAppRows - 1) / kAppRows), c->kv_heads, 2), block(kAppWarps * 32);
+    auto kernel = c->format == NNQ_KV_INT8 ? (dt == NNQ_F32 ? kv_append_kernel<NNQ_KV_INT8, true> : kv_append_kernel<NNQ_KV_INT8, false>)
+                                           : (dt == NNQ_F32 ? kv_append_kernel<NNQ_KV_E4M3, true> : kv_append_kernel<NNQ_KV_E4M3, false>);
+    launch_pdl(kernel, grid, block, (cudaStream_t)stream, a);
+    ctx->launches++;
+    return check_cuda(ctx, cudaGetLastError(), "cache append launch");
+}
+
+nnq_status nnq_kv_read(nnq_ctx *ctx, const nnq_kv_cache *c, const int32_t *slot_dev, int64_t rows, void *k_dev, void *v_dev, nnq_dtype dt, void *stream) {
+    if (!ctx) return NNQ_ERR_INVALID_ARG;
+    nnq_status s = check_kv_cache(ctx, c);
+    if (s != NNQ_OK) return s;
+    if (dt != NNQ_F32 && dt != NNQ_BF16) return fail(ctx, NNQ_ERR_INVALID_ARG, "unknown dtype %d", (int)dt);
+    if (rows < 0 || rows > INT32_MAX) return fail(ctx, NNQ_ERR_INVALID_ARG, "%lld rows", (long long)rows);
+    if (rows == 0) return NNQ_OK;
+    if (!k_dev || !v_dev || !slot_dev) return fail(ctx, NNQ_ERR_INVALID_ARG, "NULL tensor");
+    if (((uintptr_t)k_dev | (uintptr_t)v_dev) & 15u) return fail(ctx, NNQ_ERR_INVALID_ARG, "outputs must be 16-byte aligned");
+    if ((s = check_cuda(ctx, cudaSetDevice(ctx->device), "cudaSetDevice")) != NNQ_OK) return s;
+    const ReadArgs a = {{(const uint8_t *)c->k, c->k_exp, k_dev}, {(const uint8_t *)c->v, c->v_exp, v_dev}, slot_dev, rows, c->blocks * c->block, c->kv_heads, c->dim,
+                        log2_of(c->block), ctx->d_status};
+    const int64_t units = rows * c->kv_heads * (c->dim >> 4);
+    const dim3 grid((unsigned)std::min<int64_t>((units + 255) / 256, (int64_t)8 * ctx->sm_count), 2);
+    auto kernel = c->format == NNQ_KV_INT8 ? (dt == NNQ_F32 ? kv_read_kernel<NNQ_KV_INT8, true> : kv_read_kernel<NNQ_KV_INT8, false>)
+                                           : (dt == NNQ_F32 ? kv_read_kernel<NNQ_KV_E4M3, true> : kv_read_kernel<NNQ_KV_E4M3, false>);
+    launch_pdl(kernel, grid, dim3(256), (cudaStream_t)stream, a);
+    ctx->launches++;
+    return check_cuda(ctx, cudaGetLastError(), "cache read launch");
+}
+
+}  // extern "C"

@@ -1,0 +1,147 @@
+"""Log probabilities, entropies and most probable tokens of rows of logits against 64 bits."""
+import numpy as np
+import pytest
+
+torch = pytest.importorskip("torch")
+
+from nn_b200 import api
+from nn_b200.logprobs import token_logprobs
+from tests import kv_reference as ref
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+
+
+def check(x, tokens, top):
+    """lse = m + ln l: an exponent is off by 2^-22 relative and its argument by 2^-24 of itself, a thread's sums round by 2^-24 per
+    element (one in 512 of the row), differences to the maximum by 2^-24 of their size. Entropy: the same on numbers of its size."""
+    r = token_logprobs(x, tokens, top)
+    lp, ent, order, tl = ref.logprobs(x.double().cpu().numpy(), tokens.cpu().numpy(), top)
+    eps = 2.0 ** -20 + (x.shape[1] / 512 + 64) * 2.0 ** -24
+    spread = 1 + np.log(x.shape[1])
+    assert (np.abs(r.logprob.double().cpu().numpy() - lp) <= eps * spread + 2.0 ** -22 * np.abs(lp)).all()
+    assert (np.abs(r.entropy.double().cpu().numpy() - ent) <= 2 * eps * spread).all()
+    if top:
+        assert np.array_equal(r.top_tokens.cpu().numpy(), order)
+        assert (np.abs(r.top_logprobs.double().cpu().numpy() - tl) <= eps * spread + 2.0 ** -22 * np.abs(tl)).all()
+    return r
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows,vocab", [(1, 1), (1, 2), (3, 31), (2, 100), (5, 1000), (1, 4097), (1, 151936), (7, 32001), (160, 9001), (400, 515)])
+@pytest.mark.parametrize("top", [0, 1, 5, 32])
+def test_rows_of_every_size(dtype, rows, vocab, top):
+    g = torch.Generator(device=DEV).manual_seed(vocab + top)
+    x = (torch.randn(rows, vocab, device=DEV, generator=g) * 3).to(dtype)
+    t = torch.randint(0, vocab, (rows,), device=DEV, generator=g, dtype=torch.int32)
+    check(x, t, min(top, vocab))
+    api.gpu_backend().device_status()
+
+
+@pytest.mark.parametrize("vocab", [700, 40000])
+def test_orders_and_equal_values(vocab):
+    i = torch.arange(vocab, device=DEV, dtype=torch.float32)
+    rows = [i / vocab * 20, -i / vocab * 20, torch.zeros_like(i), (i % 3), -(i % 7), torch.where(i == vocab - 1, 5.0, 0.0), torch.where(i < 20, 1.0, -60.0), i * 0 - 0.0]
+    x = torch.stack(rows)
+    x[7, ::2] = 0.0   # 0 and -0 are equal
+    t = torch.tensor([0, vocab - 1, 5, 7, 100, vocab - 1, 3, 9], device=DEV)
+    for top in (1, 7, 32):
+        check(x, t, top)
+
+
+def test_large_small_and_shifted_logits():
+    x = torch.randn(6, 5001, device=DEV)
+    x[0] += 5000
+    x[1] -= 5000
+    x[2] *= 300
+    x[3] *= 1e-30
+    x[4] = 1e30 * torch.sign(x[4])
+    x[5, 17] = 200
+    t = torch.full((6,), 17, device=DEV)
+    r = check(x[[0, 1, 2, 3, 5]], t[:5], 8)
+    assert r.entropy.isfinite().all()
+    r = token_logprobs(x[4:5], t[:1], 4)
+    assert r.logprob.item() <= 0 and torch.equal(r.top_tokens[0].long(), (x[4] > 0).nonzero()[:4, 0])
+
+
+@pytest.mark.parametrize("vocab", [50, 20000])
+def test_logits_of_minus_infinity(vocab):
+    x = torch.randn(4, vocab, device=DEV)
+    x[0, 1:] = -float("inf")          # one token left
+    x[1, ::2] = -float("inf")
+    x[2] = -float("inf")              # none
+    x[3, 5:] = torch.finfo(torch.float32).min
+    t = torch.tensor([0, 0, 3, 7], device=DEV)
+    r = token_logprobs(x, t, 6)
+    lp, ent, order, tl = (a[[0, 1, 3]] for a in ref.logprobs(x.double().cpu().numpy(), t.cpu().numpy(), 6))
+    keep = [0, 1, 3]
+    got = r.top_logprobs.double().cpu().numpy()[keep]
+    assert np.array_equal(r.top_tokens.cpu().numpy()[keep], order)
+    assert np.allclose(r.logprob.double().cpu().numpy()[keep], lp, rtol=1e-6, atol=1e-5) and np.allclose(r.entropy.double().cpu().numpy()[keep], ent, atol=1e-5)
+    assert np.allclose(got, tl, rtol=1e-6, atol=1e-5)
+    assert r.logprob[2] == -float("inf") and r.entropy[2] == 0 and (r.top_logprobs[2] == -float("inf")).all() and r.top_tokens[2].tolist() == list(range(6))
+
+
+@pytest.mark.parametrize("what", [float("nan"), float("inf")])
+@pytest.mark.parametrize("vocab,at", [(40, 3), (30000, 0), (30000, 29999)])
+def test_rows_with_numbers_that_are_not_finite(what, vocab, at):
+    x = torch.randn(3, vocab, device=DEV)
+    clean = token_logprobs(x, torch.zeros(3, device=DEV, dtype=torch.int32), 4)
+    x[1, at] = what
+    r = token_logprobs(x, torch.zeros(3, device=DEV, dtype=torch.int32), 4)
+    assert r.entropy[1].isnan() and r.top_tokens[1, 0] == at
+    assert r.logprob[1].isnan() or (what > 0 and at != 0)
+    for a, b in ((clean.logprob, r.logprob), (clean.entropy, r.entropy), (clean.top_tokens, r.top_tokens), (clean.top_logprobs, r.top_logprobs)):
+        assert torch.equal(a[[0, 2]], b[[0, 2]])
+
+
+def test_tokens_that_are_none_and_beyond():
+    x = torch.randn(3, 100, device=DEV)
+    r = token_logprobs(x, torch.tensor([-1, -100, 5], device=DEV))
+    assert r.logprob[0] == 0 and r.logprob[1] == 0 and r.top_tokens is None
+    api.gpu_backend().device_status()
+    r = token_logprobs(x, torch.tensor([100, 2 ** 40, 5], device=DEV))
+    assert r.logprob[0].isnan() and r.logprob[1].isnan() and r.logprob[2].isfinite()
+    with pytest.raises(api.InvalidArgument):
+        api.gpu_backend().device_status()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_rows_that_lie_apart_or_off_their_boundaries(dtype):
+    base = (torch.randn(6, 5003, device=DEV) * 2).to(dtype)
+    t = torch.tensor([1, 2, 3, 4, 5, 6], device=DEV)
+    for lo, hi in ((1, 5003), (3, 4100), (7, 4999), (0, 5003)):
+        check(base[:, lo:hi], t, 9)
+    check(base.t().contiguous().t(), t, 9)
+    check(base[:1].expand(6, 5003), t, 3)
+    check(base[::2], t[:3], 3)
+    check(base.half() if dtype == torch.float32 else base.double(), t, 3)
+
+
+def test_the_same_bits_every_time_and_on_another_stream():
+    x = torch.randn(3, 60000, device=DEV)
+    t = torch.tensor([5, 6, 7], device=DEV, dtype=torch.int32)
+    want = token_logprobs(x, t, 32)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=s):
+            got = token_logprobs(x, t, 32)
+        for _ in range(5):
+            g.replay()
+    torch.cuda.synchronize()
+    for name in ("logprob", "entropy", "top_tokens", "top_logprobs"):
+        assert torch.equal(getattr(want, name), getattr(got, name))
+
+
+def test_many_rows():
+    check(torch.randn(70001, 33, device=DEV), torch.zeros(70001, device=DEV, dtype=torch.int32), 3)
+
+
+def test_wrong_tensors_are_refused():
+    x, t = torch.zeros(2, 10, device=DEV), torch.zeros(2, device=DEV, dtype=torch.int32)
+    for args in ((x[0], t), (x, t[:1]), (x.cpu(), t), (x, t.cpu()), (x, t, 11), (x, t, -1), (torch.zeros(2, 100, device=DEV), t, 33)):
+        with pytest.raises(api.TensorError):
+            token_logprobs(*args)
+    assert token_logprobs(x[:0], t[:0], 2).top_tokens.shape == (0, 2)
