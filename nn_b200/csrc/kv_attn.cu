@@ -27,6 +27,7 @@ namespace nnq {
 
 constexpr int kKvWarps = 8, kKvCols = 8, kKvStep = 16;
 constexpr int kKvMinSteps = 2 * kKvWarps;   // of a CTA's part
+constexpr int kFew = 32;   // see nnq_kv_attention
 constexpr int kNothing = INT32_MIN;   // in place of a block: no key of the step is seen
 constexpr float kKvLog2E = 1.4426950408889634f;
 constexpr float kKvSlack = 8.0f;   // a score may pass the reference by this power of two: weights up to 256 in f16
@@ -42,7 +43,7 @@ struct KvPlan {
 
 // Steps of an item of the request (the same for all its heads and vectors), and its items of one head.
 __device__ __forceinline__ int64_t item_steps(const KvAttn &a, const KvRequest &q) {
-    if (q.rows == 0) return 0;
+    if (q.rows == 0 || q.rows * a.group > a.few) return 0;
     const int64_t lo = row_first(a, max(row_pos(q, 0), (int64_t)0)), steps = ((q.length + kKvStep - 1) / kKvStep) - lo / kKvStep;
     return max(steps, (int64_t)1);
 }
@@ -263,17 +264,27 @@ __global__ void __launch_bounds__(kKvWarps * 32, D <= 128 ? 2 : 1) kv_attn_kerne
             load_step<D>(a, blk1, key_of(s + kKvWarps), head, lane, next);
             if (now.there) {
                 // ---- scores
-                float sc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                // (sums of 32 dimensions each: the tensor core cuts off what its f32 sums cannot hold, and long chains of that lean one way)
+                float part[D / 32][4];
 #pragma unroll
                 for (int c = 0; c < D / 64; c++) {
+#pragma unroll
+                    for (int e = 0; e < 8; e++) part[2 * c + (e >> 2)][e & 3] = 0.0f;
                     const uint32_t r0[4] = {now.k[0][c].x, now.k[0][c].y, now.k[0][c].z, now.k[0][c].w}, r1[4] = {now.k[1][c].x, now.k[1][c].y, now.k[1][c].z, now.k[1][c].w};
 #pragma unroll
                     for (int j = 0; j < 4; j++) {
                         const uint32_t u = Codes::word(r0[j]), w = Codes::word(r1[j]);
                         const uint32_t x[4] = {Codes::low(u), Codes::low(w), Codes::high(u), Codes::high(w)};
-                        if constexpr (QT == 2) mma_f16(sc, x, ql[4 * c + j][0], ql[4 * c + j][1]);
-                        mma_f16(sc, x, qh[4 * c + j][0], qh[4 * c + j][1]);
+                        if constexpr (QT == 2) mma_f16(part[2 * c + (j >> 1)], x, ql[4 * c + j][0], ql[4 * c + j][1]);
+                        mma_f16(part[2 * c + (j >> 1)], x, qh[4 * c + j][0], qh[4 * c + j][1]);
                     }
+                }
+                float sc[4];
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    sc[i] = part[0][i] + part[1][i];
+#pragma unroll
+                    for (int c = 1; c < D / 64; c++) sc[i] += part[2 * c][i] + part[2 * c + 1][i];
                 }
                 const float kf = pow2_byte(now.ke), ve = (float)(now.ve - 127);
                 const int64_t key0 = key_of(s);
@@ -504,7 +515,7 @@ nnq_status nnq_kv_attention_workspace(nnq_ctx *ctx, const nnq_kv_cache *c, const
     if (!bytes) return fail(ctx, NNQ_ERR_INVALID_ARG, "NULL result");
     nnq_status s = check_batch(ctx, c, b, heads);
     if (s != NNQ_OK) return s;
-    *bytes = (size_t)kv_parts(ctx, c->dim) * 2 * kKvCols * kv_record_floats(c->dim) * 4;
+    *bytes = std::max((size_t)kv_parts(ctx, c->dim) * 2 * kKvCols * kv_record_floats(c->dim) * 4, kv_attn_tc_workspace(ctx, c->dim));
     return NNQ_OK;
 }
 
@@ -526,8 +537,14 @@ nnq_status nnq_kv_attention(nnq_ctx *ctx, const nnq_kv_cache *c, const nnq_kv_ba
     if (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15u))
         return fail(ctx, NNQ_ERR_INVALID_ARG, "the workspace must be %zu bytes, 16-byte aligned (got %zu)", need, workspace ? workspace_bytes : (size_t)0);
     if ((s = check_cuda(ctx, cudaSetDevice(ctx->device), "cudaSetDevice")) != NNQ_OK) return s;
-    const KvAttn a = {(const uint8_t *)c->k, (const uint8_t *)c->v, c->k_exp, c->v_exp, b->length, b->row_start, b->table, q_dev, y_dev, c->blocks, b->table_ld, b->requests, q_ld, y_ld, b->rows,
-                      c->kv_heads, heads / c->kv_heads, c->dim, log2_of(c->block), window, (int)q_dt, (int)y_dt, scale, ctx->d_status};
+    KvAttn a = {(const uint8_t *)c->k, (const uint8_t *)c->v, c->k_exp, c->v_exp, b->length, b->row_start, b->table, q_dev, y_dev, c->blocks, b->table_ld, b->requests, q_ld, y_ld, b->rows,
+                      c->kv_heads, heads / c->kv_heads, c->dim, log2_of(c->block), window, (int)q_dt, (int)y_dt, INT32_MAX, scale, ctx->d_status};
+    // Requests of more than kFew query vectors per key / value head go to the tensor-core kernel where there can be any; the rest of the
+    // batch, down to single tokens beside a prompt, to this file's.
+    if (kv_attn_tc_supported(a) && b->max_rows > kFew / a.group) {
+        a.few = b->requests == 1 ? 0 : kFew;   // (a request alone is a prompt)
+        if ((s = launch_kv_attn_tc(ctx, a, c->format, (float *)workspace, (cudaStream_t)stream)) != NNQ_OK || a.few == 0) return s;
+    }
     return c->format == NNQ_KV_INT8 ? launch_kv_attn<NNQ_KV_INT8>(ctx, a, (float *)workspace, (cudaStream_t)stream)
                                     : launch_kv_attn<NNQ_KV_E4M3>(ctx, a, (float *)workspace, (cudaStream_t)stream);
 }

@@ -12,6 +12,7 @@ struct KvAttn {
     int64_t blocks, table_ld, requests, q_ld, y_ld, rows;
     int kv_heads, group, dim, shift, window;   // window 0: every earlier position
     int q_dt, y_dt;
+    int few;   // query vectors of a request and key / value head up to which kv_attn_kernel takes it; beyond: kv_attn_tc_kernel
     float scale;
     int *status;
 };
@@ -81,5 +82,10 @@ __device__ __forceinline__ void kv_split(float x, float y, uint32_t &hi, uint32_
     hi = half_bits(h);
     lo = half_bits(__floats2half2_rn(x - f.x, y - f.y));
 }
+
+// kv_attn_tc.cu: requests of more than a.few query vectors per key / value head
+bool kv_attn_tc_supported(const KvAttn &a);
+size_t kv_attn_tc_workspace(nnq_ctx *ctx, int dim);
+nnq_status launch_kv_attn_tc(nnq_ctx *ctx, const KvAttn &a, int fmt, float *records, cudaStream_t st);
 
 }  // namespace nnq
