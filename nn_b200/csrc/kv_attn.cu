@@ -4,10 +4,11 @@
 //   y = sum_j p_j v_j / sum_j p_j,  p_j = exp(scale q . k_j - m),  over the positions that a row sees.
 //
 // What bounds it is the reading of the cache, 2 dim bytes per key and head once for all query heads of the group. The codes go from
-// global memory to the operand registers of mma.sync (m16n8k16, f16) without a stop in shared memory:
+// global memory by cp.async into a ring of a warp's own, two steps of 16 keys ahead of the one that is worked on (128 KB under way on an
+// SM), and from there as bytes into the operand registers of mma.sync (m16n8k16, f16):
 //   scores   S^T [16 keys x 8 vectors] = K [16 x dim] Q^T: lane (g, t) of a warp reads 16 bytes of keys g and g + 8 at a time; which
 //            dimension stands at which place of k is free as long as the queries agree.
-//   values   O^T [dim x 8 vectors] += V^T [dim x 16 keys] P^T: lane (g, t) reads dim / 8 neighbouring bytes of the four keys whose
+//   values   O^T [dim x 8 vectors] += V^T [dim x 16 keys] P^T: lane (g, t) reads 8 neighbouring bytes of the four keys whose
 //            weights it holds, and a byte permutation puts two keys of a dimension side by side; the weights are turned by movmatrix.
 // Keys as the 16 rows waste none of the tensor core on missing query vectors. Codes are exact in f16; a query vector enters under a
 // power of two (one f16 term for bf16 queries, which is exact; two for f32), weights as two f16 terms (22 bits), so that scores, sums
@@ -17,90 +18,110 @@
 // in place of the maxima's exchange.
 //
 // Work is dealt in steps of 16 keys: all steps of all (request, head, vectors) items in one row, cut into equal parts, one for each
-// CTA, whatever the requests' lengths are. An item inside one part is written directly; of an item that is cut every part leaves a
-// record (m, mv, l, O), and kv_join_kernel joins them in their order.
+// CTA, whatever the requests' lengths are. An item counts kKvPad steps more than it has, about what beginning and ending one takes, so
+// that many short requests in one part weigh what they cost. An item inside one part is written directly; of an item that is cut every part
+// leaves a record (m, mv, l, O), and kv_join_kernel joins them in their order.
 #include <algorithm>
 
 #include "kv_attn.cuh"
+#include "sync.cuh"
 
 namespace nnq {
 
-constexpr int kKvWarps = 8, kKvCols = 8, kKvStep = 16;
-constexpr int kKvMinSteps = 2 * kKvWarps;   // of a CTA's part
+constexpr int kKvWarps = 8, kKvCols = 8, kKvStep = 16, kKvStages = 3;
+constexpr int kKvMinSteps = kKvWarps;   // of a CTA's part
+constexpr int kKvPad = 16;
 constexpr int kFew = 32;   // see nnq_kv_attention
 constexpr int kNothing = INT32_MIN;   // in place of a block: no key of the step is seen
 constexpr float kKvLog2E = 1.4426950408889634f;
 constexpr float kKvSlack = 8.0f;   // a score may pass the reference by this power of two: weights up to 256 in f16
 
-// records: [part][began before, begins here][column]: m, mv, l, unused, then O[dim]
+// records: [part][began before, begins here][column]: m, mv, l, unused, then O[dim]; behind them what every part has to join
 __host__ __device__ inline int kv_record_floats(int dim) { return 4 + dim; }
+struct KvJoin {
+    int first;   // part that the item begins in, -1: nothing to join
+    int vecs, group_row, head;   // vectors; first vector of the item as (row of q, query head)
+    int rest;    // number of the first vector within its row's group
+    int unused[3];
+};
 
 struct KvPlan {
     int64_t total, chunk;   // steps in all, steps of a part
-    int64_t r;              // request of the first step of this part
-    int64_t off;            // and the step's number within the request
+    int64_t off;            // number within its request of the part's first step
+    int r;                  // its request
 };
 
 // Steps of an item of the request (the same for all its heads and vectors), and its items of one head.
-__device__ __forceinline__ int64_t item_steps(const KvAttn &a, const KvRequest &q) {
+__device__ __forceinline__ int item_steps(const KvAttn &a, const KvRequest &q) {
     if (q.rows == 0 || q.rows * a.group > a.few) return 0;
-    const int64_t lo = row_first(a, max(row_pos(q, 0), (int64_t)0)), steps = ((q.length + kKvStep - 1) / kKvStep) - lo / kKvStep;
-    return max(steps, (int64_t)1);
+    const int lo = row_first(a, max(row_pos(q, 0), 0)), steps = (q.length + kKvStep - 1) / kKvStep - lo / kKvStep;
+    return max(steps, 1) + kKvPad;
 }
-__device__ __forceinline__ int64_t item_count(const KvAttn &a, const KvRequest &q) { return ((int64_t)q.rows * a.group + kKvCols - 1) / kKvCols; }
+__device__ __forceinline__ int item_count(const KvAttn &a, const KvRequest &q) { return (q.rows * a.group + kKvCols - 1) / kKvCols; }
 
-__device__ __forceinline__ int64_t block_scan(int64_t &v, int64_t *warp_sums) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
-    long long x = v;
-#pragma unroll
-    for (int off = 1; off < 32; off <<= 1) {
-        const long long b = __shfl_up_sync(0xFFFFFFFFu, x, off);
-        if (lane >= off) x += b;
-    }
-    __syncthreads();
-    if (lane == 31) warp_sums[warp] = x;
-    __syncthreads();
-    int64_t before = 0, all = 0;
-    for (int w = 0; w < nw; w++) {
-        if (w == warp) before = all;
-        all += warp_sums[w];
-    }
-    v = before + x - v;
-    return all;
-}
-
-// Every CTA sums the steps of all requests (twice, where there are more requests than threads) and finds where its part begins.
+// Sums the steps of all requests and finds where this CTA's part begins. Up to 32 requests every warp does so for itself, without a
+// barrier; more are summed by the whole CTA, twice.
 __device__ KvPlan kv_plan(const KvAttn &a, int parts) {
     __shared__ int64_t warp_sums[32], found[2];
-    const int nt = blockDim.x, tid = threadIdx.x;
+    const int nt = blockDim.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, nw = nt >> 5;
     auto steps_of = [&](int64_t r) -> int64_t {
         if (r >= a.requests) return 0;
         const KvRequest q = kv_request(a, r);
-        return item_steps(a, q) * item_count(a, q) * a.kv_heads;
+        return (int64_t)item_steps(a, q) * item_count(a, q) * a.kv_heads;
+    };
+    auto scan = [&](long long x) {
+#pragma unroll
+        for (int off = 1; off < 32; off <<= 1) {
+            const long long b = __shfl_up_sync(0xFFFFFFFFu, x, off);
+            if (lane >= off) x += b;
+        }
+        return x;
     };
     KvPlan p;
-    p.total = 0;
-    for (int64_t r0 = 0; r0 < a.requests; r0 += nt) {
-        int64_t v = steps_of(r0 + tid);
-        p.total += block_scan(v, warp_sums);
+    p.r = 0;
+    p.off = 0;
+    if (a.requests <= 32) {
+        const int64_t mine = steps_of(lane), upto = scan(mine);
+        p.total = __shfl_sync(0xFFFFFFFFu, (long long)upto, 31);
+        p.chunk = max((p.total + parts - 1) / parts, (int64_t)kKvMinSteps);
+        const int64_t begin = p.chunk * blockIdx.x;
+        const uint32_t m = __ballot_sync(0xFFFFFFFFu, begin >= upto - mine && begin < upto);
+        if (m) {
+            p.r = __ffs(m) - 1;
+            p.off = begin - __shfl_sync(0xFFFFFFFFu, (long long)(upto - mine), p.r);
+        }
+        return p;
     }
+    auto block_scan = [&](int64_t mine, int64_t &before) {
+        const int64_t x = scan(mine);
+        __syncthreads();
+        if (lane == 31) warp_sums[warp] = x;
+        __syncthreads();
+        int64_t all = 0;
+        before = x - mine;
+        for (int w = 0; w < nw; w++) {
+            if (w < warp) before += warp_sums[w];
+            all += warp_sums[w];
+        }
+        return all;
+    };
+    p.total = 0;
+    int64_t before;
+    for (int64_t r0 = 0; r0 < a.requests; r0 += nt) p.total += block_scan(steps_of(r0 + tid), before);
     p.chunk = max((p.total + parts - 1) / parts, (int64_t)kKvMinSteps);
     const int64_t begin = p.chunk * blockIdx.x;
-    p.r = p.off = 0;
     if (begin >= p.total) return p;
     int64_t done = 0;
     for (int64_t r0 = 0; r0 < a.requests && done <= begin; r0 += nt) {
-        const int64_t mine = steps_of(r0 + tid);
-        int64_t v = mine;
-        const int64_t all = block_scan(v, warp_sums);
-        if (begin >= done + v && begin < done + v + mine) {
+        const int64_t mine = steps_of(r0 + tid), all = block_scan(mine, before);
+        if (begin >= done + before && begin < done + before + mine) {
             found[0] = r0 + tid;
-            found[1] = begin - done - v;
+            found[1] = begin - done - before;
         }
         done += all;
     }
     __syncthreads();
-    p.r = found[0];
+    p.r = (int)found[0];
     p.off = found[1];
     return p;
 }
@@ -114,92 +135,134 @@ __device__ __forceinline__ uint32_t turn8x8(uint32_t v) {
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
     return r;
 }
+__device__ __forceinline__ void copy16(uint32_t dst, const void *src) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory"); }
+__device__ __forceinline__ uint4 lds128(uint32_t p) {
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(p) : "memory");
+    return v;
+}
+__device__ __forceinline__ uint2 lds64(uint32_t p) {
+    uint2 v;
+    asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(p) : "memory");
+    return v;
+}
 
-// Codes of 16 keys as a lane holds them, and the scales of their block.
-template <int D>
-struct KvStepData {
-    uint4 k[2][D / 64];
-    uint2 v[4][D / 64];
-    int ke, ve;
-    bool there;   // false: the table has no such block
-};
+// A step in the ring: keys, then values, in pieces of 64 dimensions: 16 rows of 64 bytes, two to a line of 128, whose eight 16-byte
+// chunks are exchanged by the line's number so that neither the copies nor the reads of either operand meet in a bank.
+__device__ __forceinline__ uint32_t chunk_at(int row, int c) { return (uint32_t)((row >> 1) * 128 + (((((row & 1) << 2) | c) ^ (((row >> 1) & 3) << 1)) << 4)); }
 
 template <int D>
-__device__ __forceinline__ void load_step(const KvAttn &a, int blk, int64_t key0, int head, int lane, KvStepData<D> &s) {
-    const int g = lane >> 2, t = lane & 3;
-    s.there = blk >= 0 && blk < a.blocks;
-    if (!s.there) return;
-    const int64_t bh = (int64_t)blk * a.kv_heads + head;
-    const int64_t at = ((bh << a.shift) + (key0 & ((1 << a.shift) - 1))) * D;
-    const uint8_t *kp = a.k + at + g * D + t * 16, *vp = a.v + at + 2 * t * D + g * (D / 8);
-#pragma unroll
-    for (int c = 0; c < D / 64; c++) {
-        s.k[0][c] = __ldg(reinterpret_cast<const uint4 *>(kp + c * 64));
-        s.k[1][c] = __ldg(reinterpret_cast<const uint4 *>(kp + 8 * D + c * 64));
-    }
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-        const uint8_t *p = vp + ((i & 1) + (i >> 1) * 8) * D;
-        if constexpr (D % 128 == 0) {
-#pragma unroll
-            for (int c = 0; c < D / 128; c++) {
-                const uint4 x = __ldg(reinterpret_cast<const uint4 *>(p) + c);
-                s.v[i][2 * c] = make_uint2(x.x, x.y);
-                s.v[i][2 * c + 1] = make_uint2(x.z, x.w);
-            }
-        } else {
-#pragma unroll
-            for (int c = 0; c < D / 64; c++) s.v[i][c] = __ldg(reinterpret_cast<const uint2 *>(p) + c);
-        }
-    }
-    s.ke = a.k_exp[bh];
-    s.ve = a.v_exp[bh];
+constexpr int kv_ring_bytes() { return kKvWarps * kKvStages * 2 * kKvStep * D; }
+template <int D>
+constexpr int kv_smem_bytes() {
+    const int merge = kKvWarps * kKvCols * (4 + D) * 4;
+    return kv_ring_bytes<D>() > merge ? kv_ring_bytes<D>() : merge;
+}
+
+__device__ __forceinline__ void store_out(const KvAttn &a, int64_t at, float y) {
+    if (a.y_dt == NNQ_F32) reinterpret_cast<float *>(a.y)[at] = y;
+    else reinterpret_cast<__nv_bfloat16 *>(a.y)[at] = __float2bfloat16_rn(y);
 }
 
 template <int FMT, int D, int QT>
-__global__ void __launch_bounds__(kKvWarps * 32, D <= 128 ? 2 : 1) kv_attn_kernel(const KvAttn a, float *records) {
-    extern __shared__ __align__(16) float sm[];   // a record of every warp and column
+__global__ void __launch_bounds__(kKvWarps * 32, D <= 128 ? 2 : 1) kv_attn_kernel(const KvAttn a, float *records, KvJoin *joins) {
+    extern __shared__ __align__(128) uint8_t kv_smem[];   // the warps' rings; at the end of an item a record of every warp and column
     typedef CodePairs<FMT> Codes;
-    constexpr int REC = 4 + D;
+    constexpr int REC = 4 + D, STEP = 2 * kKvStep * D;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
+    const uint32_t ring = smem_u32(kv_smem) + warp * kKvStages * STEP;
+    float *sm = reinterpret_cast<float *>(kv_smem);
     pdl_prologue();
+    pdl_release();
     const KvPlan plan = kv_plan(a, gridDim.x);
-    int64_t at = plan.chunk * blockIdx.x;
+    int64_t at = plan.chunk * blockIdx.x, off = plan.off;
     const int64_t end = min(plan.total, at + plan.chunk);
-    int64_t r = plan.r, off = plan.off;
+    int r = plan.r;
+    KvJoin join = {-1, 0, 0, 0, 0, {0, 0, 0}};
+    KvRequest rq;
+    int spi = 0, cols = 0;
+    int64_t of_request = -1;
     while (at < end) {
         // ---- the next request with steps left, the item and the part of it that is this CTA's
-        const KvRequest rq = kv_request(a, r);
-        const int64_t spi = item_steps(a, rq), cols = item_count(a, rq), of_request = spi * cols * a.kv_heads;
+        if (of_request < 0) {
+            rq = kv_request(a, r);
+            spi = item_steps(a, rq);
+            cols = item_count(a, rq);
+            of_request = (int64_t)spi * cols * a.kv_heads;
+        }
         if (off >= of_request) {
             off = 0;
             r++;
+            of_request = -1;
             continue;
         }
-        const int64_t item = off / spi, s0 = off - item * spi, s1 = min(spi, s0 + end - at);
-        const int head = (int)(item / cols), vec0 = (int)(item - (int64_t)head * cols) * kKvCols, vecs = min(kKvCols, rq.rows * a.group - vec0);
-        const int64_t lo_all = row_first(a, max(row_pos(rq, 0), (int64_t)0)) / kKvStep * kKvStep;   // the item's step 0 begins here
+        const int item = (int)(off / spi), v0 = (int)(off - (int64_t)item * spi), v1 = (int)min((int64_t)spi, v0 + end - at);   // steps, the padding first
+        const int s0 = max(v0 - kKvPad, 0), s1 = max(v1 - kKvPad, 0);
+        const int head = item / cols, vec0 = (item - head * cols) * kKvCols, vecs = min(kKvCols, rq.rows * a.group - vec0);
+        const int lo_all = row_first(a, max(row_pos(rq, 0), 0)) / kKvStep * kKvStep;   // the item's step 0 begins here
+        // positions of the first and the last vector's row; what every vector sees, and what some vector sees
+        const int first_pos = row_pos(rq, vec0 / a.group), last_pos = row_pos(rq, (vec0 + vecs - 1) / a.group);
+        const int lo_some = row_first(a, max(first_pos, 0)), lo_every = row_first(a, max(last_pos, 0));
+        const int n = s1 > s0 + warp ? (s1 - s0 - warp + kKvWarps - 1) / kKvWarps : 0;   // this warp's steps
+        const int32_t *table = a.table + (int64_t)r * a.table_ld;
+        const int key_base = lo_all + (s0 + warp) * kKvStep;
+        // lane i has the block of the warp's steps j with j mod 32 = i, and its exponent bytes, a batch of 32 at a time and one ahead
+        auto block_of = [&](int j) {
+            const int key = key_base + j * kKvWarps * kKvStep;
+            return j < n && key <= last_pos && key + kKvStep > lo_some ? table[key >> a.shift] : kNothing;
+        };
+        auto bytes_of = [&](int b, int &ke, int &ve) {
+            ke = ve = 127;
+            if (b >= 0 && b < a.blocks) {
+                ke = a.k_exp[(int64_t)b * a.kv_heads + head];
+                ve = a.v_exp[(int64_t)b * a.kv_heads + head];
+            } else if (b != kNothing) {
+                atomicExch(a.status, kStatusIndex);
+            }
+        };
+        auto fetch = [&](int j, int b) {
+            if (b >= 0 && b < a.blocks) {
+                const int key = key_base + j * kKvWarps * kKvStep;
+                const int64_t from = (((((int64_t)b * a.kv_heads + head) << a.shift) + (key & ((1 << a.shift) - 1))) + (lane >> 2)) * D + (lane & 3) * 16;
+                const uint8_t *kp = a.k + from, *vp = a.v + from;
+                const uint32_t dst = ring + (uint32_t)(j % kKvStages) * STEP + chunk_at(lane >> 2, lane & 3);
+#pragma unroll
+                for (int c = 0; c < D / 64; c++)
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        copy16(dst + c * 1024 + h * 512, kp + c * 64 + h * 8 * D);
+                        copy16(dst + kKvStep * D + c * 1024 + h * 512, vp + c * 64 + h * 8 * D);
+                    }
+            }
+            asm volatile("cp.async.commit_group;" ::: "memory");
+        };
+        __syncthreads();   // the records of the item before have been read
+        int blk = block_of(lane), ke, ve;
+        fetch(0, __shfl_sync(0xFFFFFFFFu, blk, 0));
+        fetch(1, __shfl_sync(0xFFFFFFFFu, blk, 1));
+        bytes_of(blk, ke, ve);
+        int blk1 = kNothing, ke1 = 127, ve1 = 127;
 
         // ---- queries: lane (g, t) has vector g's dimensions c * 64 + t * 16 .. + 15 of every c, as the scores' second operand
         uint32_t qh[D / 16][2], ql[QT == 2 ? D / 16 : 1][2];
         float q_un = 1.0f;
         {
             float x[D / 64][16];
-            const int v = vec0 + g, row = v / a.group, qhead = head * a.group + v % a.group;
+            const int v = vec0 + g, row = v / a.group, qhead = head * a.group + v - row * a.group;
+            const int64_t from = (int64_t)(rq.row0 + row) * a.q_ld + (int64_t)qhead * D + t * 16;
             uint32_t top = 0;
 #pragma unroll
             for (int c = 0; c < D / 64; c++)
 #pragma unroll
                 for (int i = 0; i < 16; i += 8) {
                     float y[8] = {};
-                    const int64_t from = (int64_t)(rq.row0 + row) * a.q_ld + (int64_t)qhead * D + c * 64 + t * 16 + i;
                     if (g < vecs) {
                         if constexpr (QT == 2) {
-                            const float4 u = __ldg(reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(a.q) + from));
-                            const float4 w = __ldg(reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(a.q) + from) + 1);
+                            const float4 *p = reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(a.q) + from + c * 64 + i);
+                            const float4 u = __ldg(p), w = __ldg(p + 1);
                             y[0] = u.x; y[1] = u.y; y[2] = u.z; y[3] = u.w; y[4] = w.x; y[5] = w.y; y[6] = w.z; y[7] = w.w;
                         } else {
-                            const uint4 u = __ldg(reinterpret_cast<const uint4 *>(reinterpret_cast<const __nv_bfloat16 *>(a.q) + from));
+                            const uint4 u = __ldg(reinterpret_cast<const uint4 *>(reinterpret_cast<const __nv_bfloat16 *>(a.q) + from + c * 64 + i));
                             const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
                             for (int e = 0; e < 4; e++) {
@@ -232,17 +295,13 @@ __global__ void __launch_bounds__(kKvWarps * 32, D <= 128 ? 2 : 1) kv_attn_kerne
         }
         // this lane's two columns of the scores are vectors 2t and 2t + 1: factor, position and first position seen
         float fac[2];
-        int64_t pos[2], low[2];
+        int pos[2], low[2];
 #pragma unroll
         for (int j = 0; j < 2; j++) {
             fac[j] = a.scale * kKvLog2E * Codes::unscale * __shfl_sync(0xFFFFFFFFu, q_un, (2 * t + j) * 4);
-            const int v = min(2 * t + j, vecs - 1);
-            pos[j] = row_pos(rq, (vec0 + v) / a.group);
+            pos[j] = row_pos(rq, (vec0 + min(2 * t + j, vecs - 1)) / a.group);
             low[j] = row_first(a, pos[j]);
         }
-        // positions that every vector sees, and that some vector sees
-        const int64_t first_pos = row_pos(rq, vec0 / a.group), last_pos = row_pos(rq, (vec0 + vecs - 1) / a.group);
-        const int64_t lo_some = row_first(a, max(first_pos, (int64_t)0)), lo_every = row_first(a, max(last_pos, (int64_t)0));
 
         float acc[D / 16][4];
 #pragma unroll
@@ -250,19 +309,25 @@ __global__ void __launch_bounds__(kKvWarps * 32, D <= 128 ? 2 : 1) kv_attn_kerne
 #pragma unroll
             for (int j = 0; j < 4; j++) acc[i][j] = 0.0f;
         float m[2] = {0.0f, 0.0f}, mv[2] = {0.0f, 0.0f}, l[2] = {0.0f, 0.0f};
-        float thr[2] = {-INFINITY, -INFINITY}, thv[2] = {-INFINITY, -INFINITY};   // references and what makes them move
+        float thr[2] = {-INFINITY, -INFINITY}, thv[2] = {-INFINITY, -INFINITY};   // what makes the references move
 
-        const int32_t *table = a.table + r * a.table_ld;
-        auto key_of = [&](int64_t s) { return lo_all + s * kKvStep; };
-        auto wanted = [&](int64_t s) { return s < s1 && key_of(s) <= last_pos && key_of(s) + kKvStep > lo_some; };
-        auto block_of = [&](int64_t s) { return wanted(s) ? table[key_of(s) >> a.shift] : kNothing; };
-        KvStepData<D> now, next;
-        int blk = block_of(s0 + warp), blk1 = block_of(s0 + warp + kKvWarps);
-        load_step<D>(a, blk, key_of(s0 + warp), head, lane, now);
-        for (int64_t s = s0 + warp; s < s1; s += kKvWarps) {
-            const int blk2 = block_of(s + 2 * kKvWarps);
-            load_step<D>(a, blk1, key_of(s + kKvWarps), head, lane, next);
-            if (now.there) {
+        for (int j = 0; j < n; j++) {
+            if ((j & 31) == 0) {
+                if (j) {
+                    blk = blk1;
+                    ke = ke1;
+                    ve = ve1;
+                }
+                blk1 = n > j + 32 ? block_of(j + 32 + lane) : kNothing;
+            }
+            if ((j & 31) == 16 && n > (j | 31)) bytes_of(blk1, ke1, ve1);
+            fetch(j + 2, __shfl_sync(0xFFFFFFFFu, (j & 31) < 30 ? blk : blk1, (j + 2) & 31));
+            const int b = __shfl_sync(0xFFFFFFFFu, blk, j & 31);
+            const float kf = pow2_byte(__shfl_sync(0xFFFFFFFFu, ke, j & 31)), vexp = (float)(__shfl_sync(0xFFFFFFFFu, ve, j & 31) - 127);
+            asm volatile("cp.async.wait_group 2;" ::: "memory");
+            __syncwarp();
+            if (b >= 0 && b < a.blocks) {
+                const uint32_t k_s = ring + (uint32_t)(j % kKvStages) * STEP, v_s = k_s + kKvStep * D;
                 // ---- scores
                 // (sums of 32 dimensions each: the tensor core cuts off what its f32 sums cannot hold, and long chains of that lean one way)
                 float part[D / 32][4];
@@ -270,13 +335,14 @@ __global__ void __launch_bounds__(kKvWarps * 32, D <= 128 ? 2 : 1) kv_attn_kerne
                 for (int c = 0; c < D / 64; c++) {
 #pragma unroll
                     for (int e = 0; e < 8; e++) part[2 * c + (e >> 2)][e & 3] = 0.0f;
-                    const uint32_t r0[4] = {now.k[0][c].x, now.k[0][c].y, now.k[0][c].z, now.k[0][c].w}, r1[4] = {now.k[1][c].x, now.k[1][c].y, now.k[1][c].z, now.k[1][c].w};
+                    const uint4 u0 = lds128(k_s + c * 1024 + chunk_at(g, t)), u1 = lds128(k_s + c * 1024 + 512 + chunk_at(g, t));
+                    const uint32_t r0[4] = {u0.x, u0.y, u0.z, u0.w}, r1[4] = {u1.x, u1.y, u1.z, u1.w};
 #pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        const uint32_t u = Codes::word(r0[j]), w = Codes::word(r1[j]);
+                    for (int i = 0; i < 4; i++) {
+                        const uint32_t u = Codes::word(r0[i]), w = Codes::word(r1[i]);
                         const uint32_t x[4] = {Codes::low(u), Codes::low(w), Codes::high(u), Codes::high(w)};
-                        if constexpr (QT == 2) mma_f16(part[2 * c + (j >> 1)], x, ql[4 * c + j][0], ql[4 * c + j][1]);
-                        mma_f16(part[2 * c + (j >> 1)], x, qh[4 * c + j][0], qh[4 * c + j][1]);
+                        if constexpr (QT == 2) mma_f16(part[2 * c + (i >> 1)], x, ql[4 * c + i][0], ql[4 * c + i][1]);
+                        mma_f16(part[2 * c + (i >> 1)], x, qh[4 * c + i][0], qh[4 * c + i][1]);
                     }
                 }
                 float sc[4];
@@ -285,43 +351,40 @@ __global__ void __launch_bounds__(kKvWarps * 32, D <= 128 ? 2 : 1) kv_attn_kerne
                     sc[i] = part[0][i] + part[1][i];
 #pragma unroll
                     for (int c = 1; c < D / 64; c++) sc[i] += part[2 * c][i] + part[2 * c + 1][i];
+                    sc[i] *= fac[i & 1] * kf;
                 }
-                const float kf = pow2_byte(now.ke), ve = (float)(now.ve - 127);
-                const int64_t key0 = key_of(s);
-#pragma unroll
-                for (int i = 0; i < 4; i++) sc[i] = sc[i] * kf * fac[i & 1];
+                const int key0 = key_base + j * kKvWarps * kKvStep;
                 if (key0 + kKvStep - 1 > first_pos || key0 < lo_every) {   // (the same for the whole warp)
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
-                        const int64_t j = key0 + g + (i >> 1) * 8;
-                        if (j > pos[i & 1] || j < low[i & 1]) sc[i] = -INFINITY;
+                        const int k = key0 + g + (i >> 1) * 8;
+                        if (k > pos[i & 1] || k < low[i & 1]) sc[i] = -INFINITY;
                     }
                 }
                 // ---- references
-                const float big0 = fmaxf(sc[0], sc[2]), big1 = fmaxf(sc[1], sc[3]);
-                if (__any_sync(0xFFFFFFFFu, big0 > thr[0] || big1 > thr[1] || big0 + ve > thv[0] || big1 + ve > thv[1])) {
-                    float b[2] = {big0, big1};
+                float big[2] = {fmaxf(sc[0], sc[2]), fmaxf(sc[1], sc[3])};
+                if (__any_sync(0xFFFFFFFFu, big[0] > thr[0] || big[1] > thr[1] || big[0] + vexp > thv[0] || big[1] + vexp > thv[1])) {
 #pragma unroll
                     for (int o = 4; o < 32; o <<= 1) {
-                        b[0] = fmaxf(b[0], __shfl_xor_sync(0xFFFFFFFFu, b[0], o));
-                        b[1] = fmaxf(b[1], __shfl_xor_sync(0xFFFFFFFFu, b[1], o));
+                        big[0] = fmaxf(big[0], __shfl_xor_sync(0xFFFFFFFFu, big[0], o));
+                        big[1] = fmaxf(big[1], __shfl_xor_sync(0xFFFFFFFFu, big[1], o));
                     }
 #pragma unroll
-                    for (int j = 0; j < 2; j++) {
-                        if (b[j] == -INFINITY) continue;   // nothing seen yet or here
-                        const bool none = thr[j] == -INFINITY;   // a first reference: the sums are zero
-                        const float mn = none ? b[j] : fmaxf(m[j], b[j]), vn = none ? b[j] + ve : fmaxf(mv[j], b[j] + ve);
-                        const float f = none ? 1.0f : exp2f(mv[j] - vn);
-                        l[j] *= none ? 1.0f : exp2f(m[j] - mn);
+                    for (int i = 0; i < 2; i++) {
+                        if (big[i] == -INFINITY) continue;   // nothing seen yet or here
+                        const bool none = thr[i] == -INFINITY;   // a first reference: the sums are zero
+                        const float mn = none ? big[i] : fmaxf(m[i], big[i]), vn = none ? big[i] + vexp : fmaxf(mv[i], big[i] + vexp);
+                        const float f = none ? 1.0f : kv_ex2(mv[i] - vn);
+                        l[i] *= none ? 1.0f : kv_ex2(m[i] - mn);
 #pragma unroll
-                        for (int i = 0; i < D / 16; i++) {
-                            acc[i][j] *= f;
-                            acc[i][j + 2] *= f;
+                        for (int k = 0; k < D / 16; k++) {
+                            acc[k][i] *= f;
+                            acc[k][i + 2] *= f;
                         }
-                        m[j] = mn;
-                        mv[j] = vn;
-                        thr[j] = mn + kKvSlack;
-                        thv[j] = vn + kKvSlack;
+                        m[i] = mn;
+                        mv[i] = vn;
+                        thr[i] = mn + kKvSlack;
+                        thv[i] = vn + kKvSlack;
                     }
                 }
                 // ---- weights
@@ -329,7 +392,7 @@ __global__ void __launch_bounds__(kKvWarps * 32, D <= 128 ? 2 : 1) kv_attn_kerne
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
                     l[i & 1] += kv_ex2(sc[i] - m[i & 1]);
-                    w[i] = kv_ex2(sc[i] + (ve - mv[i & 1]));
+                    w[i] = kv_ex2(sc[i] + (vexp - mv[i & 1]));
                 }
                 uint32_t h0, l0, h1, l1;
                 kv_split(w[0], w[1], h0, l0);
@@ -340,141 +403,172 @@ __global__ void __launch_bounds__(kKvWarps * 32, D <= 128 ? 2 : 1) kv_attn_kerne
                 l1 = turn8x8(l1);
                 // ---- values: 8 dimensions (four MMA rows each of g and g + 8) per two words of four keys
 #pragma unroll
-                for (int c = 0; c < D / 64; c++)
+                for (int c = 0; c < D / 64; c++) {
+                    const uint32_t p = v_s + c * 1024 + (g & 1) * 8, even = p + chunk_at(2 * t, g >> 1), odd = p + chunk_at(2 * t + 1, g >> 1);
+                    const uint2 y0 = lds64(even), y1 = lds64(odd), y2 = lds64(even + 512), y3 = lds64(odd + 512);
 #pragma unroll
                     for (int hw = 0; hw < 2; hw++) {
-                        const uint32_t k0 = Codes::word(hw ? now.v[0][c].y : now.v[0][c].x), k1 = Codes::word(hw ? now.v[1][c].y : now.v[1][c].x);
-                        const uint32_t k2 = Codes::word(hw ? now.v[2][c].y : now.v[2][c].x), k3 = Codes::word(hw ? now.v[3][c].y : now.v[3][c].x);
-                        const uint32_t a01 = __byte_perm(k0, k1, 0x5140), b01 = __byte_perm(k0, k1, 0x7362), a23 = __byte_perm(k2, k3, 0x5140), b23 = __byte_perm(k2, k3, 0x7362);
-                        const uint32_t x0[4] = {Codes::low(a01), Codes::high(a01), Codes::low(a23), Codes::high(a23)};
-                        const uint32_t x1[4] = {Codes::low(b01), Codes::high(b01), Codes::low(b23), Codes::high(b23)};
+                        uint32_t x0[4], x1[4];
+                        Codes::pairs(hw ? y0.y : y0.x, hw ? y1.y : y1.x, x0[0], x0[1], x1[0], x1[1]);
+                        Codes::pairs(hw ? y2.y : y2.x, hw ? y3.y : y3.x, x0[2], x0[3], x1[2], x1[3]);
                         mma_f16(acc[4 * c + 2 * hw], x0, l0, l1);
                         mma_f16(acc[4 * c + 2 * hw + 1], x1, l0, l1);
                         mma_f16(acc[4 * c + 2 * hw], x0, h0, h1);
                         mma_f16(acc[4 * c + 2 * hw + 1], x1, h0, h1);
                     }
-            } else if (blk != kNothing && lane == 0) {
-                atomicExch(a.status, kStatusIndex);
+                }
             }
-            now = next;
-            blk = blk1;
-            blk1 = blk2;
+            __syncwarp();   // the stage may be written again
         }
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
 
         // ---- the warps' sums in shared memory: a record per warp and column (m = -inf: nothing seen)
         __syncthreads();
-        {
-            float *mine = sm + warp * kKvCols * REC;
 #pragma unroll
-            for (int j = 0; j < 2; j++) {
+        for (int j = 0; j < 2; j++) {
 #pragma unroll
-                for (int o = 4; o < 32; o <<= 1) l[j] += __shfl_xor_sync(0xFFFFFFFFu, l[j], o);
-                float *rec = mine + (2 * t + j) * REC;
-                if (g == 0) {
-                    rec[0] = thr[j] > -INFINITY ? m[j] : (l[j] == 0.0f ? -INFINITY : l[j]);   // (scores that are all NaN move no reference)
-                    rec[1] = mv[j];
-                    rec[2] = l[j];
-                }
+            for (int o = 4; o < 32; o <<= 1) l[j] += __shfl_xor_sync(0xFFFFFFFFu, l[j], o);
+            if (2 * t + j >= vecs) continue;
+            float *rec = sm + (warp * kKvCols + 2 * t + j) * REC;
+            if (g == 0) {
+                rec[0] = thr[j] > -INFINITY ? m[j] : (l[j] == 0.0f ? -INFINITY : l[j]);   // (scores that are all NaN move no reference)
+                rec[1] = mv[j];
+                rec[2] = l[j];
+            }
+            if (thr[j] > -INFINITY) {
 #pragma unroll
-                for (int i = 0; i < D / 16; i++) {
-                    rec[4 + g * (D / 8) + 2 * i] = acc[i][j];
-                    rec[4 + g * (D / 8) + 2 * i + 1] = acc[i][j + 2];
-                }
+                for (int i = 0; i < D / 16; i += 2)
+                    *reinterpret_cast<float4 *>(rec + 4 + (i >> 2) * 64 + 8 * g + (i & 2) * 2) = make_float4(acc[i][j], acc[i][j + 2], acc[i + 1][j], acc[i + 1][j + 2]);
             }
         }
         __syncthreads();
-        const bool whole = s0 == 0 && s1 == spi;
+        const bool whole = v0 == 0 && v1 == spi;
         for (int u = tid; u < vecs * D; u += kKvWarps * 32) {
             const int col = u / D, d = u - col * D;
-            float mm = -INFINITY, mvv = -INFINITY;
+            float wm[kKvWarps], mm = -INFINITY, mvv = -INFINITY;
 #pragma unroll
             for (int w = 0; w < kKvWarps; w++) {
                 const float *rec = sm + (w * kKvCols + col) * REC;
-                if (rec[0] == -INFINITY) continue;
-                mm = fmaxf(mm, rec[0]);
-                mvv = fmaxf(mvv, rec[1]);
-                if (rec[0] != rec[0]) mm = mvv = rec[0];
+                wm[w] = rec[0];
+                mm = fmaxf(mm, wm[w]);
+                if (wm[w] != -INFINITY) mvv = fmaxf(mvv, rec[1]);
             }
             float ll = 0.0f, o = 0.0f;
 #pragma unroll
             for (int w = 0; w < kKvWarps; w++) {
                 const float *rec = sm + (w * kKvCols + col) * REC;
-                if (rec[0] == -INFINITY) continue;
-                ll += rec[2] * exp2f(rec[0] - mm);
-                o += rec[4 + d] * exp2f(rec[1] - mvv);
+                if (wm[w] == -INFINITY) continue;
+                ll += rec[2] * kv_ex2(wm[w] - mm);
+                o += rec[4 + d] * kv_ex2(rec[1] - mvv);
             }
             if (whole) {
-                const int v = vec0 + col;
-                const int64_t to = (int64_t)(rq.row0 + v / a.group) * a.y_ld + (int64_t)(head * a.group + v % a.group) * D + d;
-                // (the values' factor of e4m3 codes; exponents of both references are far inside the range)
-                const float y = mm == -INFINITY ? 0.0f : o * (exp2f(mvv - mm) * Codes::unscale) / ll;
-                if (a.y_dt == NNQ_F32) reinterpret_cast<float *>(a.y)[to] = y;
-                else reinterpret_cast<__nv_bfloat16 *>(a.y)[to] = __float2bfloat16_rn(y);
+                const int v = vec0 + col, row = v / a.group;
+                // (the values' factor of e4m3 codes; exponents of both references are far inside the range. No key seen: 0; NaN: l is)
+                const float y = ll == 0.0f ? 0.0f : o * (exp2f(mvv - mm) * Codes::unscale) / ll;
+                store_out(a, (int64_t)(rq.row0 + row) * a.y_ld + (int64_t)(head * a.group + v - row * a.group) * D + d, y);
             } else {
-                float *rec = records + (((int64_t)blockIdx.x * 2 + (s0 == 0 ? 1 : 0)) * kKvCols + col) * REC;
+                float *rec = records + (((int64_t)blockIdx.x * 2 + (v0 == 0 ? 1 : 0)) * kKvCols + col) * REC;
                 rec[4 + d] = o;
                 if (d == 0) {
-                    rec[0] = mm;
+                    rec[0] = ll == 0.0f ? -INFINITY : mm > -INFINITY ? mm : ll;   // (NaN where all scores are)
                     rec[1] = mvv;
                     rec[2] = ll;
                 }
             }
         }
-        at += s1 - s0;
-        off += s1 - s0;
+        if (!whole && v1 == spi) {
+            join.first = (int)((at - v0) / plan.chunk);
+            join.vecs = vecs;
+            join.group_row = rq.row0 + vec0 / a.group;
+            join.head = head;
+            join.rest = vec0 % a.group;
+        }
+        at += v1 - v0;
+        off += v1 - v0;
     }
+    if (tid == 0) joins[blockIdx.x] = join;
 }
 
-// Joins the records of the items that were cut: CTA (part, column) does so where the item at the part's beginning began before it and
-// ends in it.
+// Joins the records of an item that was cut: CTA (part that the item ends in, vector), the records dealt to eight warps.
 template <int FMT>
-__global__ void __launch_bounds__(256) kv_join_kernel(const KvAttn a, const float *records) {
+__global__ void __launch_bounds__(256) kv_join_kernel(const KvAttn a, const float *records, const KvJoin *joins) {
+    __shared__ float4 part[8][64];
+    __shared__ float2 part_l[8];
     pdl_prologue();
-    const KvPlan plan = kv_plan(a, gridDim.x);
-    const int64_t at = plan.chunk * blockIdx.x;
-    if (at >= plan.total) return;
-    const KvRequest rq = kv_request(a, plan.r);
-    const int64_t spi = item_steps(a, rq), cols = item_count(a, rq), item = plan.off / spi, s0 = plan.off - item * spi;
-    if (s0 == 0 || spi - s0 > plan.chunk) return;   // begins here, or reaches beyond this part
-    const int head = (int)(item / cols), vec0 = (int)(item - (int64_t)head * cols) * kKvCols, vecs = min(kKvCols, rq.rows * a.group - vec0);
-    const int col = blockIdx.y;
-    if (col >= vecs) return;
-    const int64_t first = (at - s0) / plan.chunk;   // the part that the item begins in
-    const int rec_floats = kv_record_floats(a.dim), d = threadIdx.x;
-    auto record = [&](int64_t p) { return records + ((p * 2 + (p == first ? 1 : 0)) * kKvCols + col) * rec_floats; };
-    float mm = -INFINITY, mvv = -INFINITY;
-    for (int64_t p = first; p <= blockIdx.x; p++) {
-        const float *rec = record(p);
-        if (rec[0] == -INFINITY) continue;
-        mm = fmaxf(mm, rec[0]);
-        mvv = fmaxf(mvv, rec[1]);
-        if (rec[0] != rec[0]) mm = mvv = rec[0];
+    const KvJoin j = joins[blockIdx.x];
+    const int col = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, quads = a.dim / 4, last = blockIdx.x;
+    if (j.first < 0 || col >= j.vecs) return;
+    const int rec_floats = kv_record_floats(a.dim);
+    auto record = [&](int p) { return records + ((int64_t)(p * 2 + (p == j.first ? 1 : 0)) * kKvCols + col) * rec_floats; };
+    // the references of all records, a lane per record and turn
+    float mm = -INFINITY, mv = -INFINITY;
+    for (int p = j.first + lane; p <= last; p += 32) {
+        const float4 h = *reinterpret_cast<const float4 *>(record(p));
+        if (h.x == -INFINITY) continue;
+        mm = fmaxf(mm, h.x);
+        mv = fmaxf(mv, h.y);
     }
-    if (d >= a.dim) return;
-    float ll = 0.0f, o = 0.0f;
-    for (int64_t p = first; p <= blockIdx.x; p++) {
-        const float *rec = record(p);
-        if (rec[0] == -INFINITY) continue;
-        ll += rec[2] * exp2f(rec[0] - mm);
-        o += rec[4 + d] * exp2f(rec[1] - mvv);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        mm = fmaxf(mm, __shfl_xor_sync(0xFFFFFFFFu, mm, o));
+        mv = fmaxf(mv, __shfl_xor_sync(0xFFFFFFFFu, mv, o));
     }
-    const int v = vec0 + col;
-    const int64_t to = (int64_t)(rq.row0 + v / a.group) * a.y_ld + (int64_t)(head * a.group + v % a.group) * a.dim + d;
-    const float y = mm == -INFINITY ? 0.0f : o * (exp2f(mvv - mm) * CodePairs<FMT>::unscale) / ll;
-    if (a.y_dt == NNQ_F32) reinterpret_cast<float *>(a.y)[to] = y;
-    else reinterpret_cast<__nv_bfloat16 *>(a.y)[to] = __float2bfloat16_rn(y);
+    float4 o[2] = {};
+    float l = 0.0f;
+#pragma unroll 4
+    for (int p = j.first + warp; p <= last; p += 8) {
+        const float *rec = record(p);
+        const float4 h = *reinterpret_cast<const float4 *>(rec);
+        if (h.x == -INFINITY) continue;
+        const float f = exp2f(h.y - mv);
+        l += h.z * exp2f(h.x - mm);
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            if (lane + 32 * i >= quads) continue;
+            const float4 x = reinterpret_cast<const float4 *>(rec + 4)[lane + 32 * i];
+            o[i].x += x.x * f;
+            o[i].y += x.y * f;
+            o[i].z += x.z * f;
+            o[i].w += x.w * f;
+        }
+    }
+    part[warp][lane] = o[0];
+    part[warp][lane + 32] = o[1];
+    if (lane == 0) part_l[warp] = make_float2(l, 0.0f);
+    __syncthreads();
+    const int q = threadIdx.x;
+    if (q >= quads) return;
+    float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    l = 0.0f;
+#pragma unroll
+    for (int w = 0; w < 8; w++) {
+        const float4 x = part[w][q];
+        s.x += x.x;
+        s.y += x.y;
+        s.z += x.z;
+        s.w += x.w;
+        l += part_l[w].x;
+    }
+    const float f = l == 0.0f ? 0.0f : exp2f(mv - mm) * CodePairs<FMT>::unscale / l;
+    const int v = j.rest + col, row = v / a.group;
+    const int64_t to = (int64_t)(j.group_row + row) * a.y_ld + (int64_t)(j.head * a.group + v - row * a.group) * a.dim + 4 * q;
+    const float y[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+    for (int i = 0; i < 4; i++) store_out(a, to + i, l == 0.0f ? 0.0f : y[i] * f);
 }
 
 static int kv_parts(nnq_ctx *ctx, int dim) { return (dim <= 128 ? 2 : 1) * ctx->sm_count; }
+static size_t kv_records_bytes(nnq_ctx *ctx, int dim) { return (size_t)kv_parts(ctx, dim) * 2 * kKvCols * kv_record_floats(dim) * 4; }
 
 template <int FMT, int D, int QT>
 static nnq_status launch_kv_attn(nnq_ctx *ctx, const KvAttn &a, float *records, cudaStream_t st) {
-    const size_t smem = (size_t)kKvWarps * kKvCols * kv_record_floats(D) * 4;
-    nnq_status s = check_cuda(ctx, cudaFuncSetAttribute(kv_attn_kernel<FMT, D, QT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem), "attention shared memory");
+    constexpr int smem = kv_smem_bytes<D>();
+    nnq_status s = check_cuda(ctx, cudaFuncSetAttribute(kv_attn_kernel<FMT, D, QT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), "attention shared memory");
     if (s != NNQ_OK) return s;
     const int parts = kv_parts(ctx, D);
-    launch_pdl_smem(kv_attn_kernel<FMT, D, QT>, dim3(parts), dim3(kKvWarps * 32), smem, st, a, records);
-    launch_pdl(kv_join_kernel<FMT>, dim3(parts, kKvCols), dim3(256), st, a, records);
+    KvJoin *joins = reinterpret_cast<KvJoin *>(reinterpret_cast<uint8_t *>(records) + kv_records_bytes(ctx, D));
+    launch_pdl_smem(kv_attn_kernel<FMT, D, QT>, dim3(parts), dim3(kKvWarps * 32), smem, st, a, records, joins);
+    launch_pdl(kv_join_kernel<FMT>, dim3(parts, (unsigned)std::min<int64_t>(kKvCols, (int64_t)a.rows * a.group)), dim3(256), st, a, records, joins);
     ctx->launches += 2;
     return check_cuda(ctx, cudaGetLastError(), "cache attention launch");
 }
@@ -515,7 +609,7 @@ nnq_status nnq_kv_attention_workspace(nnq_ctx *ctx, const nnq_kv_cache *c, const
     if (!bytes) return fail(ctx, NNQ_ERR_INVALID_ARG, "NULL result");
     nnq_status s = check_batch(ctx, c, b, heads);
     if (s != NNQ_OK) return s;
-    *bytes = std::max((size_t)kv_parts(ctx, c->dim) * 2 * kKvCols * kv_record_floats(c->dim) * 4, kv_attn_tc_workspace(ctx, c->dim));
+    *bytes = std::max(kv_records_bytes(ctx, c->dim) + kv_parts(ctx, c->dim) * sizeof(KvJoin), kv_attn_tc_workspace(ctx, c->dim));
     return NNQ_OK;
 }
 

@@ -20,21 +20,21 @@ struct KvAttn {
 // One request of the batch as the kernels take it: numbers outside their range are brought inside (the results of such a request are
 // undefined, its reads and writes are not).
 struct KvRequest {
-    int row0, rows;       // its rows of q and y
-    int64_t length;       // positions held, the rows' own included
+    int row0, rows;   // its rows of q and y
+    int length;       // positions held, the rows' own included
 };
 __device__ __forceinline__ KvRequest kv_request(const KvAttn &a, int64_t r) {
     KvRequest q;
     const int s0 = (int)min(max((int64_t)a.row_start[r], (int64_t)0), a.rows), s1 = (int)min(max((int64_t)a.row_start[r + 1], (int64_t)s0), a.rows);
     q.row0 = s0;
     q.rows = s1 - s0;
-    q.length = min(max((int64_t)a.length[r], (int64_t)0), a.table_ld << a.shift);
+    q.length = (int)min(max((int64_t)a.length[r], (int64_t)0), a.table_ld << a.shift);
     if (q.length < a.length[r] || s0 != a.row_start[r] || s1 != a.row_start[r + 1]) atomicExch(a.status, kStatusIndex);
     return q;
 }
 // position of row i, and the first position it sees
-__device__ __forceinline__ int64_t row_pos(const KvRequest &q, int i) { return q.length - q.rows + i; }
-__device__ __forceinline__ int64_t row_first(const KvAttn &a, int64_t pos) { return a.window > 0 ? max(pos - a.window + 1, (int64_t)0) : 0; }
+__device__ __forceinline__ int row_pos(const KvRequest &q, int i) { return q.length - q.rows + i; }
+__device__ __forceinline__ int row_first(const KvAttn &a, int pos) { return a.window > 0 && pos >= a.window ? pos - a.window + 1 : 0; }
 
 // Two f16 numbers of two codes that lie in the bytes of a 16-bit half each: int8 exactly, e4m3 times 2^-8 (its bits moved to their
 // place in an f16 number, subnormal ones included).
@@ -52,6 +52,14 @@ struct CodePairs<NNQ_KV_INT8> {
     // bytes 0, 1 (2, 3) of a word
     static __device__ __forceinline__ uint32_t low(uint32_t w) { return half(__byte_perm(w, 0x64646464u, 0x4140)); }
     static __device__ __forceinline__ uint32_t high(uint32_t w) { return half(__byte_perm(w, 0x64646464u, 0x4342)); }
+    // bytes i of x and y side by side, i = 0 .. 3
+    static __device__ __forceinline__ void pairs(uint32_t x, uint32_t y, uint32_t &p0, uint32_t &p1, uint32_t &p2, uint32_t &p3) {
+        const uint32_t u = __byte_perm(word(x), word(y), 0x5140), v = __byte_perm(word(x), word(y), 0x7362);
+        p0 = low(u);
+        p1 = high(u);
+        p2 = low(v);
+        p3 = high(v);
+    }
 };
 template <>
 struct CodePairs<NNQ_KV_E4M3> {
@@ -60,6 +68,12 @@ struct CodePairs<NNQ_KV_E4M3> {
     static __device__ __forceinline__ uint32_t half(uint32_t x) { return (x & 0x80008000u) | ((x >> 1) & 0x3F803F80u); }
     static __device__ __forceinline__ uint32_t low(uint32_t w) { return half(__byte_perm(w, 0, 0x1404)); }
     static __device__ __forceinline__ uint32_t high(uint32_t w) { return half(__byte_perm(w, 0, 0x3424)); }
+    static __device__ __forceinline__ void pairs(uint32_t x, uint32_t y, uint32_t &p0, uint32_t &p1, uint32_t &p2, uint32_t &p3) {
+        p0 = half(__byte_perm(x, y, 0x4400));   // (the lower bytes of the halves are masked out)
+        p1 = half(__byte_perm(x, y, 0x5511));
+        p2 = half(__byte_perm(x, y, 0x6622));
+        p3 = half(__byte_perm(x, y, 0x7733));
+    }
 };
 
 __device__ __forceinline__ float kv_ex2(float x) {
