@@ -6,9 +6,9 @@
 //   warps 0-3, 4-7: softmax. Thread r of a group owns query vector r: its scores from tensor memory, maximum and sum; the weights go back
 //                   into the columns of the scores as f16, where the second product reads them. The weighted values of all tiles
 //                   add up in tensor memory; a reference moves only when a score passes it by 2^8, and then the sums there are scaled.
-//   warps 8-11:     codes from the blocks of the table to f16 tiles in shared memory, swizzled as the products read them, keys and values
+//   warps 8-15:     codes from the blocks of the table to f16 tiles in shared memory, swizzled as the products read them, keys and values
 //                   as they lie (the values are the MN-major operand); the next tile's codes are under way meanwhile.
-//   warp 12:        one lane issues the MMAs: S(t + 1) of a group right behind its O += P(t) V(t). MMAs run in the order they are issued,
+//   warp 16:        (three more complete its group) one lane issues the MMAs: S(t + 1) of a group right behind its O += P(t) V(t). MMAs run in the order they are issued,
 //                   so the scores may overwrite the weights in front of them.
 // While one group is at its softmax, the other's products run. Codes are exact in f16. T = 1 (bf16 queries and outputs): a query vector is
 // exact under its power of two, a weight is one f16 number, off by up to 2^-11 of itself where the output's own rounding is 2^-8 of it. T = 2 (f32
@@ -21,13 +21,15 @@
 // long contexts load all SMs alike. An item inside a part is written directly, of one that is cut every part leaves a record, and
 // kv_tc_join_kernel joins them in order.
 #include <algorithm>
+#include <type_traits>
 
 #include "kv_attn.cuh"
 #include "tcgen05.cuh"
 
 namespace nnq {
 
-constexpr int kTcCols = 256, kTcThreads = 13 * 32, kTcStages = 2, kTcMinSteps = 4;
+constexpr int kTcCols = 256, kTcThreads = 20 * 32, kTcStages = 2, kTcMinSteps = 4;
+constexpr int kTcNone = INT32_MIN;   // in place of a block: no such key
 constexpr float kTcLog2E = 1.4426950408889634f, kTcSlack = 8.0f;
 
 // keys of a tile: 128, 64 where the queries' second terms take the room
@@ -198,6 +200,12 @@ struct TcWalk {
 
 __host__ __device__ inline int64_t tc_record_floats(int dim) { return (int64_t)kTcCols * (4 + dim); }   // per vector m, mv, l, unused; then [dim / 4][vector] of four
 
+struct TcJoin {   // what a part has to join: the item that ends in it
+    int first;   // part that the item begins in, -1: nothing
+    int vecs, row, head, rest;   // vectors; row of the first one, first query head of its group, its number there
+    int unused[3];
+};
+
 template <int D, int T>
 struct TcShared {
     static constexpr int KT = TcTile<T>::keys, atoms = D / 64;
@@ -216,41 +224,72 @@ __device__ __forceinline__ uint64_t tc_desc_mn(uint32_t addr, uint32_t next) {
     const uint32_t lo = ((addr >> 4) & 0x3FFFu) | ((next >> 4) << 16), hi = (1024u >> 4) | (1u << 14) | (2u << 29);
     return ((uint64_t)hi << 32) | lo;
 }
+// loads of 32 columns without a wait, and the wait, which the loaded registers depend on
+__device__ __forceinline__ void tc_ld(uint32_t addr, uint32_t (&v)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]),
+          "=r"(v[14]), "=r"(v[15]), "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]),
+          "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+        : "r"(addr));
+}
+__device__ __forceinline__ void tc_tie(uint32_t (&v)[32]) {
+    asm volatile("" : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]), "+r"(v[8]), "+r"(v[9]), "+r"(v[10]), "+r"(v[11]), "+r"(v[12]), "+r"(v[13]),
+                      "+r"(v[14]), "+r"(v[15]), "+r"(v[16]), "+r"(v[17]), "+r"(v[18]), "+r"(v[19]), "+r"(v[20]), "+r"(v[21]), "+r"(v[22]), "+r"(v[23]), "+r"(v[24]), "+r"(v[25]), "+r"(v[26]),
+                      "+r"(v[27]) : : "memory");
+    asm volatile("" : "+r"(v[28]), "+r"(v[29]), "+r"(v[30]), "+r"(v[31]) : : "memory");
+}
+__device__ __forceinline__ void tc_ld_wait(uint32_t (&a)[32], uint32_t (&b)[32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+    tc_tie(a);
+    tc_tie(b);
+}
+// A role's registers, of the 640 threads x 96 = 61440 that the block is launched with: 256 x 152 + 256 x 64 + 128 x 40 = 60416.
+template <int N>
+__device__ __forceinline__ void tc_registers() {
+    if constexpr (N > 96) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+    else asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
 __device__ __forceinline__ void group_sync(int w) { asm volatile("bar.sync %0, 128;" ::"r"(1 + w) : "memory"); }
 
 template <int FMT, int D, int T>
-__global__ void __launch_bounds__(kTcThreads, 1) kv_attn_tc_kernel(const KvAttn a, float *records) {
+__global__ void __launch_bounds__(kTcThreads, 1) kv_attn_tc_kernel(const KvAttn a, float *records, TcJoin *joins) {
     typedef TcShared<D, T> Sh;
     typedef CodePairs<FMT> Codes;
     constexpr int KT = Sh::KT, ATOMS = Sh::atoms, SUBS = KT / 16;
     extern __shared__ __align__(1024) uint8_t tc_smem_raw[];
     uint8_t *smem = tc_smem_raw + (-smem_u32(tc_smem_raw) & 1023u);
-    __shared__ __align__(8) uint64_t bars[2 * kTcStages + 9];   // full, empty; q_full, s_full, p_full, o_done of two groups; drain
+    __shared__ __align__(8) uint64_t bars[2 * kTcStages + 11];   // full, empty; q_full, s_full, p_full (64 keys each), o_done of two groups; drain
     __shared__ int2 sub_info[kTcStages][SUBS];                  // exponent bytes of keys and values of every 16 keys; x < 0: unseen
-    __shared__ float q_un[2][128];
     __shared__ uint32_t tmem_s;
     __shared__ int found[4];
     __shared__ int64_t sums[33];
     const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xFFFFFFFFu, tid >> 5, 0);
-    const uint32_t full = smem_u32(bars), empty = full + 8 * kTcStages, qf = empty + 8 * kTcStages, sf = qf + 16, pf = sf + 16, of = pf + 16, drain = of + 16;
+    const uint32_t full = smem_u32(bars), empty = full + 8 * kTcStages, qf = empty + 8 * kTcStages, sf = qf + 16, pf = sf + 16, of = pf + 32, drain = of + 16;
     pdl_prologue();
+    pdl_release();
     const TcPlan plan = tc_plan<KT>(a, gridDim.x, found, sums);
-    if (plan.begin >= plan.end) return;
+    if (plan.begin >= plan.end) {
+        if (tid == 0) joins[blockIdx.x].first = -1;
+        return;
+    }
     if (tid == 0) {
         for (int i = 0; i < kTcStages; i++) {
-            mbar_init(full + 8 * i, 4);
+            mbar_init(full + 8 * i, 8);
             mbar_init(empty + 8 * i, 1);
         }
         for (int w = 0; w < 2; w++) {
             mbar_init(qf + 8 * w, 1);
             mbar_init(sf + 8 * w, 1);
-            mbar_init(pf + 8 * w, 4);
+            mbar_init(pf + 16 * w, 4);
+            mbar_init(pf + 16 * w + 8, 4);
             mbar_init(of + 8 * w, 1);
         }
         mbar_init(drain, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 12) {
+    if (warp == 16) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_s)), "r"(512u) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
@@ -266,6 +305,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attn_tc_kernel(const KvAttn 
 
     if (warp < 8) {
         // ---------------- softmax ----------------
+        tc_registers<152>();
         const int w = warp >> 2, me = tid & 127;
         const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16, o_t = tmem + 256 * w + lane_base, s_t = o_t + 128;
         uint8_t *q_s = smem + w * T * ATOMS * Sh::q_atom;
@@ -275,99 +315,98 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attn_tc_kernel(const KvAttn 
                 n += it.s1 - it.s0;
                 continue;
             }
+            const int vec = it.vec0 + min(w * 128 + me, it.vecs - 1), row = vec / a.group, qhead = it.head * a.group + vec - row * a.group;
+            uint32_t big = 0;
             {
-                // the group's query vectors, a warp per vector and turn, a lane has D / 32 dimensions; the loads of a turn before its stores
-                constexpr int E = D / 32, QN = 8;
-                for (int v0 = warp & 3; v0 < 128; v0 += 4 * QN) {
-                    float x[QN][E];
+                // the thread's query vector, 32 dimensions at a time: first for its largest value, then (from L1) for the terms
+                const int64_t at = (int64_t)(it.row0 + row) * a.q_ld + (int64_t)qhead * D;
+                auto part = [&](int c, float (&x)[32]) {
+                    if (T == 2 && a.q_dt == NNQ_F32) {
+                        const float4 *p = reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(a.q) + at + 32 * c);
 #pragma unroll
-                    for (int i = 0; i < QN; i++) {
-                        const int v = w * 128 + v0 + 4 * i, vec = it.vec0 + v, row = vec / a.group;
+                        for (int i = 0; i < 8; i++) {
+                            const float4 f = __ldg(p + i);
+                            x[4 * i] = f.x; x[4 * i + 1] = f.y; x[4 * i + 2] = f.z; x[4 * i + 3] = f.w;
+                        }
+                    } else {
+                        const uint4 *p = reinterpret_cast<const uint4 *>(reinterpret_cast<const __nv_bfloat16 *>(a.q) + at + 32 * c);
 #pragma unroll
-                        for (int e = 0; e < E; e++) x[i][e] = 0.0f;
-                        if (v >= it.vecs) continue;
-                        const int64_t at = (int64_t)(it.row0 + row) * a.q_ld + (int64_t)(it.head * a.group + vec - row * a.group) * D + lane * E;
-                        if (a.q_dt == NNQ_F32) {
+                        for (int i = 0; i < 4; i++) {
+                            const uint4 u = __ldg(p + i);
+                            const uint32_t v[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-                            for (int e = 0; e < E; e += 2) {
-                                const float2 f = __ldg(reinterpret_cast<const float2 *>(reinterpret_cast<const float *>(a.q) + at + e));
-                                x[i][e] = f.x;
-                                x[i][e + 1] = f.y;
-                            }
-                        } else {
-#pragma unroll
-                            for (int e = 0; e < E; e += 2) {
-                                const uint32_t u = __ldg(reinterpret_cast<const uint32_t *>(reinterpret_cast<const __nv_bfloat16 *>(a.q) + at + e));
-                                x[i][e] = __uint_as_float(u << 16);
-                                x[i][e + 1] = __uint_as_float(u & 0xFFFF0000u);
+                            for (int e = 0; e < 4; e++) {
+                                x[8 * i + 2 * e] = __uint_as_float(v[e] << 16);
+                                x[8 * i + 2 * e + 1] = __uint_as_float(v[e] & 0xFFFF0000u);
                             }
                         }
                     }
+                };
 #pragma unroll
-                    for (int i = 0; i < QN; i++) {
-                        const int v = v0 + 4 * i, d = lane * E;
-                        uint32_t big = 0;
+                for (int c = 0; c < D / 32; c++) {
+                    float x[32];
+                    part(c, x);
 #pragma unroll
-                        for (int e = 0; e < E; e++) big = max(big, __float_as_uint(x[i][e]) & 0x7FFFFFFFu);
-                        big = __reduce_max_sync(0xFFFFFFFFu, big);
-                        const float sc = kv_top_scale(big);
-                        if (lane == 0) q_un[w][v] = kv_top_unscale(big);
-                        uint32_t hi[E / 2], lo[E / 2];
+                    for (int i = 0; i < 32; i++) big = max(big, __float_as_uint(x[i]) & 0x7FFFFFFFu);
+                }
+                const float sc = kv_top_scale(big);
 #pragma unroll
-                        for (int e = 0; e < E / 2; e++) kv_split(x[i][2 * e] * sc, x[i][2 * e + 1] * sc, hi[e], lo[e]);
-                        uint8_t *dst = q_s + (d >> 6) * Sh::q_atom + swz(v, (d & 63) >> 3) + 2 * (d & 7);
+                for (int c = 0; c < D / 32; c++) {
+                    float x[32];
+                    part(c, x);
 #pragma unroll
-                        for (int e = 0; e < E / 2; e++) {
-                            reinterpret_cast<uint32_t *>(dst)[e] = hi[e];
-                            if (T == 2) reinterpret_cast<uint32_t *>(dst + ATOMS * Sh::q_atom)[e] = lo[e];
-                        }
+                    for (int i = 0; i < 4; i++) {
+                        uint32_t hi[4], lo[4];
+#pragma unroll
+                        for (int e = 0; e < 4; e++) kv_split(x[8 * i + 2 * e] * sc, x[8 * i + 2 * e + 1] * sc, hi[e], lo[e]);
+                        uint8_t *dst = q_s + (c >> 1) * Sh::q_atom + swz(me, (c & 1) * 4 + i);
+                        *reinterpret_cast<uint4 *>(dst) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                        if (T == 2) *reinterpret_cast<uint4 *>(dst + ATOMS * Sh::q_atom) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
                     }
                 }
             }
             fence_async_smem();
             group_sync(w);
             if (me == 0) mbar_arrive(qf + 8 * w);
-            const int vec = it.vec0 + min(w * 128 + me, it.vecs - 1), row = vec / a.group, pos = it.length - it.rows + row;
+            const int pos = it.length - it.rows + row;
             const int low = a.window > 0 ? max(pos - a.window + 1, 0) : 0;
-            const float fac = a.scale * kTcLog2E * Codes::unscale * q_un[w][me];
+            const float fac = a.scale * kTcLog2E * Codes::unscale * kv_top_unscale(big);
             float m = 0.0f, mv = 0.0f, l = 0.0f, thr = -INFINITY, thv = -INFINITY;
-            for (int s = it.s0; s < it.s1; s++, n++, nw++) {
-                const int st = n % kTcStages, key0 = (it.first + s) * KT;
-                // (the scores first: behind them the tile's barrier is in the phase asked for, whatever tiles this group has skipped)
-                ok = __all_sync(0xFFFFFFFFu, mbar_wait_fast(sf + 8 * w, nw & 1) && mbar_wait_fast(full + 8 * st, (n / kTcStages) & 1));
-                if (!ok) break;
-                tc_fence_after();
-                const int hi = pos - key0, lo = low - key0;   // visible keys of the tile: lo .. hi
-                // (in tiles that all vectors of the warp see whole, of blocks that exist, nothing is masked)
-                bool there = true;
+            // A tile of keys, starting at key0; CLEAR: every vector of the warp sees all of it.
+            auto tile = [&](auto clear, int st, int key0, bool first) {
+                constexpr bool CLEAR = decltype(clear)::value;
+                uint32_t seen[KT / 32];   // a bit per key
+                if constexpr (!CLEAR) {
 #pragma unroll
-                for (int b = 0; b < SUBS; b++) there = there && sub_info[st][b].x >= 0;
-                const bool clear = __all_sync(0xFFFFFFFFu, hi >= KT - 1 && lo <= 0) && there;
-                auto masked = [&](int i, float x) { return clear || (i <= hi && i >= lo && sub_info[st][i >> 4].x >= 0) ? x : -INFINITY; };
+                    for (int c = 0; c < KT / 32; c++) {
+                        const int hi = pos - key0 - 32 * c, lo = low - key0 - 32 * c;   // visible keys of the 32: lo .. hi
+                        seen[c] = (hi >= 31 ? 0xFFFFFFFFu : hi < 0 ? 0u : (2u << hi) - 1u) & (lo <= 0 ? 0xFFFFFFFFu : lo > 31 ? 0u : 0xFFFFFFFFu << lo);
+                        if (sub_info[st][2 * c].x < 0) seen[c] &= 0xFFFF0000u;
+                        if (sub_info[st][2 * c + 1].x < 0) seen[c] &= 0xFFFFu;
+                    }
+                }
                 // ---- maxima: of the scores, and of scores + value exponents
                 float mt = -INFINITY, vt = -INFINITY;
-                uint32_t sc[T == 2 ? 64 : 32];
+                uint32_t x[2][32];
 #pragma unroll
-                for (int c = 0; c < KT / 32; c++) {
-                    uint32_t x[32];
-                    tmem_ld32(s_t + 32 * c, x);
+                for (int h = 0; h < KT / 64; h++) {
+                    tc_ld(s_t + 64 * h, x[0]);
+                    tc_ld(s_t + 64 * h + 32, x[1]);
+                    tc_ld_wait(x[0], x[1]);
 #pragma unroll
-                    for (int b = 0; b < 2; b++) {
-                        const int2 info = sub_info[st][2 * c + b];
-                        float t0 = -INFINITY, t1 = -INFINITY;
+                    for (int b = 0; b < 4; b++) {
+                        const int2 info = sub_info[st][4 * h + b];
+                        float t[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-                        for (int i = 0; i < 16; i += 2) {
-                            t0 = fmaxf(t0, masked(32 * c + 16 * b + i, __uint_as_float(x[16 * b + i])));
-                            t1 = fmaxf(t1, masked(32 * c + 16 * b + i + 1, __uint_as_float(x[16 * b + i + 1])));
+                        for (int i = 0; i < 16; i++) {
+                            float v = __uint_as_float(x[b >> 1][16 * (b & 1) + i]);
+                            if (!CLEAR) v = seen[2 * h + (b >> 1)] >> (16 * (b & 1) + i) & 1u ? v : -INFINITY;
+                            t[i & 1] = fmaxf(t[i & 1], v);
                         }
-                        float t = fmaxf(t0, t1);
-                        if (t > -INFINITY) t *= fac * pow2_byte(info.x);   // (the factor can be zero)
-                        mt = fmaxf(mt, t);
-                        vt = fmaxf(vt, t + (float)(info.y - 127));
-                    }
-                    if (T == 2) {
-#pragma unroll
-                        for (int i = 0; i < 32; i++) sc[32 * (c & 1) + i] = x[i];
+                        float top = fmaxf(t[0], t[1]);
+                        if (CLEAR || top > -INFINITY) top *= fac * pow2_byte(info.x);   // (the factor can be zero)
+                        mt = fmaxf(mt, top);
+                        vt = fmaxf(vt, top + (float)(info.y - 127));
                     }
                 }
                 // ---- references
@@ -386,58 +425,78 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attn_tc_kernel(const KvAttn 
                         thr = mn + kTcSlack;
                         thv = vn + kTcSlack;
                     }
-                    if (s > it.s0 && __any_sync(0xFFFFFFFFu, f != 1.0f)) {
+                    if (!first && __any_sync(0xFFFFFFFFu, f != 1.0f)) {
                         ok = __all_sync(0xFFFFFFFFu, mbar_wait_fast(of + 8 * w, (nw - 1) & 1));
-                        if (!ok) break;
+                        if (!ok) return;
                         tc_fence_after();
-#pragma unroll
+#pragma unroll 1
                         for (int c = 0; c < D / 32; c++) {
-                            uint32_t x[32], y[16];
-                            tmem_ld32(o_t + 32 * c, x);
+                            uint32_t o[32], y[16];
+                            tmem_ld32(o_t + 32 * c, o);
 #pragma unroll
                             for (int h = 0; h < 2; h++) {
 #pragma unroll
-                                for (int i = 0; i < 16; i++) y[i] = __float_as_uint(__uint_as_float(x[16 * h + i]) * f);
+                                for (int i = 0; i < 16; i++) y[i] = __float_as_uint(__uint_as_float(o[16 * h + i]) * f);
                                 tc_st(o_t + 32 * c + 16 * h, y);
                             }
                         }
                     }
                 }
-                // ---- weights
-                float2 sum = make_float2(0.0f, 0.0f);
-                const float2 nm = make_float2(-m, -m);
+                // ---- weights (two terms: the scores of the tile's 64 keys are still there)
+                const float fv0 = m - mv - 127.0f;
 #pragma unroll
-                for (int c = 0; c < KT / 32; c++) {
-                    uint32_t x[32], h[16], lw[16];
-                    if (T == 2) {
-#pragma unroll
-                        for (int i = 0; i < 32; i++) x[i] = sc[32 * (c & 1) + i];
-                    } else {
-                        tmem_ld32(s_t + 32 * c, x);
+                for (int h = 0; h < KT / 64; h++) {
+                    if (KT > 64) {
+                        tc_ld(s_t + 64 * h, x[0]);
+                        tc_ld(s_t + 64 * h + 32, x[1]);
+                        tc_ld_wait(x[0], x[1]);
                     }
 #pragma unroll
-                    for (int b = 0; b < 2; b++) {
-                        const int2 info = sub_info[st][2 * c + b];
-                        const float fk = fac * pow2_byte(max(info.x, 0)), fv = kv_ex2(m - mv + (float)(info.y - 127));
+                    for (int c = 0; c < 2; c++) {
+                        uint32_t hw[16], lw[16];
 #pragma unroll
-                        for (int i = 0; i < 16; i += 2) {
-                            const int k = 32 * c + 16 * b + i;
-                            const float2 y = __ffma2_rn(make_float2(__uint_as_float(x[16 * b + i]), __uint_as_float(x[16 * b + i + 1])), make_float2(fk, fk), nm);
-                            const float2 p = make_float2(kv_ex2(masked(k, y.x)), kv_ex2(masked(k + 1, y.y)));
-                            sum = __fadd2_rn(sum, p);
-                            const float2 v = __fmul2_rn(p, make_float2(fv, fv));
-                            if (T == 2) kv_split(v.x, v.y, h[8 * b + i / 2], lw[8 * b + i / 2]);
-                            else h[8 * b + i / 2] = half_bits(__floats2half2_rn(v.x, v.y));
+                        for (int b = 0; b < 2; b++) {
+                            const int2 info = sub_info[st][4 * h + 2 * c + b];
+                            // w = 2^(s - m + lf); the sum takes 2^-lf of the 16 together (below 2^-56 a weight is zero in f16 either way)
+                            const float fk = fac * pow2_byte(max(info.x, 0)), lf = fmaxf(fv0 + (float)info.y, -64.0f);
+                            const float2 nm = make_float2(lf - m, lf - m);
+                            float2 sum = make_float2(0.0f, 0.0f);
+#pragma unroll
+                            for (int i = 0; i < 16; i += 2) {
+                                const int k = 16 * b + i;
+                                float2 y = __ffma2_rn(make_float2(__uint_as_float(x[c][k]), __uint_as_float(x[c][k + 1])), make_float2(fk, fk), nm);
+                                if (!CLEAR) {
+                                    y.x = seen[2 * h + c] >> k & 1u ? y.x : -INFINITY;
+                                    y.y = seen[2 * h + c] >> (k + 1) & 1u ? y.y : -INFINITY;
+                                }
+                                const float2 v = make_float2(kv_ex2(y.x), kv_ex2(y.y));
+                                sum = __fadd2_rn(sum, v);
+                                if (T == 2) kv_split(v.x, v.y, hw[k / 2], lw[k / 2]);
+                                else hw[k / 2] = half_bits(__floats2half2_rn(v.x, v.y));
+                            }
+                            l = fmaf(sum.x + sum.y, kv_ex2(-lf), l);
                         }
+                        tc_st(s_t + 32 * h + 16 * c, hw);
+                        if (T == 2) tc_st(s_t + 32 + 16 * c, lw);
                     }
-                    tc_st(s_t + 16 * c, h);
-                    if (T == 2) tc_st(s_t + 32 + 16 * c, lw);
+                    // the products of these 64 keys may begin
+                    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                    tc_fence_before();
+                    __syncwarp();
+                    if (elect_one()) mbar_arrive(pf + 8 * (2 * w + h));
                 }
-                l += sum.x + sum.y;
-                asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-                tc_fence_before();
-                __syncwarp();
-                if (elect_one()) mbar_arrive(pf + 8 * w);
+            };
+            for (int s = it.s0; s < it.s1 && ok; s++, n++, nw++) {
+                const int st = n % kTcStages, key0 = (it.first + s) * KT;
+                // (the scores first: behind them the tile's barrier is in the phase asked for, whatever tiles this group has skipped)
+                ok = __all_sync(0xFFFFFFFFu, mbar_wait_fast(sf + 8 * w, nw & 1) && mbar_wait_fast(full + 8 * st, (n / kTcStages) & 1));
+                if (!ok) break;
+                tc_fence_after();
+                bool all = pos - key0 >= KT - 1 && low <= key0;
+#pragma unroll
+                for (int b = 0; b < SUBS; b++) all = all && sub_info[st][b].x >= 0;
+                if (__all_sync(0xFFFFFFFFu, all)) tile(std::true_type(), st, key0, s == it.s0);
+                else tile(std::false_type(), st, key0, s == it.s0);
             }
             if (!ok) break;
             ok = __all_sync(0xFFFFFFFFu, mbar_wait_fast(of + 8 * w, (nw - 1) & 1));
@@ -446,7 +505,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attn_tc_kernel(const KvAttn 
             const bool whole = it.s0 == 0 && it.s1 == it.steps, mine = w * 128 + me < it.vecs, none = !(thr > -INFINITY) && l == 0.0f;
             if (whole) {
                 const float inv = none ? 0.0f : exp2f(mv - m) * Codes::unscale / l;
-                const int64_t to = (int64_t)(it.row0 + row) * a.y_ld + (int64_t)(it.head * a.group + vec - row * a.group) * D;
+                const int64_t to = (int64_t)(it.row0 + row) * a.y_ld + (int64_t)qhead * D;
 #pragma unroll
                 for (int c = 0; c < D / 32; c++) {
                     uint32_t x[32];
@@ -482,70 +541,82 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attn_tc_kernel(const KvAttn 
             }
             tc_fence_before();
         }
-    } else if (warp < 12) {
+    } else if (warp < 16) {
         // ---------------- codes to f16 tiles ----------------
-        constexpr int CH = D / 16, PER = KT * CH / 128;   // 16-byte chunks of a row, chunks of a thread
+        tc_registers<64>();
+        constexpr int CH = D / 16, PER = KT * CH / 256;   // 16-byte chunks of a row, chunks of a thread
         const int pt = tid - 256;
         while (ok && walk.next(it)) {
             const int32_t *table = a.table + (int64_t)it.r * a.table_ld;
             uint4 k[PER], v[PER];
-            int2 info = make_int2(-1, 0);
-            auto block_at = [&](int key) -> int {
-                if (key >= it.length) return -1;
-                const int b = table[key >> a.shift];
-                if (b >= 0 && b < a.blocks) return b;
-                atomicExch(a.status, kStatusIndex);
-                return -1;
+            int blk[PER];   // of the next tile's chunks
+            int2 info = make_int2(-1, 127);
+            const int key_of = pt / CH, c = pt % CH;   // chunk i of this thread: 16 bytes c of key key_of + 256 / CH i
+            constexpr int KEYS = 256 / CH;
+            auto blocks = [&](int s) {
+                const int key0 = (it.first + s) * KT + key_of;
+#pragma unroll
+                for (int i = 0; i < PER; i++) blk[i] = s < it.s1 && key0 + KEYS * i < it.length ? table[(key0 + KEYS * i) >> a.shift] : kTcNone;
             };
-            auto load = [&](int s) {
-                const int key0 = (it.first + s) * KT;
+            auto load = [&](const uint8_t *codes, int s, uint4 (&x)[PER]) {
+                const int key0 = (it.first + s) * KT + key_of;
 #pragma unroll
                 for (int i = 0; i < PER; i++) {
-                    const int u = pt + 128 * i, key = key0 + u / CH, c = u % CH, b = block_at(key);
-                    k[i] = v[i] = make_uint4(0, 0, 0, 0);
-                    if (b >= 0) {
-                        const int64_t at = ((((int64_t)b * a.kv_heads + it.head) << a.shift) + (key & ((1 << a.shift) - 1))) * D + c * 16;
-                        k[i] = __ldg(reinterpret_cast<const uint4 *>(a.k + at));
-                        v[i] = __ldg(reinterpret_cast<const uint4 *>(a.v + at));
-                    }
-                }
-                if (pt < SUBS) {
-                    const int b = block_at(key0 + 16 * pt);
-                    const int64_t bh = (int64_t)b * a.kv_heads + it.head;
-                    info = b >= 0 ? make_int2(a.k_exp[bh], a.v_exp[bh]) : make_int2(-1, 127);
+                    x[i] = make_uint4(0, 0, 0, 0);
+                    if (blk[i] >= 0 && blk[i] < a.blocks)
+                        x[i] = __ldg(reinterpret_cast<const uint4 *>(codes + ((((int64_t)blk[i] * a.kv_heads + it.head) << a.shift) + ((key0 + KEYS * i) & ((1 << a.shift) - 1))) * D + c * 16));
+                    else if (blk[i] != kTcNone)
+                        atomicExch(a.status, kStatusIndex);
                 }
             };
-            load(it.s0);
+            auto bytes = [&](int s) {
+                const int key = (it.first + s) * KT + 16 * pt;
+                const int b = pt < SUBS && s < it.s1 && key < it.length ? table[key >> a.shift] : kTcNone;
+                const int64_t bh = (int64_t)b * a.kv_heads + it.head;
+                info = b >= 0 && b < a.blocks ? make_int2(a.k_exp[bh], a.v_exp[bh]) : make_int2(-1, 127);
+            };
+            auto store = [&](uint8_t *dst, const uint4 (&x)[PER]) {
+                const int flip = (c >> 2) & 1, c8 = (c & 3) * 2;   // (neighbours of two pieces store their halves in turn: no bank twice)
+#pragma unroll
+                for (int i = 0; i < PER; i++) {
+                    const int key = key_of + KEYS * i;
+                    const uint32_t w[4] = {Codes::word(x[i].x), Codes::word(x[i].y), Codes::word(x[i].z), Codes::word(x[i].w)};
+                    const uint4 lo = make_uint4(Codes::low(w[0]), Codes::high(w[0]), Codes::low(w[1]), Codes::high(w[1])), hi = make_uint4(Codes::low(w[2]), Codes::high(w[2]), Codes::low(w[3]), Codes::high(w[3]));
+                    uint8_t *p = dst + (c >> 2) * Sh::k_atom;
+                    *reinterpret_cast<uint4 *>(p + swz(key, c8 + flip)) = flip ? hi : lo;
+                    *reinterpret_cast<uint4 *>(p + swz(key, c8 + 1 - flip)) = flip ? lo : hi;
+                }
+            };
+            blocks(it.s0);
+            load(a.k, it.s0, k);
+            load(a.v, it.s0, v);
+            bytes(it.s0);
+            blocks(it.s0 + 1);
             for (int s = it.s0; s < it.s1; s++, n++) {
                 const int st = n % kTcStages;
                 if (n >= kTcStages) ok = __all_sync(0xFFFFFFFFu, mbar_wait_fast(empty + 8 * st, (n / kTcStages - 1) & 1));
                 if (!ok) break;
                 uint8_t *k_s = stages + st * Sh::stage, *v_s = k_s + ATOMS * Sh::k_atom;
-#pragma unroll
-                for (int i = 0; i < PER; i++) {
-                    const int u = pt + 128 * i, key = u / CH, c = u % CH, flip = (c >> 2) & 1;   // (neighbours of two pieces store their halves in turn: no bank twice)
-                    const uint32_t kw[4] = {Codes::word(k[i].x), Codes::word(k[i].y), Codes::word(k[i].z), Codes::word(k[i].w)};
-                    const uint32_t vw[4] = {Codes::word(v[i].x), Codes::word(v[i].y), Codes::word(v[i].z), Codes::word(v[i].w)};
-                    const int at = (c >> 2) * Sh::k_atom, c8 = (c & 3) * 2;
-                    const uint4 k0 = make_uint4(Codes::low(kw[0]), Codes::high(kw[0]), Codes::low(kw[1]), Codes::high(kw[1])), k1 = make_uint4(Codes::low(kw[2]), Codes::high(kw[2]), Codes::low(kw[3]), Codes::high(kw[3]));
-                    const uint4 v0 = make_uint4(Codes::low(vw[0]), Codes::high(vw[0]), Codes::low(vw[1]), Codes::high(vw[1])), v1 = make_uint4(Codes::low(vw[2]), Codes::high(vw[2]), Codes::low(vw[3]), Codes::high(vw[3]));
-                    *reinterpret_cast<uint4 *>(k_s + at + swz(key, c8 + flip)) = flip ? k1 : k0;
-                    *reinterpret_cast<uint4 *>(k_s + at + swz(key, c8 + 1 - flip)) = flip ? k0 : k1;
-                    *reinterpret_cast<uint4 *>(v_s + at + swz(key, c8 + flip)) = flip ? v1 : v0;
-                    *reinterpret_cast<uint4 *>(v_s + at + swz(key, c8 + 1 - flip)) = flip ? v0 : v1;
-                }
+                store(k_s, k);
+                load(a.k, s + 1, k);
+                store(v_s, v);
+                load(a.v, s + 1, v);
                 if (pt < SUBS) sub_info[st][pt] = info;
                 fence_async_smem();
                 __syncwarp();
                 if (elect_one()) mbar_arrive(full + 8 * st);
-                if (s + 1 < it.s1) load(s + 1);
+                bytes(s + 1);
+                blocks(s + 2);
             }
         }
     } else {
+        tc_registers<40>();
+        if (warp == 16) {
         // ---------------- MMA issuer (the warp waits together, one lane issues) ----------------
         const uint32_t id_s = (1u << 4) | ((uint32_t)(KT >> 3) << 17) | ((128u >> 4) << 24);                 // both operands f16
         const uint32_t id_o = (1u << 4) | (1u << 16) | ((uint32_t)(D >> 3) << 17) | ((128u >> 4) << 24);     // B is MN-major
         int nw[2] = {0, 0}, items[2] = {0, 0};
+        TcJoin join = {-1, 0, 0, 0, 0, {0, 0, 0}};
         auto wait = [&](uint32_t bar, int count) {
             ok = ok && __all_sync(0xFFFFFFFFu, mbar_wait_fast(bar, count & 1));
             return ok;
@@ -567,6 +638,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attn_tc_kernel(const KvAttn 
         };
         while (ok && walk.next(it)) {
             const int groups = it.vecs > 128 ? 2 : 1, steps = it.s1 - it.s0;
+            if (it.s0 > 0 && it.s1 == it.steps) join = {(int)((plan.begin - it.s0) / plan.chunk), it.vecs, it.row0 + it.vec0 / a.group, it.head * a.group, it.vec0 % a.group, {0, 0, 0}};
             for (int w = 0; w < groups; w++) wait(qf + 8 * w, items[w]++);
             if (!wait(full + 8 * (n % kTcStages), n / kTcStages)) break;
             tc_fence_after();
@@ -574,19 +646,26 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attn_tc_kernel(const KvAttn 
             for (int s = 0; s < steps && ok; s++, n++) {
                 const int st = n % kTcStages, st1 = (n + 1) % kTcStages;
                 for (int w = 0; w < groups; w++) {
-                    if (!wait(pf + 8 * w, nw[w]++)) break;
-                    tc_fence_after();
-                    if (elect_one()) {
-                        const uint32_t va = smem_u32(stages + st * Sh::stage + ATOMS * Sh::k_atom), pa = tmem + 256 * w + 128;
-                        const uint64_t dv = tc_desc_mn(va, Sh::k_atom);
 #pragma unroll
-                        for (int x = T - 1; x >= 0; x--)
+                    for (int h = 0; h < KT / 64; h++) {
+                        if (!wait(pf + 8 * (2 * w + h), nw[w])) break;
+                        tc_fence_after();
+                        if (elect_one()) {
+                            const uint32_t va = smem_u32(stages + st * Sh::stage + ATOMS * Sh::k_atom) + h * 64 * 128, pa = tmem + 256 * w + 128 + 32 * h;
+                            const uint64_t dv = tc_desc_mn(va, Sh::k_atom);
 #pragma unroll
-                            for (int k = 0; k < KT / 16; k++) umma_ts(tmem + 256 * w, pa + 32 * x + 8 * k, dv + (2048 >> 4) * k, id_o, s > 0 || x < T - 1 || k != 0);
-                        umma_commit(of + 8 * w);
-                        if (w == groups - 1) umma_commit(empty + 8 * st);
+                            for (int x = T - 1; x >= 0; x--)
+#pragma unroll
+                                for (int k = 0; k < 4; k++) umma_ts(tmem + 256 * w, pa + 32 * x + 8 * k, dv + (2048 >> 4) * k, id_o, s > 0 || h > 0 || x < T - 1 || k != 0);
+                            if (h == KT / 64 - 1) {
+                                umma_commit(of + 8 * w);
+                                if (w == groups - 1) umma_commit(empty + 8 * st);
+                            }
+                        }
+                        __syncwarp();
                     }
-                    __syncwarp();
+                    if (!ok) break;
+                    nw[w]++;
                     if (s + 1 < steps) {
                         if (w == 0 && !wait(full + 8 * st1, (n + 1) / kTcStages)) break;
                         tc_fence_after();
@@ -595,79 +674,82 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attn_tc_kernel(const KvAttn 
                 }
             }
         }
+        if (lane == 0) joins[blockIdx.x] = join;
         // MMAs that were issued may still read shared memory and write tensor memory
         if (elect_one()) umma_commit(drain);
         __syncwarp();
         ok = __all_sync(0xFFFFFFFFu, mbar_wait(drain, 0)) && ok;
+        }
     }
     if (!ok && lane == 0) atomicExch(a.status, 1);
     tc_fence_before();
     __syncthreads();
-    if (warp == 12) {
+    if (warp == 16) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
     }
 }
 
-// Joins the records of the items that were cut: CTA (part, some dimensions) where the item at the part's beginning began before it
-// and ends in it. A thread has a vector.
-template <int KT>
-__global__ void __launch_bounds__(kTcCols) kv_tc_join_kernel(const KvAttn a, const float *records, float unscale) {
-    __shared__ int found[4];
-    __shared__ int64_t sums[33];
+// Joins the records of the items that were cut: CTA (part that the item ends in, some dimensions). A thread has a vector.
+__global__ void __launch_bounds__(kTcCols) kv_tc_join_kernel(const KvAttn a, const float *records, const TcJoin *joins, float unscale) {
     pdl_prologue();
-    const TcPlan plan = tc_plan<KT>(a, gridDim.x, found, sums);
-    TcItem it;
-    TcWalk<KT> walk(a, plan, found);
-    if (!walk.next(it) || it.s0 == 0 || it.s1 < it.steps) return;
-    const int first = (int)((plan.begin - it.s0) / plan.chunk), v = threadIdx.x;   // the part that the item begins in
-    if (v >= it.vecs) return;
+    const TcJoin j = joins[blockIdx.x];
+    const int first = j.first, last = blockIdx.x, v = threadIdx.x;
+    if (first < 0 || v >= j.vecs) return;
     const int64_t rec_floats = tc_record_floats(a.dim);
     auto record = [&](int p) { return reinterpret_cast<const float4 *>(records + ((int64_t)p * 2 + (p == first ? 1 : 0)) * rec_floats); };
     float mm = -INFINITY, mv = -INFINITY;
-    for (int p = first; p <= (int)blockIdx.x; p++) {
+    for (int p = first; p <= last; p++) {
         const float4 h = record(p)[v];
         if (h.x == -INFINITY) continue;
         mm = fmaxf(mm, h.x);
         mv = fmaxf(mv, h.y);
     }
+    constexpr int Q = 4;   // quadruples of dimensions at a time
+    const int vec = j.rest + v, row = vec / a.group, quads = a.dim / 4, q0 = blockIdx.y * Q;
+    float4 o[Q];
+#pragma unroll
+    for (int q = 0; q < Q; q++) o[q] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     float l = 0.0f;
-    for (int p = first; p <= (int)blockIdx.x; p++) {
+    for (int p = first; p <= last; p++) {
         const float4 h = record(p)[v];
         if (h.x == -INFINITY) continue;
         l += h.z * exp2f(h.x - mm);
-    }
-    const int vec = it.vec0 + v, row = vec / a.group, quads = a.dim / 4, per = (quads + gridDim.y - 1) / gridDim.y;
-    const int64_t to = (int64_t)(it.row0 + row) * a.y_ld + (int64_t)(it.head * a.group + vec - row * a.group) * a.dim;
-    const float inv = mm == -INFINITY && l == 0.0f ? 0.0f : exp2f(mv - mm) * unscale / l;   // (l is NaN where only NaN scores came)
-    for (int q = blockIdx.y * per; q < min(quads, (int)(blockIdx.y + 1) * per); q++) {
-        float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        for (int p = first; p <= (int)blockIdx.x; p++) {
-            const float4 h = record(p)[v];
-            if (h.x == -INFINITY) continue;
-            const float f = exp2f(h.y - mv);
-            const float4 x = record(p)[kTcCols * (1 + q) + v];
-            o.x += x.x * f;
-            o.y += x.y * f;
-            o.z += x.z * f;
-            o.w += x.w * f;
+        const float f = exp2f(h.y - mv);
+        float4 x[Q];
+#pragma unroll
+        for (int q = 0; q < Q; q++) x[q] = record(p)[kTcCols * (1 + min(q0 + q, quads - 1)) + v];
+#pragma unroll
+        for (int q = 0; q < Q; q++) {
+            o[q].x += x[q].x * f;
+            o[q].y += x[q].y * f;
+            o[q].z += x[q].z * f;
+            o[q].w += x[q].w * f;
         }
-        o = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
-        if (a.y_dt == NNQ_F32) *reinterpret_cast<float4 *>(reinterpret_cast<float *>(a.y) + to + 4 * q) = o;
-        else *reinterpret_cast<uint2 *>(reinterpret_cast<__nv_bfloat16 *>(a.y) + to + 4 * q) = make_uint2(pack_bf16(o.x, o.y), pack_bf16(o.z, o.w));
+    }
+    const int64_t to = (int64_t)(j.row + row) * a.y_ld + (int64_t)(j.head + vec - row * a.group) * a.dim;
+    const float inv = l == 0.0f ? 0.0f : exp2f(mv - mm) * unscale / l;   // (l is NaN where only NaN scores came)
+#pragma unroll
+    for (int q = 0; q < Q; q++) {
+        if (q0 + q >= quads) break;
+        const float4 y = make_float4(o[q].x * inv, o[q].y * inv, o[q].z * inv, o[q].w * inv);
+        if (a.y_dt == NNQ_F32) *reinterpret_cast<float4 *>(reinterpret_cast<float *>(a.y) + to + 4 * (q0 + q)) = y;
+        else *reinterpret_cast<uint2 *>(reinterpret_cast<__nv_bfloat16 *>(a.y) + to + 4 * (q0 + q)) = make_uint2(pack_bf16(y.x, y.y), pack_bf16(y.z, y.w));
     }
 }
 
 bool kv_attn_tc_supported(const KvAttn &a) { return a.dim == 64 || a.dim == 128; }
-size_t kv_attn_tc_workspace(nnq_ctx *ctx, int dim) { return (size_t)ctx->sm_count * 2 * tc_record_floats(dim) * 4; }
+static size_t tc_records_bytes(nnq_ctx *ctx, int dim) { return (size_t)ctx->sm_count * 2 * tc_record_floats(dim) * 4; }
+size_t kv_attn_tc_workspace(nnq_ctx *ctx, int dim) { return tc_records_bytes(ctx, dim) + ctx->sm_count * sizeof(TcJoin); }
 
 template <int FMT, int D, int T>
 static nnq_status launch_tc(nnq_ctx *ctx, const KvAttn &a, float *records, cudaStream_t st) {
     constexpr int smem = TcShared<D, T>::bytes;
     nnq_status s = check_cuda(ctx, cudaFuncSetAttribute(kv_attn_tc_kernel<FMT, D, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), "attention shared memory");
     if (s != NNQ_OK) return s;
-    launch_pdl_smem(kv_attn_tc_kernel<FMT, D, T>, dim3(ctx->sm_count), dim3(kTcThreads), smem, st, a, records);
-    launch_pdl(kv_tc_join_kernel<TcTile<T>::keys>, dim3(ctx->sm_count, 8), dim3(kTcCols), st, a, records, CodePairs<FMT>::unscale);
+    TcJoin *joins = reinterpret_cast<TcJoin *>(reinterpret_cast<uint8_t *>(records) + tc_records_bytes(ctx, D));
+    launch_pdl_smem(kv_attn_tc_kernel<FMT, D, T>, dim3(ctx->sm_count), dim3(kTcThreads), smem, st, a, records, joins);
+    launch_pdl(kv_tc_join_kernel, dim3(ctx->sm_count, D / 16), dim3(kTcCols), st, a, records, joins, CodePairs<FMT>::unscale);
     ctx->launches += 2;
     return check_cuda(ctx, cudaGetLastError(), "cache attention launch");
 }
