@@ -3,14 +3,15 @@
 //
 // One CTA has up to 256 query vectors of one key / value head (consecutive (row, query head of the group) pairs), 128 for each of two
 // softmax groups, and walks over tiles of keys that both share.
-//   warps 0-3, 4-7: softmax. Thread r of a group owns query vector r: its scores from tensor memory, maximum and sum; the weights go back
-//                   into the columns of the scores as f16, where the second product reads them. The weighted values of all tiles
-//                   add up in tensor memory; a reference moves only when a score passes it by 2^8, and then the sums there are scaled.
+//   warps 0-3, 4-7: softmax. Thread r of a group owns query vector r: its scores of 64 keys from tensor memory, maximum and sum; the
+//                   weights go back into the columns of the scores as f16, where the second product reads them. Scores have two places,
+//                   so that the next tile's are there when a tile is done. The weighted values of all tiles add up in tensor
+//                   memory; a reference moves only when a score passes it by 2^8, and then the sums there are scaled.
 //   warps 8-15:     codes from the blocks of the table to f16 tiles in shared memory, swizzled as the products read them, keys and values
 //                   as they lie (the values are the MN-major operand); the next tile's codes are under way meanwhile.
-//   warp 16:        (three more complete its group) one lane issues the MMAs: S(t + 1) of a group right behind its O += P(t) V(t). MMAs run in the order they are issued,
-//                   so the scores may overwrite the weights in front of them.
-// While one group is at its softmax, the other's products run. Codes are exact in f16. T = 1 (bf16 queries and outputs): a query vector is
+//   warp 16:        (three more complete its group) one lane issues the MMAs: S(t + 1) of both groups, then O += P(t) V(t) of each. MMAs run in the order they are
+//                   issued, so S(t + 1) may overwrite the weights of t - 1, whose product stands in front of it.
+// What bounds it is the softmax: of the exponentials a thread forms, the special function unit takes 16 a clock and SM. Codes are exact in f16. T = 1 (bf16 queries and outputs): a query vector is
 // exact under its power of two, a weight is one f16 number, off by up to 2^-11 of itself where the output's own rounding is 2^-8 of it. T = 2 (f32
 // on either side): both have two terms, 22 bits.
 // Scales: a block's key exponent multiplies its scores in f32. Its value exponent enters the weight, w = p 2^(m - mv + e_v) with a
@@ -28,15 +29,9 @@
 
 namespace nnq {
 
-constexpr int kTcCols = 256, kTcThreads = 20 * 32, kTcStages = 2, kTcMinSteps = 4;
+constexpr int kTcCols = 256, kTcThreads = 20 * 32, kTcKeys = 64, kTcMinSteps = 8;
 constexpr int kTcNone = INT32_MIN;   // in place of a block: no such key
 constexpr float kTcLog2E = 1.4426950408889634f, kTcSlack = 8.0f;
-
-// keys of a tile: 128, 64 where the queries' second terms take the room
-template <int T>
-struct TcTile {
-    static constexpr int keys = T == 1 ? 128 : 64;
-};
 
 struct TcItem {
     int r, head, cb;              // request, key / value head, number of the 256 vectors
@@ -208,10 +203,10 @@ struct TcJoin {   // what a part has to join: the item that ends in it
 
 template <int D, int T>
 struct TcShared {
-    static constexpr int KT = TcTile<T>::keys, atoms = D / 64;
+    static constexpr int KT = kTcKeys, atoms = D / 64, stages = T == 1 ? 4 : 3;
     static constexpr int q_atom = 128 * 128, k_atom = KT * 128;
     static constexpr int q_bytes = 2 * T * atoms * q_atom, stage = 2 * atoms * k_atom;
-    static constexpr int bytes = 1024 + q_bytes + kTcStages * stage;
+    static constexpr int bytes = 1024 + q_bytes + stages * stage;
 };
 
 __device__ __forceinline__ void tc_st(uint32_t addr, const uint32_t (&v)[16]) {
@@ -224,26 +219,21 @@ __device__ __forceinline__ uint64_t tc_desc_mn(uint32_t addr, uint32_t next) {
     const uint32_t lo = ((addr >> 4) & 0x3FFFu) | ((next >> 4) << 16), hi = (1024u >> 4) | (1u << 14) | (2u << 29);
     return ((uint64_t)hi << 32) | lo;
 }
-// loads of 32 columns without a wait, and the wait, which the loaded registers depend on
-__device__ __forceinline__ void tc_ld(uint32_t addr, uint32_t (&v)[32]) {
+// 64 columns, and the wait for them in the same statement: a register of the load must not be touched in between
+__device__ __forceinline__ void tc_ld64(uint32_t addr, uint32_t (&v)[2][32]) {
     asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n"
-        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]),
-          "=r"(v[14]), "=r"(v[15]), "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]),
-          "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
-        : "r"(addr));
-}
-__device__ __forceinline__ void tc_tie(uint32_t (&v)[32]) {
-    asm volatile("" : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]), "+r"(v[8]), "+r"(v[9]), "+r"(v[10]), "+r"(v[11]), "+r"(v[12]), "+r"(v[13]),
-                      "+r"(v[14]), "+r"(v[15]), "+r"(v[16]), "+r"(v[17]), "+r"(v[18]), "+r"(v[19]), "+r"(v[20]), "+r"(v[21]), "+r"(v[22]), "+r"(v[23]), "+r"(v[24]), "+r"(v[25]), "+r"(v[26]),
-                      "+r"(v[27]) : : "memory");
-    asm volatile("" : "+r"(v[28]), "+r"(v[29]), "+r"(v[30]), "+r"(v[31]) : : "memory");
-}
-__device__ __forceinline__ void tc_ld_wait(uint32_t (&a)[32], uint32_t (&b)[32]) {
-    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-    tc_tie(a);
-    tc_tie(b);
+        "tcgen05.ld.sync.aligned.32x32b.x64.b32 {"
+        "%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32,%33,%34,%35,%36,%37,%38,%39,"
+        "%40,%41,%42,%43,%44,%45,%46,%47,%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63"
+        "}, [%64];\n tcgen05.wait::ld.sync.aligned;"
+        : "=r"(v[0][0]), "=r"(v[0][1]), "=r"(v[0][2]), "=r"(v[0][3]), "=r"(v[0][4]), "=r"(v[0][5]), "=r"(v[0][6]), "=r"(v[0][7]), "=r"(v[0][8]), "=r"(v[0][9]), "=r"(v[0][10]),
+          "=r"(v[0][11]), "=r"(v[0][12]), "=r"(v[0][13]), "=r"(v[0][14]), "=r"(v[0][15]), "=r"(v[0][16]), "=r"(v[0][17]), "=r"(v[0][18]), "=r"(v[0][19]), "=r"(v[0][20]), "=r"(v[0][21]),
+          "=r"(v[0][22]), "=r"(v[0][23]), "=r"(v[0][24]), "=r"(v[0][25]), "=r"(v[0][26]), "=r"(v[0][27]), "=r"(v[0][28]), "=r"(v[0][29]), "=r"(v[0][30]), "=r"(v[0][31]), "=r"(v[1][0]),
+          "=r"(v[1][1]), "=r"(v[1][2]), "=r"(v[1][3]), "=r"(v[1][4]), "=r"(v[1][5]), "=r"(v[1][6]), "=r"(v[1][7]), "=r"(v[1][8]), "=r"(v[1][9]), "=r"(v[1][10]), "=r"(v[1][11]),
+          "=r"(v[1][12]), "=r"(v[1][13]), "=r"(v[1][14]), "=r"(v[1][15]), "=r"(v[1][16]), "=r"(v[1][17]), "=r"(v[1][18]), "=r"(v[1][19]), "=r"(v[1][20]), "=r"(v[1][21]), "=r"(v[1][22]),
+          "=r"(v[1][23]), "=r"(v[1][24]), "=r"(v[1][25]), "=r"(v[1][26]), "=r"(v[1][27]), "=r"(v[1][28]), "=r"(v[1][29]), "=r"(v[1][30]), "=r"(v[1][31])
+        : "r"(addr)
+        : "memory");
 }
 // A role's registers, of the 640 threads x 96 = 61440 that the block is launched with: 256 x 152 + 256 x 64 + 128 x 40 = 60416.
 template <int N>
@@ -257,16 +247,16 @@ template <int FMT, int D, int T>
 __global__ void __launch_bounds__(kTcThreads, 1) kv_attn_tc_kernel(const KvAttn a, float *records, TcJoin *joins) {
     typedef TcShared<D, T> Sh;
     typedef CodePairs<FMT> Codes;
-    constexpr int KT = Sh::KT, ATOMS = Sh::atoms, SUBS = KT / 16;
+    constexpr int KT = Sh::KT, ATOMS = Sh::atoms, SUBS = KT / 16, STAGES = Sh::stages;
     extern __shared__ __align__(1024) uint8_t tc_smem_raw[];
     uint8_t *smem = tc_smem_raw + (-smem_u32(tc_smem_raw) & 1023u);
-    __shared__ __align__(8) uint64_t bars[2 * kTcStages + 11];   // full, empty; q_full, s_full, p_full (64 keys each), o_done of two groups; drain
-    __shared__ int2 sub_info[kTcStages][SUBS];                  // exponent bytes of keys and values of every 16 keys; x < 0: unseen
+    __shared__ __align__(8) uint64_t bars[2 * STAGES + 15];   // full, empty; of two groups q_full, and two places each of s_full, p_full, o_done; drain
+    __shared__ __align__(16) int2 sub_info[STAGES][SUBS];                  // exponent bytes of keys and values of every 16 keys; x < 0: unseen
     __shared__ uint32_t tmem_s;
     __shared__ int found[4];
     __shared__ int64_t sums[33];
     const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xFFFFFFFFu, tid >> 5, 0);
-    const uint32_t full = smem_u32(bars), empty = full + 8 * kTcStages, qf = empty + 8 * kTcStages, sf = qf + 16, pf = sf + 16, of = pf + 32, drain = of + 16;
+    const uint32_t full = smem_u32(bars), empty = full + 8 * STAGES, qf = empty + 8 * STAGES, sf = qf + 16, pf = sf + 32, of = pf + 32, drain = of + 32;
     pdl_prologue();
     pdl_release();
     const TcPlan plan = tc_plan<KT>(a, gridDim.x, found, sums);
@@ -275,16 +265,18 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attn_tc_kernel(const KvAttn 
         return;
     }
     if (tid == 0) {
-        for (int i = 0; i < kTcStages; i++) {
+        for (int i = 0; i < STAGES; i++) {
             mbar_init(full + 8 * i, 8);
             mbar_init(empty + 8 * i, 1);
         }
         for (int w = 0; w < 2; w++) {
             mbar_init(qf + 8 * w, 1);
-            mbar_init(sf + 8 * w, 1);
+            mbar_init(sf + 16 * w, 1);
+            mbar_init(sf + 16 * w + 8, 1);
             mbar_init(pf + 16 * w, 4);
             mbar_init(pf + 16 * w + 8, 4);
-            mbar_init(of + 8 * w, 1);
+            mbar_init(of + 16 * w, 1);
+            mbar_init(of + 16 * w + 8, 1);
         }
         mbar_init(drain, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -296,7 +288,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attn_tc_kernel(const KvAttn 
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = __shfl_sync(0xFFFFFFFFu, tmem_s, 0);   // of group w: O at 256 w, S and P at 256 w + 128
+    const uint32_t tmem = __shfl_sync(0xFFFFFFFFu, tmem_s, 0);   // of group w: O at 256 w, S and P at 256 w + 128 and 64 on
     uint8_t *stages = smem + Sh::q_bytes;
     bool ok = true;
     TcWalk<KT> walk(a, plan, found);
@@ -307,7 +299,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attn_tc_kernel(const KvAttn 
         // ---------------- softmax ----------------
         tc_registers<152>();
         const int w = warp >> 2, me = tid & 127;
-        const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16, o_t = tmem + 256 * w + lane_base, s_t = o_t + 128;
+        const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16, o_t = tmem + 256 * w + lane_base;
         uint8_t *q_s = smem + w * T * ATOMS * Sh::q_atom;
         int nw = 0;   // this group's tiles
         while (ok && walk.next(it)) {
@@ -374,6 +366,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attn_tc_kernel(const KvAttn 
             float m = 0.0f, mv = 0.0f, l = 0.0f, thr = -INFINITY, thv = -INFINITY;
             // A tile of keys, starting at key0; CLEAR: every vector of the warp sees all of it.
             auto tile = [&](auto clear, int st, int key0, bool first) {
+                const uint32_t s_t = o_t + 128 + 64 * (nw & 1);
                 constexpr bool CLEAR = decltype(clear)::value;
                 uint32_t seen[KT / 32];   // a bit per key
                 if constexpr (!CLEAR) {
@@ -388,25 +381,25 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attn_tc_kernel(const KvAttn 
                 // ---- maxima: of the scores, and of scores + value exponents
                 float mt = -INFINITY, vt = -INFINITY;
                 uint32_t x[2][32];
+                float lf[SUBS], fk[SUBS];   // of 16 keys: value exponent (then the weights' factor), the scores' factor
+                tc_ld64(s_t, x);
+                {
 #pragma unroll
-                for (int h = 0; h < KT / 64; h++) {
-                    tc_ld(s_t + 64 * h, x[0]);
-                    tc_ld(s_t + 64 * h + 32, x[1]);
-                    tc_ld_wait(x[0], x[1]);
-#pragma unroll
-                    for (int b = 0; b < 4; b++) {
-                        const int2 info = sub_info[st][4 * h + b];
+                    for (int b = 0; b < SUBS; b++) {
+                        const int2 info = sub_info[st][b];
+                        fk[b] = fac * pow2_byte(max(info.x, 0));
+                        lf[b] = (float)(info.y - 127);
                         float t[2] = {-INFINITY, -INFINITY};
 #pragma unroll
                         for (int i = 0; i < 16; i++) {
                             float v = __uint_as_float(x[b >> 1][16 * (b & 1) + i]);
-                            if (!CLEAR) v = seen[2 * h + (b >> 1)] >> (16 * (b & 1) + i) & 1u ? v : -INFINITY;
+                            if (!CLEAR) v = seen[b >> 1] >> (16 * (b & 1) + i) & 1u ? v : -INFINITY;
                             t[i & 1] = fmaxf(t[i & 1], v);
                         }
                         float top = fmaxf(t[0], t[1]);
-                        if (CLEAR || top > -INFINITY) top *= fac * pow2_byte(info.x);   // (the factor can be zero)
+                        if (CLEAR || top > -INFINITY) top *= fk[b];   // (the factor can be zero)
                         mt = fmaxf(mt, top);
-                        vt = fmaxf(vt, top + (float)(info.y - 127));
+                        vt = fmaxf(vt, top + lf[b]);
                     }
                 }
                 // ---- references
@@ -426,7 +419,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attn_tc_kernel(const KvAttn 
                         thv = vn + kTcSlack;
                     }
                     if (!first && __any_sync(0xFFFFFFFFu, f != 1.0f)) {
-                        ok = __all_sync(0xFFFFFFFFu, mbar_wait_fast(of + 8 * w, (nw - 1) & 1));
+                        ok = __all_sync(0xFFFFFFFFu, mbar_wait_fast(of + 8 * (2 * w + ((nw - 1) & 1)), ((nw - 1) >> 1) & 1));
                         if (!ok) return;
                         tc_fence_after();
 #pragma unroll 1
@@ -442,64 +435,55 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attn_tc_kernel(const KvAttn 
                         }
                     }
                 }
-                // ---- weights (two terms: the scores of the tile's 64 keys are still there)
-                const float fv0 = m - mv - 127.0f;
+                // ---- weights: w = 2^(s - m + lf); the sum takes 2^-lf of the 16 together (below 2^-56 a weight is zero in f16 either way)
+                {
 #pragma unroll
-                for (int h = 0; h < KT / 64; h++) {
-                    if (KT > 64) {
-                        tc_ld(s_t + 64 * h, x[0]);
-                        tc_ld(s_t + 64 * h + 32, x[1]);
-                        tc_ld_wait(x[0], x[1]);
-                    }
+                    for (int b = 0; b < SUBS; b++) lf[b] = fmaxf(lf[b] + (m - mv), -64.0f);
 #pragma unroll
                     for (int c = 0; c < 2; c++) {
                         uint32_t hw[16], lw[16];
 #pragma unroll
                         for (int b = 0; b < 2; b++) {
-                            const int2 info = sub_info[st][4 * h + 2 * c + b];
-                            // w = 2^(s - m + lf); the sum takes 2^-lf of the 16 together (below 2^-56 a weight is zero in f16 either way)
-                            const float fk = fac * pow2_byte(max(info.x, 0)), lf = fmaxf(fv0 + (float)info.y, -64.0f);
-                            const float2 nm = make_float2(lf - m, lf - m);
+                            const float2 f2 = make_float2(fk[2 * c + b], fk[2 * c + b]), nm = make_float2(lf[2 * c + b] - m, lf[2 * c + b] - m);
                             float2 sum = make_float2(0.0f, 0.0f);
 #pragma unroll
                             for (int i = 0; i < 16; i += 2) {
                                 const int k = 16 * b + i;
-                                float2 y = __ffma2_rn(make_float2(__uint_as_float(x[c][k]), __uint_as_float(x[c][k + 1])), make_float2(fk, fk), nm);
+                                float2 y = __ffma2_rn(make_float2(__uint_as_float(x[c][k]), __uint_as_float(x[c][k + 1])), f2, nm);
                                 if (!CLEAR) {
-                                    y.x = seen[2 * h + c] >> k & 1u ? y.x : -INFINITY;
-                                    y.y = seen[2 * h + c] >> (k + 1) & 1u ? y.y : -INFINITY;
+                                    y.x = seen[c] >> k & 1u ? y.x : -INFINITY;
+                                    y.y = seen[c] >> (k + 1) & 1u ? y.y : -INFINITY;
                                 }
                                 const float2 v = make_float2(kv_ex2(y.x), kv_ex2(y.y));
                                 sum = __fadd2_rn(sum, v);
                                 if (T == 2) kv_split(v.x, v.y, hw[k / 2], lw[k / 2]);
                                 else hw[k / 2] = half_bits(__floats2half2_rn(v.x, v.y));
                             }
-                            l = fmaf(sum.x + sum.y, kv_ex2(-lf), l);
+                            l = fmaf(sum.x + sum.y, kv_ex2(-lf[2 * c + b]), l);
                         }
-                        tc_st(s_t + 32 * h + 16 * c, hw);
+                        tc_st(s_t + 16 * c, hw);
                         if (T == 2) tc_st(s_t + 32 + 16 * c, lw);
                     }
-                    // the products of these 64 keys may begin
                     asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
                     tc_fence_before();
                     __syncwarp();
-                    if (elect_one()) mbar_arrive(pf + 8 * (2 * w + h));
+                    if (elect_one()) mbar_arrive(pf + 8 * (2 * w + (nw & 1)));
                 }
             };
+            // (o_done has two places as well: a warp can be done with a tile before the product of the one before is, and a parity tells two
+            // phases apart; the scores of a tile are there only when the product of two tiles before is done)
             for (int s = it.s0; s < it.s1 && ok; s++, n++, nw++) {
-                const int st = n % kTcStages, key0 = (it.first + s) * KT;
+                const int st = n % STAGES, key0 = (it.first + s) * KT;
                 // (the scores first: behind them the tile's barrier is in the phase asked for, whatever tiles this group has skipped)
-                ok = __all_sync(0xFFFFFFFFu, mbar_wait_fast(sf + 8 * w, nw & 1) && mbar_wait_fast(full + 8 * st, (n / kTcStages) & 1));
+                ok = __all_sync(0xFFFFFFFFu, mbar_wait_fast(sf + 8 * (2 * w + (nw & 1)), (nw >> 1) & 1) && mbar_wait_fast(full + 8 * st, (n / STAGES) & 1));
                 if (!ok) break;
                 tc_fence_after();
-                bool all = pos - key0 >= KT - 1 && low <= key0;
-#pragma unroll
-                for (int b = 0; b < SUBS; b++) all = all && sub_info[st][b].x >= 0;
-                if (__all_sync(0xFFFFFFFFu, all)) tile(std::true_type(), st, key0, s == it.s0);
+                const int4 i0 = *reinterpret_cast<const int4 *>(&sub_info[st][0]), i1 = *reinterpret_cast<const int4 *>(&sub_info[st][2]);
+                if (__all_sync(0xFFFFFFFFu, pos - key0 >= KT - 1 && low <= key0 && (i0.x | i0.z | i1.x | i1.z) >= 0)) tile(std::true_type(), st, key0, s == it.s0);
                 else tile(std::false_type(), st, key0, s == it.s0);
             }
             if (!ok) break;
-            ok = __all_sync(0xFFFFFFFFu, mbar_wait_fast(of + 8 * w, (nw - 1) & 1));
+            ok = __all_sync(0xFFFFFFFFu, mbar_wait_fast(of + 8 * (2 * w + ((nw - 1) & 1)), ((nw - 1) >> 1) & 1));
             if (!ok) break;
             tc_fence_after();
             const bool whole = it.s0 == 0 && it.s1 == it.steps, mine = w * 128 + me < it.vecs, none = !(thr > -INFINITY) && l == 0.0f;
@@ -551,12 +535,15 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attn_tc_kernel(const KvAttn 
             uint4 k[PER], v[PER];
             int blk[PER];   // of the next tile's chunks
             int2 info = make_int2(-1, 127);
+            int info_blk = kTcNone;
             const int key_of = pt / CH, c = pt % CH;   // chunk i of this thread: 16 bytes c of key key_of + 256 / CH i
             constexpr int KEYS = 256 / CH;
             auto blocks = [&](int s) {
                 const int key0 = (it.first + s) * KT + key_of;
 #pragma unroll
                 for (int i = 0; i < PER; i++) blk[i] = s < it.s1 && key0 + KEYS * i < it.length ? table[(key0 + KEYS * i) >> a.shift] : kTcNone;
+                const int key = (it.first + s) * KT + 16 * pt;
+                info_blk = pt < SUBS && s < it.s1 && key < it.length ? table[key >> a.shift] : kTcNone;
             };
             auto load = [&](const uint8_t *codes, int s, uint4 (&x)[PER]) {
                 const int key0 = (it.first + s) * KT + key_of;
@@ -569,11 +556,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attn_tc_kernel(const KvAttn 
                         atomicExch(a.status, kStatusIndex);
                 }
             };
-            auto bytes = [&](int s) {
-                const int key = (it.first + s) * KT + 16 * pt;
-                const int b = pt < SUBS && s < it.s1 && key < it.length ? table[key >> a.shift] : kTcNone;
-                const int64_t bh = (int64_t)b * a.kv_heads + it.head;
-                info = b >= 0 && b < a.blocks ? make_int2(a.k_exp[bh], a.v_exp[bh]) : make_int2(-1, 127);
+            auto bytes = [&]() {
+                const int64_t bh = (int64_t)info_blk * a.kv_heads + it.head;
+                info = info_blk >= 0 && info_blk < a.blocks ? make_int2(a.k_exp[bh], a.v_exp[bh]) : make_int2(-1, 127);
             };
             auto store = [&](uint8_t *dst, const uint4 (&x)[PER]) {
                 const int flip = (c >> 2) & 1, c8 = (c & 3) * 2;   // (neighbours of two pieces store their halves in turn: no bank twice)
@@ -590,11 +575,11 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attn_tc_kernel(const KvAttn 
             blocks(it.s0);
             load(a.k, it.s0, k);
             load(a.v, it.s0, v);
-            bytes(it.s0);
+            bytes();
             blocks(it.s0 + 1);
             for (int s = it.s0; s < it.s1; s++, n++) {
-                const int st = n % kTcStages;
-                if (n >= kTcStages) ok = __all_sync(0xFFFFFFFFu, mbar_wait_fast(empty + 8 * st, (n / kTcStages - 1) & 1));
+                const int st = n % STAGES;
+                if (n >= STAGES) ok = __all_sync(0xFFFFFFFFu, mbar_wait_fast(empty + 8 * st, (n / STAGES - 1) & 1));
                 if (!ok) break;
                 uint8_t *k_s = stages + st * Sh::stage, *v_s = k_s + ATOMS * Sh::k_atom;
                 store(k_s, k);
@@ -605,7 +590,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attn_tc_kernel(const KvAttn 
                 fence_async_smem();
                 __syncwarp();
                 if (elect_one()) mbar_arrive(full + 8 * st);
-                bytes(s + 1);
+                bytes();
                 blocks(s + 2);
             }
         }
@@ -621,7 +606,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attn_tc_kernel(const KvAttn 
             ok = ok && __all_sync(0xFFFFFFFFu, mbar_wait_fast(bar, count & 1));
             return ok;
         };
-        auto scores = [&](int w, int st) {
+        auto scores = [&](int w, int st, int place) {
             if (elect_one()) {
                 const uint32_t qa = smem_u32(smem + w * T * ATOMS * Sh::q_atom), ka = smem_u32(stages + st * Sh::stage);
 #pragma unroll
@@ -630,9 +615,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attn_tc_kernel(const KvAttn 
                     for (int at = 0; at < ATOMS; at++) {
                         const uint64_t dq = smem_desc(qa + (x * ATOMS + at) * Sh::q_atom), dk = smem_desc(ka + at * Sh::k_atom);
 #pragma unroll
-                        for (int k = 0; k < 4; k++) umma_bf16(tmem + 256 * w + 128, dq + 2 * k, dk + 2 * k, id_s, x < T - 1 || (at | k) != 0);
+                        for (int k = 0; k < 4; k++) umma_bf16(tmem + 256 * w + 128 + 64 * place, dq + 2 * k, dk + 2 * k, id_s, x < T - 1 || (at | k) != 0);
                     }
-                umma_commit(sf + 8 * w);
+                umma_commit(sf + 8 * (2 * w + place));
             }
             __syncwarp();
         };
@@ -640,39 +625,34 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attn_tc_kernel(const KvAttn 
             const int groups = it.vecs > 128 ? 2 : 1, steps = it.s1 - it.s0;
             if (it.s0 > 0 && it.s1 == it.steps) join = {(int)((plan.begin - it.s0) / plan.chunk), it.vecs, it.row0 + it.vec0 / a.group, it.head * a.group, it.vec0 % a.group, {0, 0, 0}};
             for (int w = 0; w < groups; w++) wait(qf + 8 * w, items[w]++);
-            if (!wait(full + 8 * (n % kTcStages), n / kTcStages)) break;
-            tc_fence_after();
-            for (int w = 0; w < groups; w++) scores(w, n % kTcStages);
-            for (int s = 0; s < steps && ok; s++, n++) {
-                const int st = n % kTcStages, st1 = (n + 1) % kTcStages;
+            for (int s = -1; s < steps && ok; s++) {
+                if (s + 1 < steps) {   // the next tile's scores
+                    const int st = (n + 1 + s) % STAGES;
+                    if (!wait(full + 8 * st, (n + 1 + s) / STAGES)) break;
+                    tc_fence_after();
+                    for (int w = 0; w < groups; w++) scores(w, st, (nw[w] + 1 + s) & 1);
+                }
+                if (s < 0) continue;
+                const int st = (n + s) % STAGES;
                 for (int w = 0; w < groups; w++) {
+                    const int place = (nw[w] + s) & 1;
+                    if (!wait(pf + 8 * (2 * w + place), (nw[w] + s) >> 1)) break;
+                    tc_fence_after();
+                    if (elect_one()) {
+                        const uint32_t va = smem_u32(stages + st * Sh::stage + ATOMS * Sh::k_atom), pa = tmem + 256 * w + 128 + 64 * place;
+                        const uint64_t dv = tc_desc_mn(va, Sh::k_atom);
 #pragma unroll
-                    for (int h = 0; h < KT / 64; h++) {
-                        if (!wait(pf + 8 * (2 * w + h), nw[w])) break;
-                        tc_fence_after();
-                        if (elect_one()) {
-                            const uint32_t va = smem_u32(stages + st * Sh::stage + ATOMS * Sh::k_atom) + h * 64 * 128, pa = tmem + 256 * w + 128 + 32 * h;
-                            const uint64_t dv = tc_desc_mn(va, Sh::k_atom);
+                        for (int x = T - 1; x >= 0; x--)
 #pragma unroll
-                            for (int x = T - 1; x >= 0; x--)
-#pragma unroll
-                                for (int k = 0; k < 4; k++) umma_ts(tmem + 256 * w, pa + 32 * x + 8 * k, dv + (2048 >> 4) * k, id_o, s > 0 || h > 0 || x < T - 1 || k != 0);
-                            if (h == KT / 64 - 1) {
-                                umma_commit(of + 8 * w);
-                                if (w == groups - 1) umma_commit(empty + 8 * st);
-                            }
-                        }
-                        __syncwarp();
+                            for (int k = 0; k < KT / 16; k++) umma_ts(tmem + 256 * w, pa + 32 * x + 8 * k, dv + (2048 >> 4) * k, id_o, s > 0 || x < T - 1 || k != 0);
+                        umma_commit(of + 8 * (2 * w + place));
+                        if (w == groups - 1) umma_commit(empty + 8 * st);
                     }
-                    if (!ok) break;
-                    nw[w]++;
-                    if (s + 1 < steps) {
-                        if (w == 0 && !wait(full + 8 * st1, (n + 1) / kTcStages)) break;
-                        tc_fence_after();
-                        scores(w, st1);
-                    }
+                    __syncwarp();
                 }
             }
+            n += steps;
+            for (int w = 0; w < groups; w++) nw[w] += steps;
         }
         if (lane == 0) joins[blockIdx.x] = join;
         // MMAs that were issued may still read shared memory and write tensor memory
