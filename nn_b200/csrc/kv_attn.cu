@@ -31,7 +31,7 @@ namespace nnq {
 constexpr int kKvWarps = 8, kKvCols = 8, kKvStep = 16, kKvStages = 3;
 constexpr int kKvMinSteps = kKvWarps;   // of a CTA's part
 constexpr int kKvPad = 16;
-constexpr int kFew = 32;   // see nnq_kv_attention
+constexpr int kFew = 64;   // see nnq_kv_attention
 constexpr int kNothing = INT32_MIN;   // in place of a block: no key of the step is seen
 constexpr float kKvLog2E = 1.4426950408889634f;
 constexpr float kKvSlack = 8.0f;   // a score may pass the reference by this power of two: weights up to 256 in f16

@@ -52,6 +52,11 @@ struct CodePairs<NNQ_KV_INT8> {
     // bytes 0, 1 (2, 3) of a word
     static __device__ __forceinline__ uint32_t low(uint32_t w) { return half(__byte_perm(w, 0x64646464u, 0x4140)); }
     static __device__ __forceinline__ uint32_t high(uint32_t w) { return half(__byte_perm(w, 0x64646464u, 0x4342)); }
+    // the four codes of a word
+    static __device__ __forceinline__ void four(uint32_t w, uint32_t &p0, uint32_t &p1) {
+        p0 = low(word(w));
+        p1 = high(word(w));
+    }
     // bytes i of x and y side by side, i = 0 .. 3
     static __device__ __forceinline__ void pairs(uint32_t x, uint32_t y, uint32_t &p0, uint32_t &p1, uint32_t &p2, uint32_t &p3) {
         const uint32_t u = __byte_perm(word(x), word(y), 0x5140), v = __byte_perm(word(x), word(y), 0x7362);
@@ -68,6 +73,12 @@ struct CodePairs<NNQ_KV_E4M3> {
     static __device__ __forceinline__ uint32_t half(uint32_t x) { return (x & 0x80008000u) | ((x >> 1) & 0x3F803F80u); }
     static __device__ __forceinline__ uint32_t low(uint32_t w) { return half(__byte_perm(w, 0, 0x1404)); }
     static __device__ __forceinline__ uint32_t high(uint32_t w) { return half(__byte_perm(w, 0, 0x3424)); }
+    // (the upper bytes of the f16 numbers of all four codes, and the lower ones, then put together)
+    static __device__ __forceinline__ void four(uint32_t w, uint32_t &p0, uint32_t &p1) {
+        const uint32_t up = (w & 0x80808080u) | (((w & 0x7F7F7F7Fu) >> 1) & 0x7F7F7F7Fu), down = (w << 7) & 0x80808080u;
+        p0 = __byte_perm(down, up, 0x5140);
+        p1 = __byte_perm(down, up, 0x7362);
+    }
     static __device__ __forceinline__ void pairs(uint32_t x, uint32_t y, uint32_t &p0, uint32_t &p1, uint32_t &p2, uint32_t &p3) {
         p0 = half(__byte_perm(x, y, 0x4400));   // (the lower bytes of the halves are masked out)
         p1 = half(__byte_perm(x, y, 0x5511));

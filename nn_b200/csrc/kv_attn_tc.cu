@@ -9,8 +9,9 @@
 //                   memory; a reference moves only when a score passes it by 2^8, and then the sums there are scaled.
 //   warps 8-15:     codes from the blocks of the table to f16 tiles in shared memory, swizzled as the products read them, keys and values
 //                   as they lie (the values are the MN-major operand); the next tile's codes are under way meanwhile.
-//   warp 16:        (three more complete its group) one lane issues the MMAs: S(t + 1) of both groups, then O += P(t) V(t) of each. MMAs run in the order they are
-//                   issued, so S(t + 1) may overwrite the weights of t - 1, whose product stands in front of it.
+//   warps 16, 17:   (two more complete their group) a lane of each issues the MMAs of one softmax group: S(t + 1), then O += P(t) V(t). They
+//                   run in the order they are issued, so S(t + 1) may overwrite the weights of t - 1, whose product stands in front
+//                   of it. (One warp for both groups took 100 clocks an MMA beside the scheduler's other warps and set the pace.)
 // What bounds it is the softmax: of the exponentials a thread forms, the special function unit takes 16 a clock and SM. Codes are exact in f16. T = 1 (bf16 queries and outputs): a query vector is
 // exact under its power of two, a weight is one f16 number, off by up to 2^-11 of itself where the output's own rounding is 2^-8 of it. T = 2 (f32
 // on either side): both have two terms, 22 bits.
@@ -235,11 +236,16 @@ __device__ __forceinline__ void tc_ld64(uint32_t addr, uint32_t (&v)[2][32]) {
         : "r"(addr)
         : "memory");
 }
-// A role's registers, of the 640 threads x 96 = 61440 that the block is launched with: 256 x 152 + 256 x 64 + 128 x 40 = 60416.
+// A role's registers, of the 640 threads x 96 = 61440 that the block is launched with: 256 x 152 + 256 x 64 + 128 x 48 = 61440.
 template <int N>
 __device__ __forceinline__ void tc_registers() {
     if constexpr (N > 96) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
     else asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
 }
 __device__ __forceinline__ void group_sync(int w) { asm volatile("bar.sync %0, 128;" ::"r"(1 + w) : "memory"); }
 
@@ -250,7 +256,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attn_tc_kernel(const KvAttn 
     constexpr int KT = Sh::KT, ATOMS = Sh::atoms, SUBS = KT / 16, STAGES = Sh::stages;
     extern __shared__ __align__(1024) uint8_t tc_smem_raw[];
     uint8_t *smem = tc_smem_raw + (-smem_u32(tc_smem_raw) & 1023u);
-    __shared__ __align__(8) uint64_t bars[2 * STAGES + 15];   // full, empty; of two groups q_full, and two places each of s_full, p_full, o_done; drain
+    __shared__ __align__(8) uint64_t bars[2 * STAGES + 16];   // full, empty; of two groups q_full, and two places each of s_full, p_full, o_done; drain
     __shared__ __align__(16) int2 sub_info[STAGES][SUBS];                  // exponent bytes of keys and values of every 16 keys; x < 0: unseen
     __shared__ uint32_t tmem_s;
     __shared__ int found[4];
@@ -267,7 +273,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attn_tc_kernel(const KvAttn 
     if (tid == 0) {
         for (int i = 0; i < STAGES; i++) {
             mbar_init(full + 8 * i, 8);
-            mbar_init(empty + 8 * i, 1);
+            mbar_init(empty + 8 * i, 2);
         }
         for (int w = 0; w < 2; w++) {
             mbar_init(qf + 8 * w, 1);
@@ -279,6 +285,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attn_tc_kernel(const KvAttn 
             mbar_init(of + 16 * w + 8, 1);
         }
         mbar_init(drain, 1);
+        mbar_init(drain + 8, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 16) {
@@ -365,7 +372,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attn_tc_kernel(const KvAttn 
             const float fac = a.scale * kTcLog2E * Codes::unscale * kv_top_unscale(big);
             float m = 0.0f, mv = 0.0f, l = 0.0f, thr = -INFINITY, thv = -INFINITY;
             // A tile of keys, starting at key0; CLEAR: every vector of the warp sees all of it.
-            auto tile = [&](auto clear, int st, int key0, bool first) {
+            auto tile = [&](auto clear, const int2 *sub, int key0, bool first) {
                 const uint32_t s_t = o_t + 128 + 64 * (nw & 1);
                 constexpr bool CLEAR = decltype(clear)::value;
                 uint32_t seen[KT / 32];   // a bit per key
@@ -374,8 +381,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attn_tc_kernel(const KvAttn 
                     for (int c = 0; c < KT / 32; c++) {
                         const int hi = pos - key0 - 32 * c, lo = low - key0 - 32 * c;   // visible keys of the 32: lo .. hi
                         seen[c] = (hi >= 31 ? 0xFFFFFFFFu : hi < 0 ? 0u : (2u << hi) - 1u) & (lo <= 0 ? 0xFFFFFFFFu : lo > 31 ? 0u : 0xFFFFFFFFu << lo);
-                        if (sub_info[st][2 * c].x < 0) seen[c] &= 0xFFFF0000u;
-                        if (sub_info[st][2 * c + 1].x < 0) seen[c] &= 0xFFFFu;
+                        if (sub[2 * c].x < 0) seen[c] &= 0xFFFF0000u;
+                        if (sub[2 * c + 1].x < 0) seen[c] &= 0xFFFFu;
                     }
                 }
                 // ---- maxima: of the scores, and of scores + value exponents
@@ -386,17 +393,16 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attn_tc_kernel(const KvAttn 
                 {
 #pragma unroll
                     for (int b = 0; b < SUBS; b++) {
-                        const int2 info = sub_info[st][b];
+                        const int2 info = sub[b];
                         fk[b] = fac * pow2_byte(max(info.x, 0));
                         lf[b] = (float)(info.y - 127);
-                        float t[2] = {-INFINITY, -INFINITY};
+                        float t[16];
 #pragma unroll
                         for (int i = 0; i < 16; i++) {
-                            float v = __uint_as_float(x[b >> 1][16 * (b & 1) + i]);
-                            if (!CLEAR) v = seen[b >> 1] >> (16 * (b & 1) + i) & 1u ? v : -INFINITY;
-                            t[i & 1] = fmaxf(t[i & 1], v);
+                            t[i] = __uint_as_float(x[b >> 1][16 * (b & 1) + i]);
+                            if (!CLEAR) t[i] = seen[b >> 1] >> (16 * (b & 1) + i) & 1u ? t[i] : -INFINITY;
                         }
-                        float top = fmaxf(t[0], t[1]);
+                        float top = max3(max3(max3(t[0], t[1], t[2]), max3(t[3], t[4], t[5]), max3(t[6], t[7], t[8])), max3(t[9], t[10], t[11]), max3(t[12], t[13], fmaxf(t[14], t[15])));
                         if (CLEAR || top > -INFINITY) top *= fk[b];   // (the factor can be zero)
                         mt = fmaxf(mt, top);
                         vt = fmaxf(vt, top + lf[b]);
@@ -478,9 +484,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attn_tc_kernel(const KvAttn 
                 ok = __all_sync(0xFFFFFFFFu, mbar_wait_fast(sf + 8 * (2 * w + (nw & 1)), (nw >> 1) & 1) && mbar_wait_fast(full + 8 * st, (n / STAGES) & 1));
                 if (!ok) break;
                 tc_fence_after();
-                const int4 i0 = *reinterpret_cast<const int4 *>(&sub_info[st][0]), i1 = *reinterpret_cast<const int4 *>(&sub_info[st][2]);
-                if (__all_sync(0xFFFFFFFFu, pos - key0 >= KT - 1 && low <= key0 && (i0.x | i0.z | i1.x | i1.z) >= 0)) tile(std::true_type(), st, key0, s == it.s0);
-                else tile(std::false_type(), st, key0, s == it.s0);
+                const int2 *sub = sub_info[st];
+                const int4 i0 = *reinterpret_cast<const int4 *>(sub), i1 = *reinterpret_cast<const int4 *>(sub + 2);
+                if (__all_sync(0xFFFFFFFFu, pos - key0 >= KT - 1 && low <= key0 && (i0.x | i0.z | i1.x | i1.z) >= 0)) tile(std::true_type(), sub, key0, s == it.s0);
+                else tile(std::false_type(), sub, key0, s == it.s0);
             }
             if (!ok) break;
             ok = __all_sync(0xFFFFFFFFu, mbar_wait_fast(of + 8 * (2 * w + ((nw - 1) & 1)), ((nw - 1) >> 1) & 1));
@@ -528,137 +535,127 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attn_tc_kernel(const KvAttn 
     } else if (warp < 16) {
         // ---------------- codes to f16 tiles ----------------
         tc_registers<64>();
-        constexpr int CH = D / 16, PER = KT * CH / 256;   // 16-byte chunks of a row, chunks of a thread
-        const int pt = tid - 256;
+        // Thread pt has 16 dimensions of every 64 of key pt / 4: four lanes read 64 bytes of a key, eight store to different banks.
+        const int pt = tid - 256, key_of = pt >> 2, c4 = pt & 3;
+        const uint32_t at_lo = swz(key_of, 2 * c4), at_hi = swz(key_of, 2 * c4 + 1);
         while (ok && walk.next(it)) {
             const int32_t *table = a.table + (int64_t)it.r * a.table_ld;
-            uint4 k[PER], v[PER];
-            int blk[PER];   // of the next tile's chunks
+            uint4 k[ATOMS], v[ATOMS];
             int2 info = make_int2(-1, 127);
-            int info_blk = kTcNone;
-            const int key_of = pt / CH, c = pt % CH;   // chunk i of this thread: 16 bytes c of key key_of + 256 / CH i
-            constexpr int KEYS = 256 / CH;
+            int blk, info_blk;   // of the next tile: this thread's key's, and (threads 0 .. SUBS - 1) that of 16 keys
             auto blocks = [&](int s) {
-                const int key0 = (it.first + s) * KT + key_of;
-#pragma unroll
-                for (int i = 0; i < PER; i++) blk[i] = s < it.s1 && key0 + KEYS * i < it.length ? table[(key0 + KEYS * i) >> a.shift] : kTcNone;
-                const int key = (it.first + s) * KT + 16 * pt;
-                info_blk = pt < SUBS && s < it.s1 && key < it.length ? table[key >> a.shift] : kTcNone;
+                const int key0 = (it.first + s) * KT, key = key0 + key_of, key16 = key0 + 16 * pt;
+                blk = s < it.s1 && key < it.length ? table[key >> a.shift] : kTcNone;
+                info_blk = pt < SUBS && s < it.s1 && key16 < it.length ? table[key16 >> a.shift] : kTcNone;
             };
-            auto load = [&](const uint8_t *codes, int s, uint4 (&x)[PER]) {
-                const int key0 = (it.first + s) * KT + key_of;
+            auto load = [&](int s) {
+                const bool there = blk >= 0 && blk < a.blocks;
+                if (!there && blk != kTcNone) atomicExch(a.status, kStatusIndex);
+                const int64_t at = ((((int64_t)blk * a.kv_heads + it.head) << a.shift) + (((it.first + s) * KT + key_of) & ((1 << a.shift) - 1))) * D + c4 * 16;
 #pragma unroll
-                for (int i = 0; i < PER; i++) {
-                    x[i] = make_uint4(0, 0, 0, 0);
-                    if (blk[i] >= 0 && blk[i] < a.blocks)
-                        x[i] = __ldg(reinterpret_cast<const uint4 *>(codes + ((((int64_t)blk[i] * a.kv_heads + it.head) << a.shift) + ((key0 + KEYS * i) & ((1 << a.shift) - 1))) * D + c * 16));
-                    else if (blk[i] != kTcNone)
-                        atomicExch(a.status, kStatusIndex);
+                for (int i = 0; i < ATOMS; i++) {
+                    k[i] = there ? __ldg(reinterpret_cast<const uint4 *>(a.k + at + 64 * i)) : make_uint4(0, 0, 0, 0);
+                    v[i] = there ? __ldg(reinterpret_cast<const uint4 *>(a.v + at + 64 * i)) : make_uint4(0, 0, 0, 0);
                 }
-            };
-            auto bytes = [&]() {
                 const int64_t bh = (int64_t)info_blk * a.kv_heads + it.head;
                 info = info_blk >= 0 && info_blk < a.blocks ? make_int2(a.k_exp[bh], a.v_exp[bh]) : make_int2(-1, 127);
             };
-            auto store = [&](uint8_t *dst, const uint4 (&x)[PER]) {
-                const int flip = (c >> 2) & 1, c8 = (c & 3) * 2;   // (neighbours of two pieces store their halves in turn: no bank twice)
-#pragma unroll
-                for (int i = 0; i < PER; i++) {
-                    const int key = key_of + KEYS * i;
-                    const uint32_t w[4] = {Codes::word(x[i].x), Codes::word(x[i].y), Codes::word(x[i].z), Codes::word(x[i].w)};
-                    const uint4 lo = make_uint4(Codes::low(w[0]), Codes::high(w[0]), Codes::low(w[1]), Codes::high(w[1])), hi = make_uint4(Codes::low(w[2]), Codes::high(w[2]), Codes::low(w[3]), Codes::high(w[3]));
-                    uint8_t *p = dst + (c >> 2) * Sh::k_atom;
-                    *reinterpret_cast<uint4 *>(p + swz(key, c8 + flip)) = flip ? hi : lo;
-                    *reinterpret_cast<uint4 *>(p + swz(key, c8 + 1 - flip)) = flip ? lo : hi;
-                }
+            auto store = [&](uint8_t *dst, const uint4 &x) {
+                uint4 lo, hi;
+                Codes::four(x.x, lo.x, lo.y);
+                Codes::four(x.y, lo.z, lo.w);
+                Codes::four(x.z, hi.x, hi.y);
+                Codes::four(x.w, hi.z, hi.w);
+                *reinterpret_cast<uint4 *>(dst + at_lo) = lo;
+                *reinterpret_cast<uint4 *>(dst + at_hi) = hi;
             };
             blocks(it.s0);
-            load(a.k, it.s0, k);
-            load(a.v, it.s0, v);
-            bytes();
+            load(it.s0);
             blocks(it.s0 + 1);
             for (int s = it.s0; s < it.s1; s++, n++) {
                 const int st = n % STAGES;
                 if (n >= STAGES) ok = __all_sync(0xFFFFFFFFu, mbar_wait_fast(empty + 8 * st, (n / STAGES - 1) & 1));
                 if (!ok) break;
                 uint8_t *k_s = stages + st * Sh::stage, *v_s = k_s + ATOMS * Sh::k_atom;
-                store(k_s, k);
-                load(a.k, s + 1, k);
-                store(v_s, v);
-                load(a.v, s + 1, v);
+#pragma unroll
+                for (int i = 0; i < ATOMS; i++) {
+                    store(k_s + i * Sh::k_atom, k[i]);
+                    store(v_s + i * Sh::k_atom, v[i]);
+                }
                 if (pt < SUBS) sub_info[st][pt] = info;
+                if (s + 1 < it.s1) load(s + 1);
                 fence_async_smem();
                 __syncwarp();
                 if (elect_one()) mbar_arrive(full + 8 * st);
-                bytes();
                 blocks(s + 2);
             }
         }
     } else {
-        tc_registers<40>();
-        if (warp == 16) {
-        // ---------------- MMA issuer (the warp waits together, one lane issues) ----------------
+        tc_registers<48>();
+        if (warp < 18) {
+        // ---------------- MMA issuers (a warp waits together, one lane issues) ----------------
+        const int w = warp - 16;
         const uint32_t id_s = (1u << 4) | ((uint32_t)(KT >> 3) << 17) | ((128u >> 4) << 24);                 // both operands f16
         const uint32_t id_o = (1u << 4) | (1u << 16) | ((uint32_t)(D >> 3) << 17) | ((128u >> 4) << 24);     // B is MN-major
-        int nw[2] = {0, 0}, items[2] = {0, 0};
+        const uint32_t qa = smem_u32(smem + w * T * ATOMS * Sh::q_atom), o_t = tmem + 256 * w;
+        int nw = 0, items = 0;
         TcJoin join = {-1, 0, 0, 0, 0, {0, 0, 0}};
         auto wait = [&](uint32_t bar, int count) {
             ok = ok && __all_sync(0xFFFFFFFFu, mbar_wait_fast(bar, count & 1));
             return ok;
         };
-        auto scores = [&](int w, int st, int place) {
-            if (elect_one()) {
-                const uint32_t qa = smem_u32(smem + w * T * ATOMS * Sh::q_atom), ka = smem_u32(stages + st * Sh::stage);
-#pragma unroll
-                for (int x = T - 1; x >= 0; x--)   // the small products first, so that their sums are rounded at their size
-#pragma unroll
-                    for (int at = 0; at < ATOMS; at++) {
-                        const uint64_t dq = smem_desc(qa + (x * ATOMS + at) * Sh::q_atom), dk = smem_desc(ka + at * Sh::k_atom);
-#pragma unroll
-                        for (int k = 0; k < 4; k++) umma_bf16(tmem + 256 * w + 128 + 64 * place, dq + 2 * k, dk + 2 * k, id_s, x < T - 1 || (at | k) != 0);
-                    }
-                umma_commit(sf + 8 * (2 * w + place));
-            }
-            __syncwarp();
-        };
         while (ok && walk.next(it)) {
-            const int groups = it.vecs > 128 ? 2 : 1, steps = it.s1 - it.s0;
+            const int steps = it.s1 - it.s0;
             if (it.s0 > 0 && it.s1 == it.steps) join = {(int)((plan.begin - it.s0) / plan.chunk), it.vecs, it.row0 + it.vec0 / a.group, it.head * a.group, it.vec0 % a.group, {0, 0, 0}};
-            for (int w = 0; w < groups; w++) wait(qf + 8 * w, items[w]++);
+            if (w * 128 >= it.vecs) {   // nothing for the second group: its word for the stages alone
+                for (int s = 0; s < steps && ok; s++, n++)
+                    if (wait(full + 8 * (n % STAGES), n / STAGES) && lane == 0) mbar_arrive(empty + 8 * (n % STAGES));
+                continue;
+            }
+            wait(qf + 8 * w, items++);
             for (int s = -1; s < steps && ok; s++) {
                 if (s + 1 < steps) {   // the next tile's scores
-                    const int st = (n + 1 + s) % STAGES;
-                    if (!wait(full + 8 * st, (n + 1 + s) / STAGES)) break;
-                    tc_fence_after();
-                    for (int w = 0; w < groups; w++) scores(w, st, (nw[w] + 1 + s) & 1);
-                }
-                if (s < 0) continue;
-                const int st = (n + s) % STAGES;
-                for (int w = 0; w < groups; w++) {
-                    const int place = (nw[w] + s) & 1;
-                    if (!wait(pf + 8 * (2 * w + place), (nw[w] + s) >> 1)) break;
+                    const int st = (n + s + 1) % STAGES, place = (nw + 1 + s) & 1;
+                    if (!wait(full + 8 * st, (n + s + 1) / STAGES)) break;
                     tc_fence_after();
                     if (elect_one()) {
-                        const uint32_t va = smem_u32(stages + st * Sh::stage + ATOMS * Sh::k_atom), pa = tmem + 256 * w + 128 + 64 * place;
-                        const uint64_t dv = tc_desc_mn(va, Sh::k_atom);
+                        const uint32_t ka = smem_u32(stages + st * Sh::stage);
 #pragma unroll
-                        for (int x = T - 1; x >= 0; x--)
+                        for (int x = T - 1; x >= 0; x--)   // the small products first, so that their sums are rounded at their size
 #pragma unroll
-                            for (int k = 0; k < KT / 16; k++) umma_ts(tmem + 256 * w, pa + 32 * x + 8 * k, dv + (2048 >> 4) * k, id_o, s > 0 || x < T - 1 || k != 0);
-                        umma_commit(of + 8 * (2 * w + place));
-                        if (w == groups - 1) umma_commit(empty + 8 * st);
+                            for (int i = 0; i < ATOMS; i++) {
+                                const uint64_t dq = smem_desc(qa + (x * ATOMS + i) * Sh::q_atom), dk = smem_desc(ka + i * Sh::k_atom);
+#pragma unroll
+                                for (int k = 0; k < 4; k++) umma_bf16(o_t + 128 + 64 * place, dq + 2 * k, dk + 2 * k, id_s, x < T - 1 || (i | k) != 0);
+                            }
+                        umma_commit(sf + 8 * (2 * w + place));
                     }
                     __syncwarp();
                 }
+                if (s < 0) continue;
+                const int st = (n + s) % STAGES, place = (nw + s) & 1;
+                if (!wait(pf + 8 * (2 * w + place), (nw + s) >> 1)) break;
+                tc_fence_after();
+                if (elect_one()) {
+                    const uint32_t va = smem_u32(stages + st * Sh::stage) + ATOMS * Sh::k_atom, pa = o_t + 128 + 64 * place;
+                    const uint64_t dv = tc_desc_mn(va, Sh::k_atom);
+#pragma unroll
+                    for (int x = T - 1; x >= 0; x--)
+#pragma unroll
+                        for (int k = 0; k < KT / 16; k++) umma_ts(o_t, pa + 32 * x + 8 * k, dv + (2048 >> 4) * k, id_o, s > 0 || x < T - 1 || k != 0);
+                    umma_commit(of + 8 * (2 * w + place));
+                    umma_commit(empty + 8 * st);
+                }
+                __syncwarp();
             }
             n += steps;
-            for (int w = 0; w < groups; w++) nw[w] += steps;
+            nw += steps;
         }
-        if (lane == 0) joins[blockIdx.x] = join;
+        if (w == 0 && lane == 0) joins[blockIdx.x] = join;
         // MMAs that were issued may still read shared memory and write tensor memory
-        if (elect_one()) umma_commit(drain);
+        if (elect_one()) umma_commit(drain + 8 * w);
         __syncwarp();
-        ok = __all_sync(0xFFFFFFFFu, mbar_wait(drain, 0)) && ok;
+        ok = __all_sync(0xFFFFFFFFu, mbar_wait(drain + 8 * w, 0)) && ok;
         }
     }
     if (!ok && lane == 0) atomicExch(a.status, 1);
