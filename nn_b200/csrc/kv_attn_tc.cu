@@ -371,6 +371,13 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attn_tc_kernel(const KvAttn 
             const int low = a.window > 0 ? max(pos - a.window + 1, 0) : 0;
             const float fac = a.scale * kTcLog2E * Codes::unscale * kv_top_unscale(big);
             float m = 0.0f, mv = 0.0f, l = 0.0f, thr = -INFINITY, thv = -INFINITY;
+            // the weights of the group's tile number `t` are in tensor memory
+            auto hand_over = [&](int t) {
+                asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                tc_fence_before();
+                __syncwarp();
+                if (elect_one()) mbar_arrive(pf + 8 * (2 * w + (t & 1)));
+            };
             // A tile of keys, starting at key0; CLEAR: every vector of the warp sees all of it.
             auto tile = [&](auto clear, const int2 *sub, int key0, bool first) {
                 const uint32_t s_t = o_t + 128 + 64 * (nw & 1);
@@ -390,6 +397,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attn_tc_kernel(const KvAttn 
                 uint32_t x[2][32];
                 float lf[SUBS], fk[SUBS];   // of 16 keys: value exponent (then the weights' factor), the scores' factor
                 tc_ld64(s_t, x);
+                if (!first) hand_over(nw - 1);   // (the weights' way to tensor memory has passed during the load)
                 {
 #pragma unroll
                     for (int b = 0; b < SUBS; b++) {
@@ -470,10 +478,6 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attn_tc_kernel(const KvAttn 
                         tc_st(s_t + 16 * c, hw);
                         if (T == 2) tc_st(s_t + 32 + 16 * c, lw);
                     }
-                    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-                    tc_fence_before();
-                    __syncwarp();
-                    if (elect_one()) mbar_arrive(pf + 8 * (2 * w + (nw & 1)));
                 }
             };
             // (o_done has two places as well: a warp can be done with a tile before the product of the one before is, and a parity tells two
@@ -490,6 +494,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attn_tc_kernel(const KvAttn 
                 else tile(std::false_type(), sub, key0, s == it.s0);
             }
             if (!ok) break;
+            hand_over(nw - 1);
             ok = __all_sync(0xFFFFFFFFu, mbar_wait_fast(of + 8 * (2 * w + ((nw - 1) & 1)), ((nw - 1) >> 1) & 1));
             if (!ok) break;
             tc_fence_after();
