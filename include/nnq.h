@@ -793,7 +793,7 @@ NNQ_API nnq_status nnq_kv_attention(nnq_ctx *ctx, const nnq_kv_cache *cache, con
 
 /* Log probabilities from rows of logits [rows, vocab] (f32 or bf16, rows ld elements apart): logprob[r] of token[r] (0 for a
  * negative token; NaN and NNQ_ERR_INVALID_ARG from nnq_device_status beyond the vocabulary), the entropy of the row in nats, and its `top`
- * (0 .. 32) most probable tokens, [rows, top], in descending order, of equal ones the lowest first. Outputs that are not wanted may be
+ * (0 .. 32; vocabularies up to 600000 tokens) most probable tokens, [rows, top], in descending order, of equal ones the lowest first. Outputs that are not wanted may be
  * NULL (token_dev too, without logprob). Logits of -inf have probability 0; a row of nothing else has entropy 0 and log probabilities of
  * -inf; with a NaN or +inf the row's numbers are NaN, and a NaN ranks highest. f32 throughout. The reference's samplers
  * do this on the host (crates/nn-core/src/layers/generation/autoregressive_sampling.rs:14-21). */

@@ -2,14 +2,17 @@
 //
 //   lse = m + ln sum e^(x - m);  log p(t) = x_t - lse;  H = -sum p ln p = ln l - T / l,  l = sum e^(x - m), T = sum e^(x - m) (x - m)
 //
-// One pass over a row keeps the running maximum, l and T (every term of T has the same sign; a new maximum m' scales l by
-// f = e^(m - m') and makes T f (T + (m - m') l)); exponents are taken to base 2. All of it is f32.
+// One pass over a row keeps the running maximum m, l = sum 2^d and T = sum 2^d d with d = (x - m) log2 e, the difference formed first,
+// so that logits of any size keep their digits (every term of T has the same sign; a new maximum scales l by f = 2^-delta and makes
+// T f (T - delta l)). All of it is f32.
 // A row is dealt to a cluster of CTAs where the rows are few, and every CTA's sums meet in the first one's shared memory, in order.
-// The most probable tokens: the 32 warps' worth of threads (groups of threads with the same lane) have seen 32 disjoint parts of the
-// CTA's slice, so at least 32 elements are not below the least of the 32 parts' maxima. A second pass, which finds the slice in L2,
-// collects the elements from that bound on (some hundred of the real rows), whose ranks are counted; where they are more than there
-// is room for (rows of equal values), the largest element below the one before is looked for `top` times. Order: larger value first, then
-// the lower index.
+// The most probable tokens: the pass leaves the largest element of every group (four 16-byte vectors of a thread) in shared memory. The
+// threads of each of 32 lanes have seen disjoint parts of the slice, so at least 32 elements are not below the least of these parts'
+// maxima: the groups from there on (about a hundred) are ranked, and the `top` best are read again, element by element. Where that
+// meets more equal values than there is room for, or a NaN, the largest element below the one before is looked for `top` times. Order:
+// larger value first, then the lower index.
+// What bounds it: bf16 rows 12 elements per clock and SM at the copy rate, where the special function unit forms 16 exponentials;
+// single rows the way through the cluster.
 // The reference turns logits into probabilities on the host (crates/nn-core/src/layers/generation/autoregressive_sampling.rs:14-21 and
 // the samplers beside it).
 #include <algorithm>
@@ -19,7 +22,7 @@
 
 namespace nnq {
 
-constexpr int kLpThreads = 512, kLpWarps = kLpThreads / 32, kLpRoom = 1024, kLpTop = 32;
+constexpr int kLpThreads = 512, kLpWarps = kLpThreads / 32, kLpRoom = 1024, kLpTop = 32, kLpUnroll = 4;
 constexpr float kLpLog2E = 1.4426950408889634f, kLpLn2 = 0.6931471805599453f;
 
 struct LogprobArgs {
@@ -32,21 +35,26 @@ struct LogprobArgs {
     int *status;
 };
 
-struct Stats {   // maximum, sum of 2^d and of 2^d d, d = (x - m) log2 e
-    float m, l, t;
+struct Stats {   // maximum (-inf: no element), sum of 2^d and of 2^d d
+    float c, l, t;
 };
-__device__ __forceinline__ float finite_ref(float m) { return m == -INFINITY ? 0.0f : m; }
+__device__ __forceinline__ float finite_ref(float c) { return c == -INFINITY ? 0.0f : c; }
+__device__ __forceinline__ float lp_ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
 __device__ __forceinline__ Stats join(Stats a, Stats b) {
-    const float m = fmaxf(a.m, b.m), r = finite_ref(m);
-    const float da = (finite_ref(a.m) - r) * kLpLog2E, db = (finite_ref(b.m) - r) * kLpLog2E;
+    const float c = fmaxf(a.c, b.c), r = finite_ref(c);
+    const float da = (finite_ref(a.c) - r) * kLpLog2E, db = (finite_ref(b.c) - r) * kLpLog2E;
     // (a side without elements has sums of zero; its reference does not matter)
-    const float fa = a.l == 0.0f ? 0.0f : exp2f(da), fb = b.l == 0.0f ? 0.0f : exp2f(db);
-    return {m, fmaf(a.l, fa, b.l * fb), (a.l == 0.0f ? 0.0f : fa * fmaf(fmaxf(da, -1e4f), a.l, a.t)) + (b.l == 0.0f ? 0.0f : fb * fmaf(fmaxf(db, -1e4f), b.l, b.t))};
+    const float fa = a.l == 0.0f ? 0.0f : lp_ex2(da), fb = b.l == 0.0f ? 0.0f : lp_ex2(db);
+    return {c, fmaf(a.l, fa, b.l * fb), (a.l == 0.0f ? 0.0f : fa * fmaf(fmaxf(da, -1e4f), a.l, a.t)) + (b.l == 0.0f ? 0.0f : fb * fmaf(fmaxf(db, -1e4f), b.l, b.t))};
 }
 
 // order of logits as unsigned numbers; NaN above everything
 __device__ __forceinline__ uint32_t order_bits(float x) {
-    if (x != x) return 0xFFFFFFFFu;
+    if (x != x) return 0xFFFFFFFEu;   // (a key of all ones stands for none yet)
     const uint32_t b = __float_as_uint(x == 0.0f ? 0.0f : x);   // (-0 equals 0)
     return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
@@ -58,86 +66,176 @@ __device__ __forceinline__ float logit(const void *x, int64_t i) {
     else return __bfloat162float(reinterpret_cast<const __nv_bfloat16 *>(x)[i]);
 }
 
-// f(value, index in the row) for the elements [lo, hi) of a row: 16 bytes at a time from the first aligned one on
-template <bool F32, typename F>
-__device__ __forceinline__ void each_logit(const void *row, int lo, int hi, F f) {
-    constexpr int V = F32 ? 4 : 8;
-    const uint8_t *p = reinterpret_cast<const uint8_t *>(row);
-    const int size = F32 ? 4 : 2, tid = threadIdx.x;
-    const int head = min(hi, lo + (int)((16 - ((uintptr_t)(p + (int64_t)lo * size) & 15u)) % 16 / size));
-    for (int i = lo + tid; i < head; i += kLpThreads) f(logit<F32>(row, i), i);
-    const int vecs = (hi - head) / V;
-    const uint4 *q = reinterpret_cast<const uint4 *>(p + (int64_t)head * size);
-#pragma unroll 4
-    for (int u = tid; u < vecs; u += kLpThreads) {
-        const uint4 w = __ldg(q + u);
-        const uint32_t c[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-        for (int e = 0; e < V; e++) {
-            const float v = F32 ? __uint_as_float(c[e & 3]) : __uint_as_float(e & 1 ? c[e >> 1] & 0xFFFF0000u : c[e >> 1] << 16);
-            f(v, head + u * V + e);
-        }
+// A CTA's slice [lo, hi) of a row: elements up to the first 16-byte boundary, vectors, elements behind the last whole one.
+template <bool F32>
+struct Slice {
+    static constexpr int V = F32 ? 4 : 8, SIZE = F32 ? 4 : 2;
+    const void *row;
+    int lo, hi, head, vecs;
+    __device__ Slice(const void *row_, int lo_, int hi_) : row(row_), lo(lo_), hi(hi_) {
+        const uintptr_t at = reinterpret_cast<uintptr_t>(row) + (uintptr_t)lo * SIZE;
+        head = min(hi, lo + (int)((16 - (at & 15u)) % 16 / SIZE));
+        vecs = (hi - head) / V;
     }
-    for (int i = head + vecs * V + tid; i < hi; i += kLpThreads) f(logit<F32>(row, i), i);
+    __device__ const uint4 *vec() const { return reinterpret_cast<const uint4 *>(reinterpret_cast<const uint8_t *>(row) + (int64_t)head * SIZE); }
+    __device__ int edges() const { return hi - lo - vecs * V; }                                         // elements outside the vectors
+    __device__ int edge(int i) const { return i < head - lo ? lo + i : head + vecs * V + i - (head - lo); }
+    __device__ int groups() const { return (vecs + kLpThreads * kLpUnroll - 1) / (kLpThreads * kLpUnroll); }   // of a thread
+};
+
+// f(value, index in the row) for all elements
+template <bool F32, typename F>
+__device__ __forceinline__ void each_logit(const Slice<F32> &s, F f) {
+    constexpr int V = Slice<F32>::V;
+    for (int i = threadIdx.x; i < s.edges(); i += kLpThreads) f(logit<F32>(s.row, s.edge(i)), s.edge(i));
+    for (int u = threadIdx.x; u < s.vecs; u += kLpThreads)
+        for (int e = 0; e < V; e++) f(logit<F32>(s.row, s.head + u * V + e), s.head + u * V + e);
 }
 
 template <bool F32>
-__global__ void __launch_bounds__(kLpThreads) logprobs_kernel(const LogprobArgs a) {
+__global__ void __launch_bounds__(kLpThreads, 2) logprobs_kernel(const LogprobArgs a) {
+    extern __shared__ float group_max[];   // [groups of a thread][threads]
     __shared__ Stats warp_stats[kLpWarps], cta_stats;
     __shared__ float part_max[kLpWarps][32];
     __shared__ float bound_s;
-    __shared__ int found;
+    __shared__ uint32_t least_s;
+    __shared__ int found, chosen;
     __shared__ uint64_t room[kLpRoom];
+    __shared__ int pick[kLpRoom];
     __shared__ uint64_t best[kLpTop];
     __shared__ uint64_t red[kLpWarps];
+    constexpr int V = Slice<F32>::V;
     pdl_prologue();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, ctas = gridDim.x, me = blockIdx.x;
     const int64_t row = blockIdx.y;
-    const void *x = reinterpret_cast<const uint8_t *>(a.x) + row * a.ld * (F32 ? 4 : 2);
-    const int lo = min(a.vocab, me * a.slice), hi = min(a.vocab, lo + a.slice);
-    Stats s = {-INFINITY, 0.0f, 0.0f};
-    each_logit<F32>(x, lo, hi, [&](float v, int) {
-        if (v > s.m) {
-            const float d = (finite_ref(s.m) - v) * kLpLog2E, f = s.l == 0.0f ? 0.0f : exp2f(d);
-            s.t = s.l == 0.0f ? 0.0f : f * fmaf(fmaxf(d, -1e4f), s.l, s.t);
-            s.l *= f;
-            s.m = v;
+    const void *x = reinterpret_cast<const uint8_t *>(a.x) + row * a.ld * Slice<F32>::SIZE;
+    const int lo = min(a.vocab, me * a.slice);
+    const Slice<F32> sl(x, lo, min(a.vocab, lo + a.slice));
+    const int groups = sl.groups();
+    const uint4 *vec = sl.vec();
+
+    // ---- the pass
+    float m = -INFINITY, ref = 0.0f;   // maximum; the same, or 0 before there is one
+    float2 l = make_float2(0.0f, 0.0f), t = l;
+    const float2 scale = make_float2(kLpLog2E, kLpLog2E);
+    auto raise = [&](float top) {
+        if (m != -INFINITY) {
+            const float d = (m - top) * kLpLog2E, f = lp_ex2(d), dd = fmaxf(d, -1e4f);
+            t = make_float2(f * fmaf(dd, l.x, t.x), f * fmaf(dd, l.y, t.y));
+            l = make_float2(l.x * f, l.y * f);
         }
-        const float d = (v - finite_ref(s.m)) * kLpLog2E, e = exp2f(d);
-        s.l += e;
-        s.t = fmaf(e, fmaxf(d, -1e4f), s.t);
-    });
-    const float mine = s.m;
+        m = ref = top;
+    };
+    auto add = [&](float2 v) {
+        const float2 d = __fmul2_rn(__fadd2_rn(v, make_float2(-ref, -ref)), scale), e = make_float2(lp_ex2(d.x), lp_ex2(d.y));
+        l = __fadd2_rn(l, e);
+        t = __ffma2_rn(e, make_float2(fmaxf(d.x, -1e4f), fmaxf(d.y, -1e4f)), t);   // (0 times -inf would be NaN)
+    };
+    for (int g = 0; g < groups; g++) {
+        uint4 w[kLpUnroll];
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) s = join(s, {__shfl_xor_sync(0xFFFFFFFFu, s.m, o), __shfl_xor_sync(0xFFFFFFFFu, s.l, o), __shfl_xor_sync(0xFFFFFFFFu, s.t, o)});
+        for (int j = 0; j < kLpUnroll; j++) {
+            const int u = (g * kLpUnroll + j) * kLpThreads + tid;
+            const uint32_t none = F32 ? 0xFF800000u : 0xFF80FF80u;   // -inf
+            w[j] = u < sl.vecs ? __ldg(vec + u) : make_uint4(none, none, none, none);
+        }
+        auto value = [&](int j, int i) {   // pair i of vector j
+            const uint32_t q[4] = {w[j].x, w[j].y, w[j].z, w[j].w};
+            if constexpr (F32) return make_float2(__uint_as_float(q[2 * i]), __uint_as_float(q[2 * i + 1]));
+            else return make_float2(__uint_as_float(q[i] << 16), __uint_as_float(q[i] & 0xFFFF0000u));
+        };
+        float top = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < kLpUnroll; j++)
+#pragma unroll
+            for (int i = 0; i < V / 2; i++) top = fmaxf(top, fmaxf(value(j, i).x, value(j, i).y));
+        if (a.top > 0) group_max[g * kLpThreads + tid] = top;
+        if (top > m) raise(top);
+#pragma unroll
+        for (int j = 0; j < kLpUnroll; j++)
+#pragma unroll
+            for (int i = 0; i < V / 2; i++) add(value(j, i));
+    }
+    const float mine = m;   // of the vectors alone
+    for (int i = tid; i < sl.edges(); i += kLpThreads) {
+        const float v = logit<F32>(x, sl.edge(i));
+        if (v > m) raise(v);
+        add(make_float2(v, -INFINITY));
+    }
+    Stats s = {m, l.x + l.y, t.x + t.y};
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) s = join(s, {__shfl_xor_sync(0xFFFFFFFFu, s.c, o), __shfl_xor_sync(0xFFFFFFFFu, s.l, o), __shfl_xor_sync(0xFFFFFFFFu, s.t, o)});
     if (lane == 0) warp_stats[warp] = s;
-    if (tid == 0) found = 0;
+    if (tid == 0) {
+        found = chosen = 0;
+        least_s = 0xFFFFFFFFu;
+    }
+    if (tid < kLpTop) best[tid] = 0;   // below every key
     part_max[warp][lane] = mine;
     __syncthreads();
     if (warp == 0) {
         s = lane < kLpWarps ? warp_stats[lane] : Stats{-INFINITY, 0.0f, 0.0f};
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) s = join(s, {__shfl_xor_sync(0xFFFFFFFFu, s.m, o), __shfl_xor_sync(0xFFFFFFFFu, s.l, o), __shfl_xor_sync(0xFFFFFFFFu, s.t, o)});
+        for (int o = 16; o > 0; o >>= 1) s = join(s, {__shfl_xor_sync(0xFFFFFFFFu, s.c, o), __shfl_xor_sync(0xFFFFFFFFu, s.l, o), __shfl_xor_sync(0xFFFFFFFFu, s.t, o)});
         if (lane == 0) cta_stats = s;
+    } else if (warp == 1) {
         float b = -INFINITY;   // maximum of the elements that the threads of this lane have seen
+#pragma unroll
         for (int w = 0; w < kLpWarps; w++) b = fmaxf(b, part_max[w][lane]);
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) b = fminf(b, __shfl_xor_sync(0xFFFFFFFFu, b, o));
         if (lane == 0) bound_s = b;
     }
     __syncthreads();
+
+    // ---- the slice's most probable tokens
     if (a.top > 0) {
-        const float bound = bound_s;
-        each_logit<F32>(x, lo, hi, [&](float v, int i) {
-            if (!(v < bound)) {   // (a NaN as well)
-                const int at = atomicAdd(&found, 1);
-                if (at < kLpRoom) room[at] = order_key(v, i);
+        bool few = !(cta_stats.l != cta_stats.l);   // (a NaN hides from the groups' maxima)
+        if (few) {
+            const float bound = bound_s;
+            for (int g = 0; g < groups; g++)
+                if ((g * kLpUnroll * kLpThreads) + tid < sl.vecs && group_max[g * kLpThreads + tid] >= bound) {
+                    const int at = atomicAdd(&found, 1);
+                    if (at < kLpRoom) room[at] = order_key(group_max[g * kLpThreads + tid], g * kLpThreads + tid);
+                }
+            __syncthreads();
+            const int n = found;
+            few = n <= kLpRoom;
+            if (few) {
+                // the `top` best groups and their equals: the elements below the least of them are not among the best
+                for (int i = tid; i < n; i += kLpThreads) {
+                    const uint32_t k = (uint32_t)(room[i] >> 32);
+                    int above = 0;
+                    for (int j = 0; j < n; j++) above += (uint32_t)(room[j] >> 32) > k;
+                    if (above < a.top) {
+                        atomicMin(&least_s, k);
+                        pick[atomicAdd(&chosen, 1)] = (int)(0xFFFFFFFFu - (uint32_t)room[i]);
+                    }
+                }
+                __syncthreads();
+                const uint32_t least = n >= a.top ? least_s : 0u;   // (with fewer groups than that everything counts)
+                const int groups_read = chosen, per = kLpUnroll * V;
+                if (tid == 0) found = 0;
+                __syncthreads();
+                auto offer = [&](int idx) {
+                    const float v = logit<F32>(x, idx);
+                    if (order_bits(v) >= least) {
+                        const int at = atomicAdd(&found, 1);
+                        if (at < kLpRoom) room[at] = order_key(v, idx);
+                    }
+                };
+#pragma unroll 2
+                for (int i = tid; i < groups_read * per; i += kLpThreads) {
+                    const int q = pick[i / per], e = i % per, u = (q / kLpThreads * kLpUnroll + e / V) * kLpThreads + q % kLpThreads;
+                    if (u < sl.vecs) offer(sl.head + u * V + e % V);
+                }
+                for (int i = tid; i < sl.edges(); i += kLpThreads) offer(sl.edge(i));
+                __syncthreads();
+                few = found <= kLpRoom;
             }
-        });
-        if (tid < kLpTop) best[tid] = 0;   // below every key
-        __syncthreads();
-        const int n = found;
-        if (n <= kLpRoom) {
+        }
+        if (few) {
+            const int n = found;
             for (int i = tid; i < n; i += kLpThreads) {
                 const uint64_t k = room[i];
                 int rank = 0;
@@ -148,7 +246,7 @@ __global__ void __launch_bounds__(kLpThreads) logprobs_kernel(const LogprobArgs 
             uint64_t below = ~0ull;
             for (int i = 0; i < a.top; i++) {
                 uint64_t b = 0;
-                each_logit<F32>(x, lo, hi, [&](float v, int j) {
+                each_logit<F32>(sl, [&](float v, int j) {
                     const uint64_t k = order_key(v, j);
                     if (k < below && k > b) b = k;
                 });
@@ -165,25 +263,28 @@ __global__ void __launch_bounds__(kLpThreads) logprobs_kernel(const LogprobArgs 
         }
         __syncthreads();
     }
+
+    // ---- the row
     if (ctas > 1) cluster_sync();
     if (me == 0) {
         const uint32_t stats_at = smem_u32(&cta_stats), best_at = smem_u32(best);
-        s = cta_stats;
-        for (int c = 1; c < ctas; c++) {
-            Stats o;
-            const uint32_t p = cluster_addr(stats_at, c);
-            asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(o.m) : "r"(p) : "memory");
-            asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(o.l) : "r"(p + 4) : "memory");
-            asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(o.t) : "r"(p + 8) : "memory");
-            s = join(s, o);
+        s = lane < ctas ? cta_stats : Stats{-INFINITY, 0.0f, 0.0f};
+        if (lane > 0 && lane < ctas) {
+            const uint32_t p = cluster_addr(stats_at, lane);
+            asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(s.c) : "r"(p) : "memory");
+            asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(s.l) : "r"(p + 4) : "memory");
+            asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(s.t) : "r"(p + 8) : "memory");
         }
-        const float log_l = log2f(s.l), r = finite_ref(s.m);
-        const bool none = s.m == -INFINITY && s.l == 0.0f;   // no token has any probability
-        auto log_prob = [&](float v) { return none ? v : fmaf(v - r, 1.0f, -log_l * kLpLn2); };
+#pragma unroll
+        for (int o = 4; o > 0; o >>= 1) s = join(s, {__shfl_xor_sync(0xFFFFFFFFu, s.c, o), __shfl_xor_sync(0xFFFFFFFFu, s.l, o), __shfl_xor_sync(0xFFFFFFFFu, s.t, o)});
+        s = {__shfl_sync(0xFFFFFFFFu, s.c, 0), __shfl_sync(0xFFFFFFFFu, s.l, 0), __shfl_sync(0xFFFFFFFFu, s.t, 0)};
+        const float log_l = log2f(s.l), r = finite_ref(s.c);
+        const bool none = s.c == -INFINITY && s.l == 0.0f;   // no token has any probability
+        auto log_prob = [&](float v) { return none ? v : fmaf(-log_l, kLpLn2, v - r); };
         if (tid == 0) {
-            const int t = a.token ? a.token[row] : -1;
-            if (t >= a.vocab) atomicExch(a.status, kStatusIndex);
-            if (a.logprob) a.logprob[row] = t < 0 ? 0.0f : t >= a.vocab ? __int_as_float(0x7FFFFFFF) : log_prob(logit<F32>(x, t));
+            const int tok = a.token ? a.token[row] : -1;
+            if (tok >= a.vocab) atomicExch(a.status, kStatusIndex);
+            if (a.logprob) a.logprob[row] = tok < 0 ? 0.0f : tok >= a.vocab ? __int_as_float(0x7FFFFFFF) : log_prob(logit<F32>(x, tok));
             if (a.entropy) a.entropy[row] = none ? 0.0f : (log_l - s.t / s.l) * kLpLn2;
         }
         if (a.top > 0) {
@@ -231,7 +332,14 @@ nnq_status nnq_token_logprobs(nnq_ctx *ctx, const void *logits_dev, nnq_dtype dt
     // CTAs of a row: as many as give every SM one, but no slices below 4096 elements
     int ctas = 1;
     while (ctas < 8 && rows * ctas < ctx->sm_count && vocab / (2 * ctas) >= 4096) ctas *= 2;
-    const int slice = (int)(((vocab + ctas - 1) / ctas + 7) / 8 * 8);
+    const int slice = (int)(((vocab + ctas - 1) / ctas + 7) / 8 * 8), v = dt == NNQ_F32 ? 4 : 8;
+    // shared memory: a float per thread and group of its vectors (vocabularies of many millions take more than there is)
+    const int64_t groups = (slice / v + kLpThreads * kLpUnroll - 1) / (kLpThreads * kLpUnroll);
+    const size_t smem = top > 0 ? (size_t)groups * kLpThreads * 4 : 0;
+    if (smem > 160 * 1024) return fail(ctx, NNQ_ERR_UNSUPPORTED, "alternatives among %lld tokens", (long long)vocab);
+    if (smem > 16 * 1024 && (s = check_cuda(ctx, dt == NNQ_F32 ? cudaFuncSetAttribute(logprobs_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem)
+                                                               : cudaFuncSetAttribute(logprobs_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem), "shared memory")) != NNQ_OK)
+        return s;
     const int64_t most = 65535;   // rows of a launch
     for (int64_t r0 = 0; r0 < rows; r0 += most) {
         LogprobArgs a = {(const uint8_t *)logits_dev + r0 * ld * (dt == NNQ_F32 ? 4 : 2), token_dev ? token_dev + r0 : nullptr, logprob_dev ? logprob_dev + r0 : nullptr,
@@ -240,6 +348,7 @@ nnq_status nnq_token_logprobs(nnq_ctx *ctx, const void *logits_dev, nnq_dtype dt
         cudaLaunchConfig_t cfg = {};
         cfg.gridDim = dim3(ctas, (unsigned)std::min(most, rows - r0));
         cfg.blockDim = dim3(kLpThreads);
+        cfg.dynamicSmemBytes = smem;
         cfg.stream = (cudaStream_t)stream;
         cudaLaunchAttribute attr[2];
         attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
