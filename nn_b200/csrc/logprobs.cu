@@ -22,7 +22,7 @@
 
 namespace nnq {
 
-constexpr int kLpThreads = 512, kLpWarps = kLpThreads / 32, kLpRoom = 1024, kLpTop = 32, kLpUnroll = 4;
+constexpr int kLpRoom = 1024, kLpTop = 32, kLpUnroll = 4;
 constexpr float kLpLog2E = 1.4426950408889634f, kLpLn2 = 0.6931471805599453f;
 
 struct LogprobArgs {
@@ -67,7 +67,7 @@ __device__ __forceinline__ float logit(const void *x, int64_t i) {
 }
 
 // A CTA's slice [lo, hi) of a row: elements up to the first 16-byte boundary, vectors, elements behind the last whole one.
-template <bool F32>
+template <bool F32, int kLpThreads>
 struct Slice {
     static constexpr int V = F32 ? 4 : 8, SIZE = F32 ? 4 : 2;
     const void *row;
@@ -84,17 +84,18 @@ struct Slice {
 };
 
 // f(value, index in the row) for all elements
-template <bool F32, typename F>
-__device__ __forceinline__ void each_logit(const Slice<F32> &s, F f) {
-    constexpr int V = Slice<F32>::V;
+template <bool F32, int kLpThreads, typename F>
+__device__ __forceinline__ void each_logit(const Slice<F32, kLpThreads> &s, F f) {
+    constexpr int V = Slice<F32, kLpThreads>::V;
     for (int i = threadIdx.x; i < s.edges(); i += kLpThreads) f(logit<F32>(s.row, s.edge(i)), s.edge(i));
     for (int u = threadIdx.x; u < s.vecs; u += kLpThreads)
         for (int e = 0; e < V; e++) f(logit<F32>(s.row, s.head + u * V + e), s.head + u * V + e);
 }
 
-template <bool F32>
-__global__ void __launch_bounds__(kLpThreads, 2) logprobs_kernel(const LogprobArgs a) {
+template <bool F32, int kLpThreads>
+__global__ void __launch_bounds__(kLpThreads, kLpThreads == 256 ? 3 : 2) logprobs_kernel(const LogprobArgs a) {
     extern __shared__ float group_max[];   // [groups of a thread][threads]
+    constexpr int kLpWarps = kLpThreads / 32;
     __shared__ Stats warp_stats[kLpWarps], cta_stats;
     __shared__ float part_max[kLpWarps][32];
     __shared__ float bound_s;
@@ -104,13 +105,13 @@ __global__ void __launch_bounds__(kLpThreads, 2) logprobs_kernel(const LogprobAr
     __shared__ int pick[kLpRoom];
     __shared__ uint64_t best[kLpTop];
     __shared__ uint64_t red[kLpWarps];
-    constexpr int V = Slice<F32>::V;
+    constexpr int V = Slice<F32, kLpThreads>::V;
     pdl_prologue();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, ctas = gridDim.x, me = blockIdx.x;
     const int64_t row = blockIdx.y;
-    const void *x = reinterpret_cast<const uint8_t *>(a.x) + row * a.ld * Slice<F32>::SIZE;
+    const void *x = reinterpret_cast<const uint8_t *>(a.x) + row * a.ld * Slice<F32, kLpThreads>::SIZE;
     const int lo = min(a.vocab, me * a.slice);
-    const Slice<F32> sl(x, lo, min(a.vocab, lo + a.slice));
+    const Slice<F32, kLpThreads> sl(x, lo, min(a.vocab, lo + a.slice));
     const int groups = sl.groups();
     const uint4 *vec = sl.vec();
 
@@ -131,14 +132,20 @@ __global__ void __launch_bounds__(kLpThreads, 2) logprobs_kernel(const LogprobAr
         l = __fadd2_rn(l, e);
         t = __ffma2_rn(e, make_float2(fmaxf(d.x, -1e4f), fmaxf(d.y, -1e4f)), t);   // (0 times -inf would be NaN)
     };
-    for (int g = 0; g < groups; g++) {
-        uint4 w[kLpUnroll];
+    uint4 w[kLpUnroll], next[kLpUnroll];
+    auto fetch = [&](int g, uint4 (&to)[kLpUnroll]) {
 #pragma unroll
         for (int j = 0; j < kLpUnroll; j++) {
             const int u = (g * kLpUnroll + j) * kLpThreads + tid;
             const uint32_t none = F32 ? 0xFF800000u : 0xFF80FF80u;   // -inf
-            w[j] = u < sl.vecs ? __ldg(vec + u) : make_uint4(none, none, none, none);
+            to[j] = u < sl.vecs ? __ldg(vec + u) : make_uint4(none, none, none, none);
         }
+    };
+    fetch(0, next);
+    for (int g = 0; g < groups; g++) {
+#pragma unroll
+        for (int j = 0; j < kLpUnroll; j++) w[j] = next[j];
+        if (g + 1 < groups) fetch(g + 1, next);
         auto value = [&](int j, int i) {   // pair i of vector j
             const uint32_t q[4] = {w[j].x, w[j].y, w[j].z, w[j].w};
             if constexpr (F32) return make_float2(__uint_as_float(q[2 * i]), __uint_as_float(q[2 * i + 1]));
@@ -246,7 +253,7 @@ __global__ void __launch_bounds__(kLpThreads, 2) logprobs_kernel(const LogprobAr
             uint64_t below = ~0ull;
             for (int i = 0; i < a.top; i++) {
                 uint64_t b = 0;
-                each_logit<F32>(sl, [&](float v, int j) {
+                each_logit(sl, [&](float v, int j) {
                     const uint64_t k = order_key(v, j);
                     if (k < below && k > b) b = k;
                 });
@@ -332,14 +339,16 @@ nnq_status nnq_token_logprobs(nnq_ctx *ctx, const void *logits_dev, nnq_dtype dt
     // CTAs of a row: as many as give every SM one, but no slices below 4096 elements
     int ctas = 1;
     while (ctas < 8 && rows * ctas < ctx->sm_count && vocab / (2 * ctas) >= 4096) ctas *= 2;
+    // threads: four CTAs of 256 on an SM are in different phases of their rows where there are many; a row's few parts are read faster by
+    // 512 (us, 256 / 512: 2000 bf16 rows of 128259 128 / 145, 129 f32 rows of 151936 26.7 / 22.7)
+    const int threads = rows >= 2 * ctx->sm_count ? 256 : 512;
+    auto kernel = dt == NNQ_F32 ? (threads == 256 ? logprobs_kernel<true, 256> : logprobs_kernel<true, 512>) : (threads == 256 ? logprobs_kernel<false, 256> : logprobs_kernel<false, 512>);
     const int slice = (int)(((vocab + ctas - 1) / ctas + 7) / 8 * 8), v = dt == NNQ_F32 ? 4 : 8;
     // shared memory: a float per thread and group of its vectors (vocabularies of many millions take more than there is)
-    const int64_t groups = (slice / v + kLpThreads * kLpUnroll - 1) / (kLpThreads * kLpUnroll);
-    const size_t smem = top > 0 ? (size_t)groups * kLpThreads * 4 : 0;
+    const int64_t groups = (slice / v + threads * kLpUnroll - 1) / (threads * kLpUnroll);
+    const size_t smem = top > 0 ? (size_t)groups * threads * 4 : 0;
     if (smem > 160 * 1024) return fail(ctx, NNQ_ERR_UNSUPPORTED, "alternatives among %lld tokens", (long long)vocab);
-    if (smem > 16 * 1024 && (s = check_cuda(ctx, dt == NNQ_F32 ? cudaFuncSetAttribute(logprobs_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem)
-                                                               : cudaFuncSetAttribute(logprobs_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem), "shared memory")) != NNQ_OK)
-        return s;
+    if (smem > 16 * 1024 && (s = check_cuda(ctx, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem), "shared memory")) != NNQ_OK) return s;
     const int64_t most = 65535;   // rows of a launch
     for (int64_t r0 = 0; r0 < rows; r0 += most) {
         LogprobArgs a = {(const uint8_t *)logits_dev + r0 * ld * (dt == NNQ_F32 ? 4 : 2), token_dev ? token_dev + r0 : nullptr, logprob_dev ? logprob_dev + r0 : nullptr,
@@ -347,7 +356,7 @@ nnq_status nnq_token_logprobs(nnq_ctx *ctx, const void *logits_dev, nnq_dtype dt
                          ld, (int)vocab, top, slice, ctx->d_status};
         cudaLaunchConfig_t cfg = {};
         cfg.gridDim = dim3(ctas, (unsigned)std::min(most, rows - r0));
-        cfg.blockDim = dim3(kLpThreads);
+        cfg.blockDim = dim3(threads);
         cfg.dynamicSmemBytes = smem;
         cfg.stream = (cudaStream_t)stream;
         cudaLaunchAttribute attr[2];
@@ -357,7 +366,7 @@ nnq_status nnq_token_logprobs(nnq_ctx *ctx, const void *logits_dev, nnq_dtype dt
         attr[1].val.clusterDim = {(unsigned)ctas, 1, 1};
         cfg.attrs = attr;
         cfg.numAttrs = 2;
-        s = check_cuda(ctx, dt == NNQ_F32 ? cudaLaunchKernelEx(&cfg, logprobs_kernel<true>, a) : cudaLaunchKernelEx(&cfg, logprobs_kernel<false>, a), "log probabilities launch");
+        s = check_cuda(ctx, cudaLaunchKernelEx(&cfg, kernel, a), "log probabilities launch");
         if (s != NNQ_OK) return s;
         ctx->launches++;
     }
