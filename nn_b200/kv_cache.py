@@ -33,11 +33,11 @@ class _Batch(ctypes.Structure):
                 ("table_ld", ctypes.c_int64), ("rows", ctypes.c_int64), ("max_rows", ctypes.c_int64)]
 
 
-def _int32(t, name: str, shape, device):
+def _int32(t, name: str, shape, index: int):
     torch = api._torch()
-    if t.dtype != torch.int32 or t.device != device or not t.is_contiguous():
-        raise api.InvalidArgument(f"{name}: expected a contiguous int32 tensor on {device}, got {t.dtype} on {t.device}")
-    if tuple(t.shape) != tuple(shape):
+    if t.dtype != torch.int32 or not t.is_cuda or t.get_device() != index or not t.is_contiguous():
+        raise api.InvalidArgument(f"{name}: expected a contiguous int32 tensor on cuda:{index}, got {t.dtype} on {t.device}")
+    if t.shape != shape:
         raise api.ShapeMismatch(f"{name}: expected {tuple(shape)}, got {tuple(t.shape)}")
     return t
 
@@ -66,10 +66,10 @@ class KvBatch:
         if table.dim() != 2 or table.shape[0] < 1 or table.shape[1] < 1:
             raise api.ShapeMismatch(f"table: expected [requests, blocks], got {tuple(table.shape)}")
         n = table.shape[0]
-        self.table, self.length = _int32(table, "table", table.shape, self.device), _int32(length, "length", (n,), self.device)
-        self.row_start = _int32(row_start, "row_start", (n + 1,), self.device)
-        self.slot = None if slot is None else _int32(slot, "slot", (slot.numel(),), self.device)
-        self.position = None if position is None else _int32(position, "position", (position.numel(),), self.device)
+        self.table, self.length = _int32(table, "table", table.shape, b.device), _int32(length, "length", (n,), b.device)
+        self.row_start = _int32(row_start, "row_start", (n + 1,), b.device)
+        self.slot = None if slot is None else _int32(slot, "slot", (slot.numel(),), b.device)
+        self.position = None if position is None else _int32(position, "position", (position.numel(),), b.device)
         self.rows = 0 if slot is None else slot.numel()
         self.used = torch.zeros(1, dtype=torch.int32, device=self.device)
         return self
@@ -86,13 +86,15 @@ class KvBatch:
         if self.slot is None or self.position is None:
             raise api.InvalidArgument("a batch without slot and position tensors cannot be built")
         n, b = self.requests, self.backend
-        past, count = _int32(past, "past", (n,), self.device), _int32(count, "count", (n,), self.device)
-        free = _int32(free, "free", (free.numel(),), self.device)
+        past, count = _int32(past, "past", (n,), b.device), _int32(count, "count", (n,), b.device)
+        free = _int32(free, "free", (free.numel(),), b.device)
         if skip is not None:
-            _int32(skip, "skip", (1,), self.device)
-        b.check(b._lib.nnq_kv_tables(b._ctx, past.data_ptr(), count.data_ptr(), n, free.data_ptr(), free.numel(), None if skip is None else skip.data_ptr(), self.block,
-                                     self.table.data_ptr(), self.table.shape[1], self.length.data_ptr(), self.row_start.data_ptr(), self.slot.data_ptr(),
-                                     self.position.data_ptr(), self.rows, self.used.data_ptr(), api._stream_ptr(None, b.device)))
+            _int32(skip, "skip", (1,), b.device)
+        st = b._lib.nnq_kv_tables(b._ctx, past.data_ptr(), count.data_ptr(), n, free.data_ptr(), free.numel(), None if skip is None else skip.data_ptr(), self.block,
+                                  self.table.data_ptr(), self.table.shape[1], self.length.data_ptr(), self.row_start.data_ptr(), self.slot.data_ptr(),
+                                  self.position.data_ptr(), self.rows, self.used.data_ptr(), api._stream_ptr(None, b.device))
+        if st:
+            b.check(st)
         return self
 
 
@@ -116,7 +118,9 @@ class KvCache:
         z = lambda *s: torch.zeros(s, dtype=torch.uint8, device=self.device)  # noqa: E731
         self.k, self.v = z(blocks, kv_heads, block, dim), z(blocks, kv_heads, block, dim)
         self.k_exp, self.v_exp = z(blocks, kv_heads).fill_(127), z(blocks, kv_heads).fill_(127)
+        self._need = {}   # workspace by the number of query heads
         self._c = _Cache(self.fmt, self.kv_heads, self.dim, self.block, self.blocks, self.k.data_ptr(), self.v.data_ptr(), self.k_exp.data_ptr(), self.v_exp.data_ptr())
+        self._ref = ctypes.byref(self._c)
 
     def memory_bytes(self) -> int:
         return 2 * self.blocks * self.kv_heads * (self.block * self.dim + 1)
@@ -124,10 +128,13 @@ class KvCache:
     def _rows(self, x, name: str, heads: int):
         """A [rows, heads, dim] tensor as the kernels read it: rows may lie apart (a slice of a wider product), heads not."""
         torch = api._torch()
-        if x.dim() != 3 or x.shape[1] != heads or x.shape[2] != self.dim:
-            raise api.ShapeMismatch(f"{name}: expected [rows, {heads}, {self.dim}], got {tuple(x.shape)}")
-        if x.device != self.device:
+        shape = x.shape
+        if len(shape) != 3 or shape[1] != heads or shape[2] != self.dim:
+            raise api.ShapeMismatch(f"{name}: expected [rows, {heads}, {self.dim}], got {tuple(shape)}")
+        if not x.is_cuda or x.get_device() != self.backend.device:
             raise api.InvalidArgument(f"{name}: expected a tensor on {self.device}, got {x.device}")
+        if x.is_contiguous() and (x.dtype == torch.float32 or x.dtype == torch.bfloat16) and x.data_ptr() % 16 == 0:
+            return x
         if x.dtype not in (torch.float32, torch.bfloat16):
             x = x.float()
         size = x.element_size()
@@ -146,12 +153,14 @@ class KvCache:
         if k.dtype != v.dtype:
             k, v = k.float(), v.float()
         n = k.shape[0]
-        _int32(slots, "slots", (n,), self.device)
+        _int32(slots, "slots", (n,), b.device)
         if v.shape[0] != n:
             raise api.ShapeMismatch(f"{n} keys and {v.shape[0]} values")
         ld = self.kv_heads * self.dim
-        b.check(b._lib.nnq_kv_append(b._ctx, ctypes.byref(self._c), k.data_ptr(), k.stride(0) if n > 1 else ld, v.data_ptr(), v.stride(0) if n > 1 else ld,
-                                     api._dtype_code(k), slots.data_ptr(), n, api._stream_ptr(None, b.device)))
+        st = b._lib.nnq_kv_append(b._ctx, self._ref, k.data_ptr(), k.stride(0) if n > 1 else ld, v.data_ptr(), v.stride(0) if n > 1 else ld,
+                                  api._dtype_code(k), slots.data_ptr(), n, api._stream_ptr(None, b.device))
+        if st:
+            b.check(st)
 
     def read(self, slots, dtype=None):
         """(keys, values) of given slots, [rows, kv_heads, dim], f32 (default) or bf16: exact in both; zeros for slot -1."""
@@ -160,11 +169,13 @@ class KvCache:
         if dtype not in (torch.float32, torch.bfloat16):
             raise api.Unsupported(f"a cache is read as float32 or bfloat16, not {dtype}")
         b = self.backend
-        _int32(slots, "slots", (slots.numel(),), self.device)
-        k = torch.empty((slots.numel(), self.kv_heads, self.dim), dtype=dtype, device=self.device)
+        _int32(slots, "slots", (slots.numel(),), b.device)
+        n = slots.numel()
+        k = torch.empty((n, self.kv_heads, self.dim), dtype=dtype, device=self.device)
         v = torch.empty_like(k)
-        b.check(b._lib.nnq_kv_read(b._ctx, ctypes.byref(self._c), slots.data_ptr(), slots.numel(), k.data_ptr(), v.data_ptr(), api._dtype_code(k),
-                                   api._stream_ptr(None, b.device)))
+        st = b._lib.nnq_kv_read(b._ctx, self._ref, slots.data_ptr(), n, k.data_ptr(), v.data_ptr(), api._dtype_code(k), api._stream_ptr(None, b.device))
+        if st:
+            b.check(st)
         return k, v
 
     def attend(self, q, batch: KvBatch, scale: Optional[float] = None, window: int = 0, max_rows: int = 1, out=None):
@@ -177,16 +188,21 @@ class KvCache:
         q = self._rows(q, "q", heads)
         n, ld = q.shape[0], heads * self.dim
         if out is None:
-            out = torch.empty_like(q, memory_format=torch.contiguous_format)
+            out = torch.empty(q.shape, dtype=q.dtype, device=self.device)
         elif out.shape != q.shape or out.device != self.device or out.dtype not in (torch.float32, torch.bfloat16) or out.stride(2) != 1 or out.stride(1) != self.dim:
             raise api.ShapeMismatch(f"out: expected {tuple(q.shape)}, heads next to each other, on {self.device}")
-        if batch.block != self.block or batch.device != self.device:
+        if batch.block != self.block or batch.backend.device != b.device:
             raise api.InvalidArgument(f"a batch of blocks of {batch.block} on {batch.device} for a cache of blocks of {self.block} on {self.device}")
-        c = _Batch(batch.length.data_ptr(), batch.row_start.data_ptr(), batch.table.data_ptr(), batch.table.shape[0], batch.table.shape[1], n, max(int(max_rows), 1))
-        need = ctypes.c_size_t()
-        b.check(b._lib.nnq_kv_attention_workspace(b._ctx, ctypes.byref(self._c), ctypes.byref(c), heads, ctypes.byref(need)))
-        work = torch.empty(need.value, dtype=torch.uint8, device=self.device)
-        b.check(b._lib.nnq_kv_attention(b._ctx, ctypes.byref(self._c), ctypes.byref(c), q.data_ptr(), api._dtype_code(q), q.stride(0) if n > 1 else ld, heads,
-                                        1.0 / math.sqrt(self.dim) if scale is None else float(scale), int(window), out.data_ptr(), api._dtype_code(out),
-                                        out.stride(0) if n > 1 else ld, work.data_ptr(), need.value, api._stream_ptr(None, b.device)))
+        c = _Batch(batch.length.data_ptr(), batch.row_start.data_ptr(), batch.table.data_ptr(), batch.requests, batch.table.shape[1], n, max(int(max_rows), 1))
+        need = self._need.get(heads)
+        if need is None:   # (depends on the cache and the heads alone)
+            size = ctypes.c_size_t()
+            b.check(b._lib.nnq_kv_attention_workspace(b._ctx, self._ref, ctypes.byref(c), heads, ctypes.byref(size)))
+            need = self._need[heads] = size.value
+        work = torch.empty(need, dtype=torch.uint8, device=self.device)
+        st = b._lib.nnq_kv_attention(b._ctx, self._ref, ctypes.byref(c), q.data_ptr(), api._dtype_code(q), q.stride(0) if n > 1 else ld, heads,
+                                     1.0 / math.sqrt(self.dim) if scale is None else float(scale), int(window), out.data_ptr(), api._dtype_code(out),
+                                     out.stride(0) if n > 1 else ld, work.data_ptr(), need, api._stream_ptr(None, b.device))
+        if st:
+            b.check(st)
         return out

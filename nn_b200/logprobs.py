@@ -24,29 +24,29 @@ def token_logprobs(logits, tokens, top: int = 0, backend: Optional[api.Backend] 
     """logits [rows, vocab] f32 or bf16 (rows may lie apart), tokens [rows] (a negative one has log probability 0); top 0 .. 32."""
     torch = api._torch()
     b = backend or api.gpu_backend()
-    dev = torch.device("cuda", b.device)
     if logits.dim() != 2:
         raise api.RankMismatch(f"expected [rows, vocab], got rank {logits.dim()}")
-    if logits.device != dev or tokens.device != dev:
-        raise api.InvalidArgument(f"expected tensors on {dev}, got {logits.device} and {tokens.device}")
+    if not (logits.is_cuda and tokens.is_cuda and logits.get_device() == b.device and tokens.get_device() == b.device):
+        raise api.InvalidArgument(f"expected tensors on cuda:{b.device}, got {logits.device} and {tokens.device}")
     rows, vocab = logits.shape
-    if tuple(tokens.shape) != (rows,):
+    if tokens.shape != (rows,):
         raise api.ShapeMismatch(f"tokens: expected ({rows},), got {tuple(tokens.shape)}")
-    if logits.dtype not in (torch.float32, torch.bfloat16):
+    if logits.dtype != torch.float32 and logits.dtype != torch.bfloat16:
         logits = logits.float()
     if (vocab > 1 and logits.stride(1) != 1) or (rows > 1 and logits.stride(0) < vocab):
         logits = logits.contiguous()
     if tokens.dtype != torch.int32:
         tokens = tokens.clamp(-1, 2 ** 31 - 1).to(torch.int32)
     tokens = tokens.contiguous()
-    lp = torch.empty((2, rows), dtype=torch.float32, device=dev)
-    tt = tl = None
-    if top:
-        if top < 0 or top > min(32, vocab):
-            raise api.Unsupported(f"{top} alternatives: at most 32 and the vocabulary's size")
-        tt = torch.empty((rows, top), dtype=torch.int32, device=dev)
-        tl = torch.empty((rows, top), dtype=torch.float32, device=dev)
-    b.check(b._lib.nnq_token_logprobs(b._ctx, logits.data_ptr(), api._dtype_code(logits), rows, vocab, logits.stride(0) if rows > 1 else vocab, tokens.data_ptr(), int(top),
-                                      lp[0].data_ptr(), lp[1].data_ptr(), tt.data_ptr() if top else None, tl.data_ptr() if top else None,
-                                      api._stream_ptr(None, b.device)))
-    return TokenLogprobs(lp[0], lp[1], tt, tl)
+    if top < 0 or top > min(32, vocab):
+        raise api.Unsupported(f"{top} alternatives: at most 32 and the vocabulary's size")
+    # one allocation: log probabilities, entropies, then both tables of alternatives
+    mem = torch.empty((2 + 2 * top) * rows, dtype=torch.float32, device=logits.device)
+    at = mem.data_ptr()
+    st = b._lib.nnq_token_logprobs(b._ctx, logits.data_ptr(), api._dtype_code(logits), rows, vocab, logits.stride(0) if rows > 1 else vocab, tokens.data_ptr(), int(top),
+                                   at, at + 4 * rows, at + 8 * rows if top else None, at + 4 * (2 + top) * rows if top else None, api._stream_ptr(None, b.device))
+    if st:
+        b.check(st)
+    if not top:
+        return TokenLogprobs(mem[:rows], mem[rows:])
+    return TokenLogprobs(mem[:rows], mem[rows:2 * rows], mem[2 * rows:(2 + top) * rows].view(torch.int32).view(rows, top), mem[(2 + top) * rows:].view(rows, top))
