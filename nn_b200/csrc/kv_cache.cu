@@ -131,11 +131,13 @@ __global__ void __launch_bounds__(1024) kv_tables_kernel(const TableArgs a) {
 
 // ---- append ---------------------------------------------------------------------------------------------------------------------
 
-// Rows whose slots run on inside one block are a run; its first row is the leader. A CTA has kAppRows rows of one head, keys or values.
-// With one leader among them all warps work on its run (which may reach beyond the CTA's rows); with several a warp takes each.
-// A run: largest absolute value (bits compare like the numbers; non-finite ones are left out), exponent byte, codes; codes the block
-// held before are rounded again where the exponent grew.
-constexpr int kAppRows = 8, kAppWarps = 8;
+// Rows whose slots run on inside one block are a run; its first row is the leader. A warp has `tile` rows of one head, keys or values, and
+// takes the runs that are led there, wherever they end: the largest absolute value (bits compare like the numbers; non-finite ones are
+// left out), the exponent byte, the codes; codes the block held before are rounded again where the exponent grew. The first pieces of
+// eight values of a lane stay in registers in between.
+// What bounds it is latency: the chain slot -> values -> codes, which a warp goes through alone (a CTA per run, with a barrier in it:
+// 12000 rows of 8 heads of 128, bf16, 43 us).
+constexpr int kAppWarps = 8;
 
 struct AppendArgs {
     struct Part {
@@ -145,128 +147,171 @@ struct AppendArgs {
     } keys, values;
     const int32_t *slot;
     int64_t rows, slots;
-    int kv_heads, dim, shift;
+    int kv_heads, dim, shift, tile;
     int *status;
 };
 
+// eight values of a row as they lie in memory
 template <bool F32>
-__device__ __forceinline__ void load8(const void *p, int64_t at, float (&v)[8]) {
-    if constexpr (F32) {
-        const float4 a = __ldg(reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(p) + at));
-        const float4 b = __ldg(reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(p) + at) + 1);
-        v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-    } else {
-        const uint4 a = __ldg(reinterpret_cast<const uint4 *>(reinterpret_cast<const __nv_bfloat16 *>(p) + at));
-        const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+struct Eight {
+    uint4 w[F32 ? 2 : 1];
+    __device__ __forceinline__ void load(const void *p, int64_t at) {
+        const uint4 *q = reinterpret_cast<const uint4 *>(reinterpret_cast<const uint8_t *>(p) + at * (F32 ? 4 : 2));
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            v[2 * i] = __uint_as_float(w[i] << 16);
-            v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+        for (int i = 0; i < (F32 ? 2 : 1); i++) w[i] = __ldg(q + i);
+    }
+    __device__ __forceinline__ void values(float (&v)[8]) const {
+        const uint32_t *u = &w[0].x;
+        if constexpr (F32) {
+#pragma unroll
+            for (int i = 0; i < 8; i++) v[i] = __uint_as_float((i < 4 ? (&w[0].x)[i] : (&w[1].x)[i - 4]));
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                v[2 * i] = __uint_as_float(u[i] << 16);
+                v[2 * i + 1] = __uint_as_float(u[i] & 0xFFFF0000u);
+            }
         }
     }
+};
+
+// Codes of eight values already divided by the scale: finite ones within the range.
+template <int FMT>
+__device__ __forceinline__ uint2 encode_within(const float (&v)[8]) {
+    uint32_t w[2];
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+        if constexpr (FMT == NNQ_KV_INT8) {   // the integer is the low byte of the sum's bits, rounded to the nearest, ties to even
+            uint32_t b[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) b[i] = __float_as_uint(v[4 * h + i] + 12582912.0f);
+            w[h] = __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
+        } else {
+            uint16_t p, q;
+            asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(p) : "f"(v[4 * h + 1]), "f"(v[4 * h]));
+            asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(q) : "f"(v[4 * h + 3]), "f"(v[4 * h + 2]));
+            w[h] = (uint32_t)p | (uint32_t)q << 16;
+        }
+    }
+    return make_uint2(w[0], w[1]);
 }
 
-// A run of `n` rows from row `t` on, by `threads` threads of which this is number `me`; sync and reduce are theirs.
-template <int FMT, bool F32, typename Reduce, typename Sync>
-__device__ __forceinline__ void append_run(const AppendArgs &a, const AppendArgs::Part &p, int head, int64_t t, int n, int me, int threads, Reduce reduce, Sync sync) {
-    const int units = a.dim >> 3, first = a.slot[t];
+// A run of `n` rows from row `t` on, by a warp.
+template <int FMT, bool F32>
+__device__ __forceinline__ void append_run(const AppendArgs &a, const AppendArgs::Part &p, int head, int64_t t, int first, int n) {
+    constexpr int KEEP = F32 ? 2 : 4;
+    const int lane = threadIdx.x & 31, per = a.dim >> 3, units = n * per, magic = (65535 + per) / per;   // (exact below 8192)
     const int64_t blk = first >> a.shift;
     const int off = first & ((1 << a.shift) - 1);
-    const int64_t base = t * p.ld + (int64_t)head * a.dim;
+    const void *x = reinterpret_cast<const uint8_t *>(p.x) + (t * p.ld + (int64_t)head * a.dim) * (F32 ? 4 : 2);
     uint8_t *codes = p.codes + (((blk * a.kv_heads + head) << a.shift) * a.dim), *exp_at = p.exps + blk * a.kv_heads + head;
-    const int old = off ? min(max((int)*exp_at, 0), kExpMax) : 0;
+    const int old = off ? min((int)*exp_at, kExpMax) : 0;
+    auto at_of = [&](int u) {
+        const int row = u * magic >> 16;   // u / per
+        return row * p.ld + (u - row * per) * 8;
+    };
     uint32_t top = 0;
     bool bad = false;
-    for (int u = me; u < n * units; u += threads) {
-        const int row = u / units, d = (u - row * units) * 8;
+    Eight<F32> keep[KEEP];
+    auto look = [&](const Eight<F32> &e) {
         float v[8];
-        load8<F32>(p.x, base + row * p.ld + d, v);
+        e.values(v);
+        uint32_t most = 0;
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-            const uint32_t b = __float_as_uint(v[i]) & 0x7FFFFFFFu;
-            if (b >= 0x7F800000u) bad = true;
-            else top = max(top, b);
+        for (int i = 0; i < 8; i++) most = max(most, __float_as_uint(v[i]) & 0x7FFFFFFFu);
+        if (most >= 0x7F800000u) {
+            bad = true;
+            most = 0;
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const uint32_t b = __float_as_uint(v[i]) & 0x7FFFFFFFu;
+                if (b < 0x7F800000u) most = max(most, b);
+            }
         }
+        top = max(top, most);
+    };
+#pragma unroll
+    for (int i = 0; i < KEEP; i++)
+        if (lane + 32 * i < units) keep[i].load(x, at_of(lane + 32 * i));
+#pragma unroll
+    for (int i = 0; i < KEEP; i++)
+        if (lane + 32 * i < units) look(keep[i]);
+#pragma unroll 4
+    for (int u = lane + 32 * KEEP; u < units; u += 32) {
+        Eight<F32> e;
+        e.load(x, at_of(u));
+        look(e);
     }
     if (bad) atomicExch(a.status, kStatusValue);
-    top = reduce(top);
-    const int e = max(exponent_byte<FMT>(top), old);
+    const int e = max(exponent_byte<FMT>(__reduce_max_sync(0xFFFFFFFFu, top)), old);
     const float inv = pow2_byte(254 - e);
-    for (int u = me; u < n * units; u += threads) {
-        const int row = u / units, d = (u - row * units) * 8;
+    uint8_t *to = codes + (int64_t)off * a.dim;   // (the rows of a run lie one behind the other in the block)
+    auto write = [&](const Eight<F32> &q, int u) {
         float v[8];
-        load8<F32>(p.x, base + row * p.ld + d, v);
-        uint32_t w[2] = {0, 0};
+        q.values(v);
+        constexpr float most = FMT == NNQ_KV_INT8 ? 127.0f : 448.0f;
 #pragma unroll
-        for (int i = 0; i < 8; i++) w[i >> 2] |= kv_encode<FMT>(v[i] * inv) << (8 * (i & 3));
-        *reinterpret_cast<uint2 *>(codes + (int64_t)(off + row) * a.dim + d) = make_uint2(w[0], w[1]);
+        for (int i = 0; i < 8; i++) {
+            v[i] *= inv;
+            if (bad) v[i] = v[i] == v[i] ? fminf(fmaxf(v[i], -most), most) : 0.0f;   // (some value of this lane's is not finite)
+        }
+        *reinterpret_cast<uint2 *>(to + (int64_t)u * 8) = encode_within<FMT>(v);
+    };
+#pragma unroll
+    for (int i = 0; i < KEEP; i++)
+        if (lane + 32 * i < units) write(keep[i], lane + 32 * i);
+#pragma unroll 4
+    for (int u = lane + 32 * KEEP; u < units; u += 32) {
+        Eight<F32> q;
+        q.load(x, at_of(u));
+        write(q, u);
     }
     if (off && e > old) {
         const float again = pow2_byte(max(127 + old - e, 0));
-        for (int u = me; u < off * units; u += threads) {
+        for (int u = lane; u < off * per; u += 32) {
             uint2 *at = reinterpret_cast<uint2 *>(codes) + u;
             const uint2 c = *at;
-            uint32_t in[2] = {c.x, c.y}, w[2] = {0, 0};
+            const uint32_t in[2] = {c.x, c.y};
+            float v[8];
 #pragma unroll
-            for (int i = 0; i < 8; i++) w[i >> 2] |= kv_encode<FMT>(kv_decode<FMT>(in[i >> 2] >> (8 * (i & 3)) & 0xFFu) * again) << (8 * (i & 3));
-            *at = make_uint2(w[0], w[1]);
+            for (int i = 0; i < 8; i++) v[i] = kv_decode<FMT>(in[i >> 2] >> (8 * (i & 3)) & 0xFFu) * again;   // (again is a half or less)
+            *at = encode_within<FMT>(v);
         }
     }
-    sync();   // everybody has read the old byte
-    if (me == 0) *exp_at = (uint8_t)e;
+    __syncwarp();   // every lane has read the old byte
+    if (lane == 0) *exp_at = (uint8_t)e;
 }
 
 template <int FMT, bool F32>
-__global__ void __launch_bounds__(kAppWarps * 32) kv_append_kernel(const AppendArgs a) {
-    __shared__ uint32_t red[kAppWarps];
+__global__ void __launch_bounds__(kAppWarps * 32, 4) kv_append_kernel(const AppendArgs a) {
     pdl_prologue();
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, head = blockIdx.y;
-    const AppendArgs::Part part = blockIdx.z ? a.values : a.keys;
-    const int64_t t0 = (int64_t)blockIdx.x * kAppRows;
-    const int block = 1 << a.shift;
-    // leaders among the CTA's rows (every warp finds them for itself)
+    const int lane = threadIdx.x & 31, heads = 2 * a.kv_heads, block = 1 << a.shift;
+    const int64_t id = (int64_t)blockIdx.x * kAppWarps + (threadIdx.x >> 5), tile = id / heads, t0 = tile * a.tile;
+    const int which = (int)(id - tile * heads), head = which >> 1;
+    if (t0 >= a.rows) return;
+    const AppendArgs::Part part = which & 1 ? a.values : a.keys;
     const int64_t t = t0 + lane;
     int s = -1, before = -1;
-    if (lane < kAppRows && t < a.rows) {
+    if (lane < a.tile && t < a.rows) {
         s = a.slot[t];
         if (t > 0) before = a.slot[t - 1];
     }
     if (s >= a.slots) {
-        if (tid < kAppRows) atomicExch(a.status, kStatusIndex);
+        atomicExch(a.status, kStatusIndex);
         s = -1;
     }
     const bool leads = s >= 0 && (before < 0 || before != s - 1 || (s & (block - 1)) == 0);
-    uint32_t leaders = __ballot_sync(0xFFFFFFFFu, leads);
-    auto run_length = [&](int64_t from) {
-        const int first = a.slot[from], most = block - (first & (block - 1));
-        for (int i0 = 0; i0 < most; i0 += 32) {
-            const int i = i0 + lane;
-            const bool on = i < most && from + i < a.rows && a.slot[from + i] == first + i;
-            const uint32_t m = __ballot_sync(0xFFFFFFFFu, on);
-            if (m != 0xFFFFFFFFu) return i0 + __ffs(~m) - 1;
+    for (uint32_t leaders = __ballot_sync(0xFFFFFFFFu, leads); leaders; leaders &= leaders - 1) {
+        const int src = __ffs(leaders) - 1, first = __shfl_sync(0xFFFFFFFFu, s, src), most = block - (first & (block - 1));
+        const int64_t from = t0 + src;
+        int n = 0;
+        for (;;) {   // rows that continue the run
+            const int i = n + lane;
+            const uint32_t m = __ballot_sync(0xFFFFFFFFu, i < most && from + i < a.rows && a.slot[from + i] == first + i);
+            n += m == 0xFFFFFFFFu ? 32 : __ffs(~m) - 1;
+            if (m != 0xFFFFFFFFu || n >= most) break;
         }
-        return most;
-    };
-    if (__popc(leaders) == 1) {
-        const int64_t from = t0 + __ffs(leaders) - 1;
-        append_run<FMT, F32>(a, part, head, from, run_length(from), tid, kAppWarps * 32,
-                             [&](uint32_t v) {
-                                 v = __reduce_max_sync(0xFFFFFFFFu, v);
-                                 if (lane == 0) red[warp] = v;
-                                 __syncthreads();
-                                 uint32_t m = 0;
-#pragma unroll
-                                 for (int w = 0; w < kAppWarps; w++) m = max(m, red[w]);
-                                 return m;
-                             },
-                             [] { __syncthreads(); });
-    } else {
-        for (int i = 0; leaders; i++) {
-            const int64_t from = t0 + __ffs(leaders) - 1;
-            leaders &= leaders - 1;
-            if (i % kAppWarps == warp)
-                append_run<FMT, F32>(a, part, head, from, run_length(from), lane, 32, [](uint32_t v) { return __reduce_max_sync(0xFFFFFFFFu, v); }, [] { __syncwarp(); });
-        }
+        append_run<FMT, F32>(a, part, head, from, first, n);
     }
 }
 
@@ -369,8 +414,10 @@ nnq_status nnq_kv_append(nnq_ctx *ctx, const nnq_kv_cache *c, const void *k_dev,
     if (!rows_aligned(k_dev, k_ld, dt) || !rows_aligned(v_dev, v_ld, dt)) return fail(ctx, NNQ_ERR_INVALID_ARG, "rows of keys and values must start at multiples of 16 bytes");
     if ((s = check_cuda(ctx, cudaSetDevice(ctx->device), "cudaSetDevice")) != NNQ_OK) return s;
     const AppendArgs a = {{k_dev, k_ld, (uint8_t *)c->k, c->k_exp}, {v_dev, v_ld, (uint8_t *)c->v, c->v_exp}, slot_dev, rows, c->blocks * c->block, c->kv_heads, c->dim,
-                          log2_of(c->block), ctx->d_status};
-    const dim3 grid((unsigned)((rows + kAppRows - 1) / kAppRows), c->kv_heads, 2), block(kAppWarps * 32);
+                          log2_of(c->block), rows > 1024 ? 8 : 1, ctx->d_status};   // (few rows are single tokens more often than not: a warp each)
+    const int64_t warps = (rows + a.tile - 1) / a.tile * 2 * c->kv_heads;
+    if (warps / kAppWarps >= INT32_MAX) return fail(ctx, NNQ_ERR_UNSUPPORTED, "%lld rows of %d heads", (long long)rows, c->kv_heads);
+    const dim3 grid((unsigned)((warps + kAppWarps - 1) / kAppWarps)), block(kAppWarps * 32);
     auto kernel = c->format == NNQ_KV_INT8 ? (dt == NNQ_F32 ? kv_append_kernel<NNQ_KV_INT8, true> : kv_append_kernel<NNQ_KV_INT8, false>)
                                            : (dt == NNQ_F32 ? kv_append_kernel<NNQ_KV_E4M3, true> : kv_append_kernel<NNQ_KV_E4M3, false>);
     launch_pdl(kernel, grid, block, (cudaStream_t)stream, a);

@@ -34,20 +34,6 @@ __device__ __forceinline__ int exponent_byte(uint32_t bits) {
     return min(max((int)(bits >> 23) - shift + ((bits & 0x7FFFFFu) > top ? 1 : 0), kExpMin), kExpMax);
 }
 
-// The code of a value divided by its scale: nearest, ties to even; values outside the range become the largest code, NaN becomes 0.
-template <int FMT>
-__device__ __forceinline__ uint32_t kv_encode(float x) {
-    if constexpr (FMT == NNQ_KV_INT8) {
-        const float r = x == x ? fminf(fmaxf(x, -127.0f), 127.0f) : 0.0f;
-        return (uint32_t)__float2int_rn(r) & 0xFFu;
-    } else {
-        const float r = x == x ? fminf(fmaxf(x, -448.0f), 448.0f) : 0.0f;
-        uint16_t p;
-        asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(p) : "f"(0.0f), "f"(r));
-        return p & 0xFFu;
-    }
-}
-
 // The value of a code. e4m3: its bits are those of an f16 number 2^8 smaller, subnormal numbers included.
 template <int FMT>
 __device__ __forceinline__ float kv_decode(uint32_t code) {
