@@ -800,6 +800,18 @@ NNQ_API nnq_status nnq_kv_attention(nnq_ctx *ctx, const nnq_kv_cache *cache, con
 NNQ_API nnq_status nnq_token_logprobs(nnq_ctx *ctx, const void *logits_dev, nnq_dtype dt, int64_t rows, int64_t vocab, int64_t ld, const int32_t *token_dev, int top,
                                       float *logprob_dev, float *entropy_dev, int32_t *top_token_dev, float *top_logprob_dev, void *stream);
 
+/* A Qwen3 decoder (nnq_decoder_create) with its keys and values in 8 bits, in blocks of `block` tokens (see nnq_kv_cache): a quarter of the
+ * memory of the f32 cache, which is given back. Before the first token. A step appends and attends through the calls above, so it is not
+ * fused with its products. With this cache nnq_decoder_buffers gives NULL for the f32 ones; nnq_decoder_cache gives a layer's,
+ * whose position p is slot p. */
+NNQ_API nnq_status nnq_decoder_set_cache(nnq_decoder *d, int format, int block);
+NNQ_API nnq_status nnq_decoder_cache(nnq_decoder *d, int layer, nnq_kv_cache *out);
+/* nnq_decoder_extend with log probabilities in place of the logits: after the `n_want` tokens want[] (at least one), the log probability of
+ * given_host[i] (a negative one: 0), the entropy and the `top` most probable tokens as in nnq_token_logprobs, to host arrays [n_want]
+ * and [n_want, top]. For both kinds of decoder. */
+NNQ_API nnq_status nnq_decoder_score(nnq_decoder *d, const int32_t *tokens_host, int count, int start_pos, const int32_t *want, int n_want, const int32_t *given_host, int top,
+                                     float *logprob_host, float *entropy_host, int32_t *top_token_host, float *top_logprob_host, void *stream);
+
 /* Number of kernels this library has launched on this context since creation. */
 NNQ_API int64_t nnq_launch_count(const nnq_ctx *ctx);
 

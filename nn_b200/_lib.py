@@ -90,6 +90,9 @@ SIGNATURES = {
     "nnq_decoder_set_head_weights": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p]),
     "nnq_decoder_set_head_options": (c_int, [c_void_p, c_void_p]),
     "nnq_decoder_extend": (c_int, [c_void_p, c_void_p, c_int, c_int, c_void_p, c_int, c_void_p, c_void_p]),
+    "nnq_decoder_set_cache": (c_int, [c_void_p, c_int, c_int]),
+    "nnq_decoder_cache": (c_int, [c_void_p, c_int, c_void_p]),
+    "nnq_decoder_score": (c_int, [c_void_p, c_void_p, c_int, c_int, c_void_p, c_int, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
     "nnq_plan_create": (c_int, [c_void_p, c_int, c_int, c_int, ctypes.POINTER(c_void_p)]),
     "nnq_plan_add": (c_int, [c_void_p, c_int, ctypes.POINTER(c_void_p), c_void_p, ctypes.POINTER(c_void_p),
                              ctypes.POINTER(c_void_p)]),

@@ -45,6 +45,23 @@ struct nnq_decoder {
     const nnq_weight *lm_head;
     float *d_cos, *d_sin;       // [max_seq, head_dim / 2]
     float *d_kcache, *d_vcache; // [layers, kv_heads, max_seq, head_dim]
+    // keys and values in 8 bits instead (nnq_decoder_set_cache): blocks of all layers one behind the other, block number = position / block
+    struct Cache8 {
+        nnq_kv_cache layer0;    // blocks: of one layer
+        uint8_t *mem;           // codes and exponent bytes of all layers
+        int *ints;              // table, the numbers 0, 1, .. (list of free blocks), and the words below
+        int *table, *numbers, *length, *row_start, *used, *call, *step_slot, *step_pos;   // call: positions held, rows
+        float *krot;            // rotated keys of a step
+        void *work;
+        size_t work_bytes;
+    } *kv8;
+    float *pf_krot;             // rotated keys of a prompt's rows, their slots and positions
+    int *pf_slot, *pf_pos;
+    struct Scores {             // nnq_decoder_score: of kWantRows rows
+        int *token, *top_token;
+        float *logprob, *entropy, *top_logprob;
+    } scores;
+    void *score_mem;
     float *d_h, *d_delta, *d_q, *d_k, *d_v, *d_qrot, *d_g, *d_u, *d_logits, *d_part;
     unsigned int *d_arrived;   // per kv head: attention CTAs that have published their record
     void *d_xn, *d_attn, *d_mid;   // activations fed to the products (f32 or bf16)
@@ -162,12 +179,13 @@ dec_norm_kernel(float *__restrict__ h, const float *__restrict__ delta, const __
 }
 
 // One CTA per head (query heads, then key heads, then value heads), one thread per dimension:
-// RMSNorm over the head (q, k), half-split rotation at the current position, append k / v.
+// RMSNorm over the head (q, k), half-split rotation at the current position, append k / v (head_ld, pos_ld: of the cache; a
+// row of keys for the 8-bit cache has pos_ld 0).
 __global__ void __launch_bounds__(256)
 dec_qk_rope_kernel(const float *__restrict__ q, const float *__restrict__ k, const float *__restrict__ v,
                    const float *__restrict__ qw, const float *__restrict__ kw, const float *__restrict__ cosv,
                    const float *__restrict__ sinv, const int *__restrict__ state, float eps, float *__restrict__ qrot,
-                   float *__restrict__ kcache, float *__restrict__ vcache, int n_heads, int n_kv, int hd, int max_seq) {
+                   float *__restrict__ kcache, float *__restrict__ vcache, int n_heads, int n_kv, int hd, size_t head_ld, size_t pos_ld) {
     pdl_prologue();
     __shared__ float red[32];
     __shared__ float xs[256];
@@ -175,7 +193,7 @@ dec_qk_rope_kernel(const float *__restrict__ q, const float *__restrict__ k, con
     const int half = hd / 2;
     if (head >= n_heads + n_kv) {   // value head: plain append
         const int kvh = head - n_heads - n_kv;
-        if (d < hd) vcache[((size_t)kvh * max_seq + pos) * hd + d] = v[kvh * hd + d];
+        if (d < hd) vcache[kvh * head_ld + pos * pos_ld + d] = v[kvh * hd + d];
         return;
     }
     const bool is_q = head < n_heads;
@@ -192,7 +210,7 @@ dec_qk_rope_kernel(const float *__restrict__ q, const float *__restrict__ k, con
     // y1 = x1 cos - x2 sin; y2 = x1 sin + x2 cos
     const float y = d < half ? xs[d] * c - xs[d + half] * s : xs[d - half] * s + xs[d] * c;
     if (is_q) qrot[head * hd + d] = y;
-    else kcache[((size_t)(head - n_heads) * max_seq + pos) * hd + d] = y;
+    else kcache[(head - n_heads) * head_ld + pos * pos_ld + d] = y;
 }
 
 // What the attention kernel of a fused step does before it attends: see ROPE below.
@@ -581,7 +599,7 @@ __global__ void dec_argmax_exchange_kernel(const float *__restrict__ bv_in, cons
 void launch_norm_rows4(float *h, const float *delta, const __nv_bfloat16 *embed, const int *tokens, const float *w, float eps, void *xn, int act_dt, int hidden, int rows,
                        cudaStream_t st);
 void launch_qk_rope_rows128(const float *q, const float *k, const float *v, const float *qw, const float *kw, const float *cosv, const float *sinv, int pos0, float eps,
-                            float *qrot, float *kcache, float *vcache, int n_heads, int n_kv, int rows, int max_seq, cudaStream_t st);
+                            float *qrot, float *kcache, float *vcache, int n_heads, int n_kv, int rows, size_t head_ld, size_t pos_ld, cudaStream_t st);
 void launch_silu_mul_rows(nnq_ctx *ctx, const float *g, const float *u, void *mid, int act_dt, int64_t total, cudaStream_t st);
 
 // row r: h = embedding of tokens[r] (first layer) or h += delta; xn = RMSNorm(h) * w. One CTA per row.
@@ -1313,6 +1331,75 @@ nnq_status nnq_decoder_set_comm(nnq_decoder *d, nnq_comm *comm) {
     return NNQ_OK;
 }
 
+static nnq_status cache8_seek(nnq_decoder *d, int pos, int count, cudaStream_t st);
+
+nnq_status nnq_decoder_set_cache(nnq_decoder *d, int format, int block) {
+    if (!d) return NNQ_ERR_INVALID_ARG;
+    nnq_ctx *ctx = d->ctx;
+    const nnq_decoder_config &c = d->cfg;
+    if (!d->layers) return fail(ctx, NNQ_ERR_UNSUPPORTED, "the blocks of a block decoder keep caches of their own");
+    if (d->kv8) return fail(ctx, NNQ_ERR_UNSUPPORTED, "the decoder has an 8-bit cache already");
+    if (d->host_pos >= 0 || d->pf_mem) return fail(ctx, NNQ_ERR_UNSUPPORTED, "the cache of a decoder is chosen before its first token");
+    if (format != NNQ_KV_INT8 && format != NNQ_KV_E4M3) return fail(ctx, NNQ_ERR_INVALID_ARG, "unknown cache format %d", format);
+    if (block < 16 || block > 256 || (block & (block - 1))) return fail(ctx, NNQ_ERR_UNSUPPORTED, "blocks of a cache must hold 16, 32, 64, 128 or 256 tokens (got %d)", block);
+    nnq_status s = check_cuda(ctx, cudaSetDevice(ctx->device), "cudaSetDevice");
+    if (s != NNQ_OK) return s;
+    nnq_decoder::Cache8 k = {};
+    const int64_t blocks = (c.max_seq + block - 1) / block, codes = (int64_t)c.n_layers * blocks * d->lkv * block * 128, exps = (int64_t)c.n_layers * blocks * d->lkv;
+    s = dev_alloc(ctx, (void **)&k.mem, 2 * codes + 2 * exps, "8-bit cache");
+    if (s == NNQ_OK) s = dev_alloc(ctx, (void **)&k.ints, (2 * blocks + 10) * 4, "cache tables");
+    if (s == NNQ_OK) s = dev_alloc(ctx, (void **)&k.krot, (size_t)d->lkv * 128 * 4, "decoder buffer");
+    if (s == NNQ_OK) {
+        k.layer0 = {format, d->lkv, 128, block, blocks, k.mem, k.mem + codes, k.mem + 2 * codes, k.mem + 2 * codes + exps};
+        const nnq_kv_batch b = {k.ints, k.ints, k.ints, 1, blocks, 1, 1};
+        s = nnq_kv_attention_workspace(ctx, &k.layer0, &b, d->lh, &k.work_bytes);
+    }
+    if (s == NNQ_OK) s = dev_alloc(ctx, &k.work, k.work_bytes, "attention workspace");
+    int *words = s == NNQ_OK ? new (std::nothrow) int[2 * blocks + 10]() : nullptr;
+    if (s == NNQ_OK && !words) s = fail(ctx, NNQ_ERR_OUT_OF_MEMORY, "host allocation failed");
+    if (s == NNQ_OK) {
+        for (int64_t i = 0; i < blocks; i++) words[i] = words[blocks + i] = (int)i;
+        words[2 * blocks + 6] = 1;   // (call[2]: the rows of a step)
+        s = check_cuda(ctx, cudaMemcpy(k.ints, words, (2 * blocks + 10) * 4, cudaMemcpyHostToDevice), "cache tables");
+    }
+    delete[] words;
+    nnq_decoder::Cache8 *held = s == NNQ_OK ? new (std::nothrow) nnq_decoder::Cache8() : nullptr;
+    if (s == NNQ_OK && !held) s = fail(ctx, NNQ_ERR_OUT_OF_MEMORY, "host allocation failed");
+    if (s != NNQ_OK) {
+        cudaFree(k.mem); cudaFree(k.ints); cudaFree(k.krot); cudaFree(k.work);
+        return s;
+    }
+    k.table = k.ints;
+    k.numbers = k.ints + blocks;
+    int *w = k.ints + 2 * blocks;
+    k.length = w;
+    k.row_start = w + 1;
+    k.used = w + 3;       // used, call[0], call[1] are written together
+    k.call = w + 4;
+    k.step_slot = w + 7;
+    k.step_pos = w + 8;
+    *held = k;
+    d->kv8 = held;
+    cudaFree(d->d_kcache);
+    cudaFree(d->d_vcache);
+    d->d_kcache = d->d_vcache = nullptr;
+    return NNQ_OK;
+}
+
+nnq_status nnq_decoder_cache(nnq_decoder *d, int layer, nnq_kv_cache *out) {
+    if (!d) return NNQ_ERR_INVALID_ARG;
+    if (!out || layer < 0 || layer >= d->cfg.n_layers) return fail(d->ctx, NNQ_ERR_INVALID_ARG, "layer %d out of range", layer);
+    if (!d->kv8) return fail(d->ctx, NNQ_ERR_UNSUPPORTED, "the decoder has no 8-bit cache");
+    const nnq_kv_cache &c = d->kv8->layer0;
+    const int64_t codes = c.blocks * c.kv_heads * c.block * c.dim, exps = c.blocks * c.kv_heads;
+    *out = c;
+    out->k = (uint8_t *)c.k + layer * codes;
+    out->v = (uint8_t *)c.v + layer * codes;
+    out->k_exp = c.k_exp + layer * exps;
+    out->v_exp = c.v_exp + layer * exps;
+    return NNQ_OK;
+}
+
 nnq_status nnq_decoder_reset(nnq_decoder *d, int token, int pos, void *stream) {
     if (!d) return NNQ_ERR_INVALID_ARG;
     if (token < 0 || token >= d->cfg.vocab || pos < 0 || pos >= d->cfg.max_seq) return fail(d->ctx, NNQ_ERR_INVALID_ARG, "token or position out of range");
@@ -1326,6 +1413,7 @@ nnq_status nnq_decoder_reset(nnq_decoder *d, int token, int pos, void *stream) {
         if (at != pos) return fail(d->ctx, NNQ_ERR_INVALID_ARG, "the decoder's state is at position %d: it can continue there or restart at 0, not at %d", at, pos);
     }
     d->host_pos = pos;
+    if (d->kv8 && (s = cache8_seek(d, pos, 1, (cudaStream_t)stream)) != NNQ_OK) return s;
     s = check_cuda(d->ctx, cudaMemcpyAsync(d->d_state, st, sizeof(st), cudaMemcpyHostToDevice, (cudaStream_t)stream), "decoder state");
     if (s == NNQ_OK) s = check_cuda(d->ctx, cudaStreamSynchronize((cudaStream_t)stream), "decoder state");   // st is on the stack
     return s;
@@ -1622,7 +1710,7 @@ static nnq_status rows_blocks(nnq_decoder *d, int n, int pos0, cudaStream_t st) 
 // kernels around them (five launches a layer instead of nine).
 static bool step_is_fused(const nnq_decoder *d) {
     const nnq_decoder_config &c = d->cfg;
-    if (d->blocks || d->comm || c.tp_world > 1 || d->act_dt != NNQ_BF16 || d->ctx->path != NNQ_PATH_AUTO || c.head_dim != 128) return false;
+    if (d->blocks || d->kv8 || d->comm || c.tp_world > 1 || d->act_dt != NNQ_BF16 || d->ctx->path != NNQ_PATH_AUTO || c.head_dim != 128) return false;
     for (int l = 0; l < c.n_layers; l++) {
         const nnq_decoder::Layer &L = d->layers[l];
         for (const nnq_weight *w : {L.q, L.k, L.v, L.gate, L.up})
@@ -1651,6 +1739,37 @@ static StepPart next_weights(StepPart part, const nnq_weight *a, const nnq_weigh
     return part;
 }
 
+// The 8-bit cache of a decoder: one request whose table is the identity. `past` and `count` are device words.
+static nnq_status cache8_tables(nnq_decoder *d, const int *past, const int *count, int rows, int *slot, int *pos, cudaStream_t st) {
+    nnq_decoder::Cache8 &k = *d->kv8;
+    const int blocks = (int)k.layer0.blocks;
+    return nnq_kv_tables(d->ctx, past, count, 1, k.numbers, blocks, k.used, k.layer0.block, k.table, blocks, k.length, k.row_start, slot, pos, rows, k.used, st);
+}
+
+// The table and the blocks taken for a sequence that goes on at position `pos` with `count` given rows.
+static nnq_status cache8_seek(nnq_decoder *d, int pos, int count, cudaStream_t st) {
+    nnq_decoder::Cache8 &k = *d->kv8;
+    const int words[3] = {(pos + k.layer0.block - 1) / k.layer0.block, pos, count};   // used, call
+    nnq_status s = check_cuda(d->ctx, cudaMemcpyAsync(k.table, k.numbers, (size_t)k.layer0.blocks * 4, cudaMemcpyDeviceToDevice, st), "cache table");
+    if (s == NNQ_OK) s = check_cuda(d->ctx, cudaMemcpyAsync(k.used, words, sizeof(words), cudaMemcpyHostToDevice, st), "cache table");
+    return s;
+}
+
+// Layer l: appends `rows` rows of rotated keys and of values, and attends to them and to what is in front of them.
+static nnq_status cache8_attend(nnq_decoder *d, int l, int rows, const float *krot, const float *v, const int *slot, const float *q, void *y, float scale, cudaStream_t st) {
+    const nnq_decoder::Cache8 &k = *d->kv8;
+    const int64_t kvdim = (int64_t)d->lkv * 128, qdim = (int64_t)d->lh * 128, codes = k.layer0.blocks * kvdim * k.layer0.block, exps = k.layer0.blocks * d->lkv;
+    nnq_kv_cache c = k.layer0;
+    c.k = (uint8_t *)c.k + (int64_t)l * codes;
+    c.v = (uint8_t *)c.v + (int64_t)l * codes;
+    c.k_exp += l * exps;
+    c.v_exp += l * exps;
+    nnq_status s = nnq_kv_append(d->ctx, &c, krot, kvdim, v, kvdim, NNQ_F32, slot, rows, st);
+    const nnq_kv_batch b = {k.length, k.row_start, k.table, 1, k.layer0.blocks, rows, rows};
+    if (s == NNQ_OK) s = nnq_kv_attention(d->ctx, &c, &b, q, NNQ_F32, qdim, d->lh, scale, 0, y, (nnq_dtype)d->act_dt, qdim, k.work, k.work_bytes, st);
+    return s;
+}
+
 static nnq_status step_qwen3(nnq_decoder *d, cudaStream_t st) {
     nnq_ctx *ctx = d->ctx;
     const nnq_decoder_config &c = d->cfg;
@@ -1661,6 +1780,7 @@ static nnq_status step_qwen3(nnq_decoder *d, cudaStream_t st) {
     const float scale = (float)(1.0 / sqrt((double)hd));
     const __nv_bfloat16 *embed = (const __nv_bfloat16 *)d->d_embed;
     const bool fused = step_is_fused(d);
+    if (d->kv8 && (s = cache8_tables(d, d->d_state + 1, d->kv8->call + 2, 1, d->kv8->step_slot, d->kv8->step_pos, st)) != NNQ_OK) return s;
     for (int l = 0; l < c.n_layers; l++) {
         const nnq_decoder::Layer &L = d->layers[l];
         if (!fused || l == 0) DEC_RUN(1, launch_pdl(dec_norm_kernel, dim3(1), dim3(1024), st, d->d_h, d->d_delta, l == 0 ? embed : nullptr, d->d_state, L.in_norm, c.rms_eps, d->d_xn, d->act_dt, c.hidden));
@@ -1674,9 +1794,13 @@ static nnq_status step_qwen3(nnq_decoder *d, cudaStream_t st) {
         } else {
             DEC_RUN(32, if ((s = nnq_linear_batch(ctx, 3, w3, x3, adt, 1, nullptr, y3, NNQ_F32, st)) != NNQ_OK) return s);
         }
-        if (!fused) DEC_RUN(2, launch_pdl(dec_qk_rope_kernel, dim3(lh + 2 * lkv), dim3(hd), st, d->d_q, d->d_k, d->d_v, L.q_norm, L.k_norm, d->d_cos, d->d_sin, d->d_state,
-                              c.rms_eps, d->d_qrot, d->d_kcache + l * layer_cache, d->d_vcache + l * layer_cache, lh, lkv, hd, c.max_seq));
-        DEC_RUN(4, {
+        if (!fused && !d->kv8) DEC_RUN(2, launch_pdl(dec_qk_rope_kernel, dim3(lh + 2 * lkv), dim3(hd), st, d->d_q, d->d_k, d->d_v, L.q_norm, L.k_norm, d->d_cos, d->d_sin, d->d_state,
+                              c.rms_eps, d->d_qrot, d->d_kcache + l * layer_cache, d->d_vcache + l * layer_cache, lh, lkv, hd, (size_t)c.max_seq * hd, (size_t)hd));
+        if (d->kv8) {
+            launch_pdl(dec_qk_rope_kernel, dim3(lh + lkv), dim3(hd), st, d->d_q, d->d_k, d->d_v, L.q_norm, L.k_norm, d->d_cos, d->d_sin, d->d_state, c.rms_eps, d->d_qrot,
+                       d->kv8->krot, (float *)nullptr, lh, lkv, hd, (size_t)hd, (size_t)0);
+            if ((s = cache8_attend(d, l, 1, d->kv8->krot, d->d_v, d->kv8->step_slot, d->d_qrot, d->d_attn, scale, st)) != NNQ_OK) return s;
+        } else DEC_RUN(4, {
             float *kc = d->d_kcache + l * layer_cache, *vc = d->d_vcache + l * layer_cache;
             const NewRows nr = {d->d_k, d->d_v, L.q_norm, L.k_norm, d->d_cos, d->d_sin, c.rms_eps};
             switch (group) {
@@ -1712,7 +1836,7 @@ static nnq_status step_qwen3(nnq_decoder *d, cudaStream_t st) {
         DEC_RUN(32, s = d->comm ? nnq_comm_linear(d->comm, L.down, d->d_mid, adt, 1, nullptr, d->d_delta, NNQ_F32, st)
                                 : nnq_linear(ctx, L.down, d->d_mid, adt, 1, nullptr, d->d_delta, NNQ_F32, st));
         if (s != NNQ_OK) return s;
-        ctx->launches += 5;
+        ctx->launches += d->kv8 ? 4 : 5;
     }
     return NNQ_OK;
 }
@@ -1783,6 +1907,7 @@ static nnq_status rows_qwen3(nnq_decoder *d, int n, int pos0, cudaStream_t st) {
     const bool together = n > 512 && ctx->path == NNQ_PATH_AUTO && d->act_dt == NNQ_BF16;
     if (together) pair_reserve(d);
     int held = 0;   // kv heads that the prompt attention on the tensor cores takes at a time
+    if (d->kv8 && (s = cache8_tables(d, d->kv8->call, d->kv8->call + 1, n, d->pf_slot, d->pf_pos, st)) != NNQ_OK) return s;
     for (int l = 0; l < c.n_layers; l++) {
         const nnq_decoder::Layer &L = d->layers[l];
         float *kc = d->d_kcache + l * layer_cache, *vc = d->d_vcache + l * layer_cache;
@@ -1791,8 +1916,11 @@ static nnq_status rows_qwen3(nnq_decoder *d, int n, int pos0, cudaStream_t st) {
         const void *x3[3] = {d->pf_xn, d->pf_xn, d->pf_xn};
         void *y3[3] = {d->pf_q, d->pf_k, d->pf_v};
         if ((s = nnq_linear_batch(ctx, 3, w3, x3, adt, n, nullptr, y3, NNQ_F32, st)) != NNQ_OK) return s;
-        if (hd == 128)
-            launch_qk_rope_rows128(d->pf_q, d->pf_k, d->pf_v, L.q_norm, L.k_norm, d->d_cos, d->d_sin, pos0, c.rms_eps, d->pf_qrot, kc, vc, lh, lkv, n, c.max_seq, st);
+        if (d->kv8)
+            launch_qk_rope_rows128(d->pf_q, d->pf_k, d->pf_v, L.q_norm, L.k_norm, d->d_cos, d->d_sin, pos0, c.rms_eps, d->pf_qrot, d->pf_krot - (int64_t)pos0 * lkv * hd, nullptr, lh, lkv, n,
+                                   hd, (size_t)lkv * hd, st);
+        else if (hd == 128)
+            launch_qk_rope_rows128(d->pf_q, d->pf_k, d->pf_v, L.q_norm, L.k_norm, d->d_cos, d->d_sin, pos0, c.rms_eps, d->pf_qrot, kc, vc, lh, lkv, n, (size_t)c.max_seq * hd, hd, st);
         else
             dec_qk_rope_rows_kernel<<<dim3(lh + 2 * lkv, n), hd, 0, st>>>(d->pf_q, d->pf_k, d->pf_v, L.q_norm, L.k_norm, d->d_cos, d->d_sin, pos0,
                                                                      c.rms_eps, d->pf_qrot, kc, vc, lh, lkv, hd, c.max_seq);
@@ -1814,7 +1942,7 @@ static nnq_status rows_qwen3(nnq_decoder *d, int n, int pos0, cudaStream_t st) {
         wa.ffn.act = d->pf_attn;
         wa.ffn.act_dt = d->act_dt;
         wa.ffn.out_k = lh * hd;
-        if (l == 0 && attn_split_supported(wa) && pos0 + n >= 64) held = image_heads(d, pos0 + n);
+        if (l == 0 && !d->kv8 && attn_split_supported(wa) && pos0 + n >= 64) held = image_heads(d, pos0 + n);
         const bool tc = held > 0;
         if (tc && (s = launch_attn_split(ctx, wa, d->pf_top, d->pf_images, held, st)) != NNQ_OK) return s;
         // 16 query vectors per warp: R = 16 / G rows share each key / value row
@@ -1824,7 +1952,8 @@ static nnq_status rows_qwen3(nnq_decoder *d, int n, int pos0, cudaStream_t st) {
             else launch_pdl(all, dim3(lkv, blocks), dim3(32), st, d->pf_qrot, kc, vc, pos0, n, scale, d->pf_attn, d->act_dt, lh, hd, c.max_seq, tc ? d->pf_top : nullptr,
                             attn_tiles(pos0 + n));
         };
-        switch (group) {
+        if (d->kv8 && (s = cache8_attend(d, l, n, d->pf_krot, d->pf_v, d->pf_slot, d->pf_qrot, d->pf_attn, scale, st)) != NNQ_OK) return s;
+        if (!d->kv8) switch (group) {
             case 1: attend(dec_attn_rows_kernel<1, 16>, dec_attn_left_kernel<1, 16>, 16); break;
             case 2: attend(dec_attn_rows_kernel<2, 8>, dec_attn_left_kernel<2, 8>, 8); break;
             case 4: attend(dec_attn_rows_kernel<4, 4>, dec_attn_left_kernel<4, 4>, 4); break;
@@ -1859,7 +1988,7 @@ static nnq_status rows_qwen3(nnq_decoder *d, int n, int pos0, cudaStream_t st) {
         s = d->comm ? nnq_comm_linear(d->comm, L.down, d->pf_mid, adt, n, nullptr, d->pf_delta, NNQ_F32, st)
                     : nnq_linear(ctx, L.down, d->pf_mid, adt, n, nullptr, d->pf_delta, NNQ_F32, st);
         if (s != NNQ_OK) return s;
-        ctx->launches += 5;
+        ctx->launches += d->kv8 ? 4 : 5;
     }
     return NNQ_OK;
 }
@@ -1921,7 +2050,7 @@ static nnq_status alloc_row_buffers(nnq_decoder *d, size_t R) {
                 {(void **)&d->pf_k, R * kvdim * 4}, {(void **)&d->pf_v, R * kvdim * 4}, {(void **)&d->pf_qrot, R * qdim * 4},
                 {(void **)&d->pf_g, R * lffn * 4}, {(void **)&d->pf_u, R * lffn * 4}, {&d->pf_xn, R * c.hidden * es},
                 {&d->pf_attn, R * qdim * es}, {&d->pf_mid, R * lffn * es}, {(void **)&d->pf_tokens, (R + 1) * 4},
-                {(void **)&d->pf_want, R * 4}, {(void **)&d->pf_top, d->lkv * (size_t)attn_tiles(c.max_seq) * sizeof(uint2)}};
+                {(void **)&d->pf_want, R * 4}, {(void **)&d->pf_krot, d->kv8 ? R * kvdim * 4 : 0}, {(void **)&d->pf_slot, d->kv8 ? R * 4 : 0}, {(void **)&d->pf_pos, d->kv8 ? R * 4 : 0}, {(void **)&d->pf_top, d->lkv * (size_t)attn_tiles(c.max_seq) * sizeof(uint2)}};
     size_t total = 0;
     for (const auto &q : part) total += (q.bytes + 255) / 256 * 256;
     void *mem = nullptr;
@@ -1978,6 +2107,7 @@ static nnq_status run_rows(nnq_decoder *d, const int32_t *tokens_host, int n, in
         if (s == NNQ_OK) s = check_cuda(d->ctx, cudaMemcpyAsync(d->d_state + 4, d->pf_tokens + n, 4, cudaMemcpyDeviceToDevice, st), "prompt tokens");
         if (s != NNQ_OK) return s;
     }
+    if (d->kv8 && (s = cache8_seek(d, pos0, n, st)) != NNQ_OK) return s;
     return d->blocks ? rows_blocks(d, n, pos0, st) : rows_qwen3(d, n, pos0, st);
 }
 
@@ -2013,14 +2143,14 @@ nnq_status nnq_decoder_prefill(nnq_decoder *d, const int32_t *tokens_host, int c
     return s;
 }
 
-nnq_status nnq_decoder_extend(nnq_decoder *d, const int32_t *tokens_host, int count, int start_pos, const int32_t *want, int n_want,
-                              float *logits_host, void *stream) {
-    if (!d) return NNQ_ERR_INVALID_ARG;
+extern "C++" {
+// Feeds `count` given tokens from start_pos on and hands the logits after the wanted ones to emit(rows of logits, first of them in
+// want[], how many) in portions of up to kWantRows, ascending; the stream is waited for behind each.
+template <typename Emit>
+static nnq_status extend_with(nnq_decoder *d, const int32_t *tokens_host, int count, int start_pos, const int32_t *want, int n_want, void *stream, Emit emit) {
     nnq_ctx *ctx = d->ctx;
     const nnq_decoder_config &c = d->cfg;
-    nnq_status s = check_tokens(d, tokens_host, count, start_pos);
-    if (s != NNQ_OK) return s;
-    if (n_want < 0 || (n_want && (!want || !logits_host))) return fail(ctx, NNQ_ERR_INVALID_ARG, "bad list of wanted positions");
+    nnq_status s = NNQ_OK;
     for (int i = 0; i < n_want; i++)
         if (want[i] < 0 || want[i] >= count || (i && want[i] <= want[i - 1])) return fail(ctx, NNQ_ERR_INVALID_ARG, "wanted positions must be ascending and inside the tokens");
     if (d->head_rows != c.vocab) return fail(ctx, NNQ_ERR_UNSUPPORTED, "wanted logits need the whole vocabulary projection on this rank");
@@ -2029,7 +2159,7 @@ nnq_status nnq_decoder_extend(nnq_decoder *d, const int32_t *tokens_host, int co
     if (count == 1) {
         if ((s = nnq_decoder_reset(d, tokens_host[0], start_pos, stream)) != NNQ_OK) return s;
         if ((s = nnq_decoder_step(d, stream)) != NNQ_OK) return s;
-        if (n_want) s = check_cuda(ctx, cudaMemcpyAsync(logits_host, d->d_logits, (size_t)c.vocab * 4, cudaMemcpyDeviceToHost, st), "logits");
+        if (n_want) s = emit(d->d_logits, 0, 1);
         if (s == NNQ_OK) s = check_cuda(ctx, cudaStreamSynchronize(st), "decoder step");
         return s;
     }
@@ -2055,7 +2185,7 @@ nnq_status nnq_decoder_extend(nnq_decoder *d, const int32_t *tokens_host, int co
             if (s == NNQ_OK) s = product(d, d->lm_head, d->pf_xn, m, nullptr, d->d_want_logits, st);
             if (s == NNQ_OK && d->logit_cap > 0.0f) s = launch_logit_cap(ctx, d->d_want_logits, d->logit_cap, (long long)m * c.vocab, st);
             if (s != NNQ_OK) return s;
-            s = check_cuda(ctx, cudaMemcpyAsync(logits_host + (size_t)w0 * c.vocab, d->d_want_logits, (size_t)m * c.vocab * 4, cudaMemcpyDeviceToHost, st), "logits");
+            s = emit(d->d_want_logits, w0, m);
             if (s == NNQ_OK) s = check_cuda(ctx, cudaStreamSynchronize(st), "logits");   // rows[] is on the stack
             if (s != NNQ_OK) return s;
             w0 += m;
@@ -2067,6 +2197,54 @@ nnq_status nnq_decoder_extend(nnq_decoder *d, const int32_t *tokens_host, int co
     if (s == NNQ_OK) s = check_cuda(ctx, cudaStreamSynchronize(st), "prompt pass");
     if (s == NNQ_OK) d->host_pos = (long long)start_pos + count;
     return s;
+}
+
+}  // extern "C++"
+
+nnq_status nnq_decoder_extend(nnq_decoder *d, const int32_t *tokens_host, int count, int start_pos, const int32_t *want, int n_want,
+                              float *logits_host, void *stream) {
+    if (!d) return NNQ_ERR_INVALID_ARG;
+    nnq_ctx *ctx = d->ctx;
+    nnq_status s = check_tokens(d, tokens_host, count, start_pos);
+    if (s != NNQ_OK) return s;
+    if (n_want < 0 || (n_want && (!want || !logits_host))) return fail(ctx, NNQ_ERR_INVALID_ARG, "bad list of wanted positions");
+    const size_t vocab = d->cfg.vocab;
+    return extend_with(d, tokens_host, count, start_pos, want, n_want, stream, [&](const float *logits, int first, int m) {
+        return check_cuda(ctx, cudaMemcpyAsync(logits_host + first * vocab, logits, m * vocab * 4, cudaMemcpyDeviceToHost, (cudaStream_t)stream), "logits");
+    });
+}
+
+nnq_status nnq_decoder_score(nnq_decoder *d, const int32_t *tokens_host, int count, int start_pos, const int32_t *want, int n_want, const int32_t *given_host, int top,
+                             float *logprob_host, float *entropy_host, int32_t *top_token_host, float *top_logprob_host, void *stream) {
+    if (!d) return NNQ_ERR_INVALID_ARG;
+    nnq_ctx *ctx = d->ctx;
+    nnq_status s = check_tokens(d, tokens_host, count, start_pos);
+    if (s != NNQ_OK) return s;
+    if (n_want < 1 || !want || !given_host || !logprob_host || !entropy_host) return fail(ctx, NNQ_ERR_INVALID_ARG, "bad list of wanted positions");
+    if (top < 0 || top > 32 || top > d->cfg.vocab) return fail(ctx, NNQ_ERR_UNSUPPORTED, "%d alternatives: at most 32 and the vocabulary's size", top);
+    if (top && (!top_token_host || !top_logprob_host)) return fail(ctx, NNQ_ERR_INVALID_ARG, "NULL result");
+    for (int i = 0; i < n_want; i++)
+        if (given_host[i] >= d->cfg.vocab) return fail(ctx, NNQ_ERR_INVALID_ARG, "given token %d out of range", i);
+    if (!d->score_mem) {
+        if ((s = check_cuda(ctx, cudaSetDevice(ctx->device), "cudaSetDevice")) != NNQ_OK) return s;
+        void *mem = nullptr;
+        if ((s = dev_alloc(ctx, &mem, (size_t)kWantRows * (3 + 64) * 4, "scores")) != NNQ_OK) return s;
+        d->score_mem = mem;
+        int *w = (int *)mem;
+        d->scores = {w, w + 3 * kWantRows, (float *)w + kWantRows, (float *)w + 2 * kWantRows, (float *)w + 35 * kWantRows};
+    }
+    cudaStream_t st = (cudaStream_t)stream;
+    return extend_with(d, tokens_host, count, start_pos, want, n_want, stream, [&](const float *logits, int first, int m) {
+        const auto &o = d->scores;
+        const size_t n = m, at = first, k = top;
+        nnq_status r = check_cuda(ctx, cudaMemcpyAsync(o.token, given_host + at, n * 4, cudaMemcpyHostToDevice, st), "given tokens");
+        if (r == NNQ_OK) r = nnq_token_logprobs(ctx, logits, NNQ_F32, m, d->cfg.vocab, d->cfg.vocab, o.token, top, o.logprob, o.entropy, o.top_token, o.top_logprob, stream);
+        if (r == NNQ_OK) r = check_cuda(ctx, cudaMemcpyAsync(logprob_host + at, o.logprob, n * 4, cudaMemcpyDeviceToHost, st), "scores");
+        if (r == NNQ_OK) r = check_cuda(ctx, cudaMemcpyAsync(entropy_host + at, o.entropy, n * 4, cudaMemcpyDeviceToHost, st), "scores");
+        if (r == NNQ_OK && top) r = check_cuda(ctx, cudaMemcpyAsync(top_token_host + at * k, o.top_token, n * k * 4, cudaMemcpyDeviceToHost, st), "scores");
+        if (r == NNQ_OK && top) r = check_cuda(ctx, cudaMemcpyAsync(top_logprob_host + at * k, o.top_logprob, n * k * 4, cudaMemcpyDeviceToHost, st), "scores");
+        return r;
+    });
 }
 
 nnq_status nnq_decoder_state(nnq_decoder *d, int *token, int *pos, int *steps, void *stream) {
@@ -2086,6 +2264,11 @@ void nnq_decoder_destroy(nnq_decoder *d) {
     if (!d) return;
     cudaSetDevice(d->ctx->device);
     cudaDeviceSynchronize();
+    if (d->kv8) {
+        cudaFree(d->kv8->mem); cudaFree(d->kv8->ints); cudaFree(d->kv8->krot); cudaFree(d->kv8->work);
+        delete d->kv8;
+    }
+    cudaFree(d->score_mem);
     if (d->layers) {
         for (int l = 0; l < d->cfg.n_layers; l++) {
             cudaFree(d->layers[l].in_norm); cudaFree(d->layers[l].post_norm);

@@ -78,7 +78,7 @@ dec_norm_rows4_kernel(float *__restrict__ h, const float *__restrict__ delta, co
 __global__ void __launch_bounds__(256)
 dec_qk_rope_rows128_kernel(const float *__restrict__ q, const float *__restrict__ k, const float *__restrict__ v, const float *__restrict__ qw,
                            const float *__restrict__ kw, const float *__restrict__ cosv, const float *__restrict__ sinv, int pos0, float eps,
-                           float *__restrict__ qrot, float *__restrict__ kcache, float *__restrict__ vcache, int n_heads, int n_kv, int rows, int max_seq) {
+                           float *__restrict__ qrot, float *__restrict__ kcache, float *__restrict__ vcache, int n_heads, int n_kv, int rows, size_t head_ld, size_t pos_ld) {
     const int lane = threadIdx.x & 31, heads = n_heads + 2 * n_kv;
     const int64_t unit = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
     if (unit >= (int64_t)rows * heads) return;
@@ -86,7 +86,7 @@ dec_qk_rope_rows128_kernel(const float *__restrict__ q, const float *__restrict_
     const size_t qoff = (size_t)row * n_heads * 128, kvoff = (size_t)row * n_kv * 128;
     if (head >= n_heads + n_kv) {
         const int kvh = head - n_heads - n_kv;
-        reinterpret_cast<float4 *>(vcache + ((size_t)kvh * max_seq + pos) * 128)[lane] = reinterpret_cast<const float4 *>(v + kvoff + kvh * 128)[lane];
+        if (vcache) reinterpret_cast<float4 *>(vcache + kvh * head_ld + pos * pos_ld)[lane] = reinterpret_cast<const float4 *>(v + kvoff + kvh * 128)[lane];
         return;
     }
     const bool is_q = head < n_heads;
@@ -105,7 +105,7 @@ dec_qk_rope_rows128_kernel(const float *__restrict__ q, const float *__restrict_
         const float b = __shfl_xor_sync(0xFFFFFFFFu, a[i], 16);
         y[i] = lane < 16 ? a[i] * c[i] - b * sn[i] : b * sn[i] + a[i] * c[i];
     }
-    float *dst = is_q ? qrot + qoff + head * 128 : kcache + ((size_t)(head - n_heads) * max_seq + pos) * 128;
+    float *dst = is_q ? qrot + qoff + head * 128 : kcache + (head - n_heads) * head_ld + pos * pos_ld;
     reinterpret_cast<float4 *>(dst)[lane] = make_float4(y[0], y[1], y[2], y[3]);
 }
 
@@ -116,9 +116,9 @@ void launch_norm_rows4(float *h, const float *delta, const __nv_bfloat16 *embed,
 }
 
 void launch_qk_rope_rows128(const float *q, const float *k, const float *v, const float *qw, const float *kw, const float *cosv, const float *sinv, int pos0, float eps,
-                            float *qrot, float *kcache, float *vcache, int n_heads, int n_kv, int rows, int max_seq, cudaStream_t st) {
+                            float *qrot, float *kcache, float *vcache, int n_heads, int n_kv, int rows, size_t head_ld, size_t pos_ld, cudaStream_t st) {
     const int64_t units = (int64_t)rows * (n_heads + 2 * n_kv);
-    dec_qk_rope_rows128_kernel<<<(unsigned)((units + 7) / 8), 256, 0, st>>>(q, k, v, qw, kw, cosv, sinv, pos0, eps, qrot, kcache, vcache, n_heads, n_kv, rows, max_seq);
+    dec_qk_rope_rows128_kernel<<<(unsigned)((units + 7) / 8), 256, 0, st>>>(q, k, v, qw, kw, cosv, sinv, pos0, eps, qrot, kcache, vcache, n_heads, n_kv, rows, head_ld, pos_ld);
 }
 
 void launch_silu_mul_rows(nnq_ctx *ctx, const float *g, const float *u, void *mid, int act_dt, int64_t total, cudaStream_t st) {

@@ -115,6 +115,42 @@ class Decoder:
                                                                 api._stream_ptr(stream)))
         return out
 
+    def set_cache(self, fmt: int, block: int = 32):
+        """Keys and values in 8 bits (kv_cache.INT8 or E4M3), a scale for each `block` tokens and head, in place of f32: a quarter of the
+        memory, and steps behind long contexts read a quarter of the bytes; steps behind short ones take longer, as they are no
+        longer fused. Before the first token; Qwen3 decoders."""
+        self.backend.check(self.backend._lib.nnq_decoder_set_cache(self._handle, int(fmt), int(block)))
+
+    def cache(self, layer: int):
+        """A layer's 8-bit cache as (codes of the keys, of the values, exponent bytes of the keys, of the values): uint8 views of the library's
+        memory, [blocks, kv_heads, block, dim] and [blocks, kv_heads]; position p is token p mod block of block p / block."""
+        import torch
+        from .kv_cache import _Cache
+        c = _Cache()
+        self.backend.check(self.backend._lib.nnq_decoder_cache(self._handle, layer, ctypes.byref(c)))
+        dev = torch.device("cuda", self.backend.device)
+        view = lambda p, *shape: torch.as_tensor(_DevArray(p, shape, "|u1"), device=dev)  # noqa: E731
+        codes, exps = (c.blocks, c.kv_heads, c.block, c.dim), (c.blocks, c.kv_heads)
+        return view(c.k, *codes), view(c.v, *codes), view(c.k_exp, *exps), view(c.v_exp, *exps)
+
+    def score(self, tokens, start_pos: int = 0, given=None, top: int = 0, stream=None):
+        """Log probabilities of given tokens: feeds `tokens` at positions start_pos .. as ``extend`` does and returns, as numpy arrays in a
+        TokenLogprobs, that of given[i] after tokens[i], the entropy there and the `top` (0 .. 32) most probable tokens. `given`
+        defaults to the tokens themselves: each but the last is judged by the one behind it, and the last has none (0)."""
+        from .logprobs import TokenLogprobs
+        arr = np.ascontiguousarray(tokens, dtype=np.int32)
+        nxt = np.append(arr[1:], -1) if given is None else given
+        nxt = np.ascontiguousarray(nxt, dtype=np.int32)
+        if nxt.shape != arr.shape or arr.ndim != 1:
+            raise api.ShapeMismatch(f"{arr.shape} tokens and {nxt.shape} given ones")
+        n, idx = arr.size, np.arange(arr.size, dtype=np.int32)
+        lp, ent = np.empty(n, np.float32), np.empty(n, np.float32)
+        tt, tl = np.empty((n, max(top, 0)), np.int32), np.empty((n, max(top, 0)), np.float32)
+        self.backend.check(self.backend._lib.nnq_decoder_score(self._handle, arr.ctypes.data, n, int(start_pos), idx.ctypes.data, n, nxt.ctypes.data, int(top),
+                                                               lp.ctypes.data, ent.ctypes.data, tt.ctypes.data if top else None, tl.ctypes.data if top else None,
+                                                               api._stream_ptr(stream)))
+        return TokenLogprobs(lp, ent, tt, tl) if top else TokenLogprobs(lp, ent)
+
     def step(self, stream=None):
         self.backend.check(self.backend._lib.nnq_decoder_step(self._handle, api._stream_ptr(stream)))
 
@@ -128,7 +164,8 @@ class Decoder:
         return t.value, p.value, n.value
 
     def buffers(self):
-        """(key cache, value cache, logits, tokens) as torch views of the library's device memory."""
+        """(key cache, value cache, logits, tokens) as torch views of the library's device memory; the caches are None where the decoder
+        keeps them in 8 bits (``cache``)."""
         import torch
         k, v, lg, tk = ctypes.c_void_p(), ctypes.c_void_p(), ctypes.c_void_p(), ctypes.c_void_p()
         self.backend.check(self.backend._lib.nnq_decoder_buffers(self._handle, ctypes.byref(k), ctypes.byref(v), ctypes.byref(lg),
@@ -136,8 +173,8 @@ class Decoder:
         c = self.cfg
         dev = torch.device("cuda", self.backend.device)
         shape = (c.n_layers, c.n_kv_heads // c.tp_world, c.max_seq, c.head_dim)
-        return (torch.as_tensor(_DevArray(k.value, shape, "<f4"), device=dev),
-                torch.as_tensor(_DevArray(v.value, shape, "<f4"), device=dev),
+        return (torch.as_tensor(_DevArray(k.value, shape, "<f4"), device=dev) if k.value else None,
+                torch.as_tensor(_DevArray(v.value, shape, "<f4"), device=dev) if v.value else None,
                 torch.as_tensor(_DevArray(lg.value, (c.vocab,), "<f4"), device=dev),
                 torch.as_tensor(_DevArray(tk.value, (c.max_seq,), "<i4"), device=dev))
 
