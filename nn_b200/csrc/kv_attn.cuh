@@ -70,9 +70,15 @@ template <>
 struct CodePairs<NNQ_KV_E4M3> {
     static constexpr float unscale = 256.0f;
     static __device__ __forceinline__ uint32_t word(uint32_t w) { return w; }
-    static __device__ __forceinline__ uint32_t half(uint32_t x) { return (x & 0x80008000u) | ((x >> 1) & 0x3F803F80u); }
-    static __device__ __forceinline__ uint32_t low(uint32_t w) { return half(__byte_perm(w, 0, 0x1404)); }
-    static __device__ __forceinline__ uint32_t high(uint32_t w) { return half(__byte_perm(w, 0, 0x3424)); }
+    // 128 (b + (b & 128)) moves the magnitude by seven bits and the sign by eight; multiplications, as the logic pipe has enough to do
+    static __device__ __forceinline__ uint32_t half(uint32_t x) {
+        uint32_t t, r;
+        asm("mul.lo.u32 %0, %1, 128;" : "=r"(t) : "r"(x));
+        asm("mad.lo.u32 %0, %1, 128, %2;" : "=r"(r) : "r"(x & 0x00800080u), "r"(t));
+        return r;
+    }
+    static __device__ __forceinline__ uint32_t low(uint32_t w) { return half(__byte_perm(w, 0, 0x4140)); }
+    static __device__ __forceinline__ uint32_t high(uint32_t w) { return half(__byte_perm(w, 0, 0x4342)); }
     // (the upper bytes of the f16 numbers of all four codes, and the lower ones, then put together)
     static __device__ __forceinline__ void four(uint32_t w, uint32_t &p0, uint32_t &p1) {
         const uint32_t up = (w & 0x80808080u) | (((w & 0x7F7F7F7Fu) >> 1) & 0x7F7F7F7Fu), down = (w << 7) & 0x80808080u;
@@ -80,10 +86,11 @@ struct CodePairs<NNQ_KV_E4M3> {
         p1 = __byte_perm(down, up, 0x7362);
     }
     static __device__ __forceinline__ void pairs(uint32_t x, uint32_t y, uint32_t &p0, uint32_t &p1, uint32_t &p2, uint32_t &p3) {
-        p0 = half(__byte_perm(x, y, 0x4400));   // (the lower bytes of the halves are masked out)
-        p1 = half(__byte_perm(x, y, 0x5511));
-        p2 = half(__byte_perm(x, y, 0x6622));
-        p3 = half(__byte_perm(x, y, 0x7733));
+        const uint32_t a = low(x), b = low(y), c = high(x), d = high(y);
+        p0 = __byte_perm(a, b, 0x5410);
+        p1 = __byte_perm(a, b, 0x7632);
+        p2 = __byte_perm(c, d, 0x5410);
+        p3 = __byte_perm(c, d, 0x7632);
     }
 };
 
