@@ -773,7 +773,7 @@ NNQ_API nnq_status nnq_kv_append(nnq_ctx *ctx, const nnq_kv_cache *cache, const 
 NNQ_API nnq_status nnq_kv_read(nnq_ctx *ctx, const nnq_kv_cache *cache, const int32_t *slot_dev, int64_t rows, void *k_dev, void *v_dev, nnq_dtype dt, void *stream);
 
 /* The batch as attention reads it: what nnq_kv_tables writes. max_rows: rows of the request with the most, as far as the
- * host knows; it decides which kernels run, not what they compute. */
+ * host knows; it decides which kernels run and how much workspace they need, not what they compute. */
 typedef struct nnq_kv_batch {
     const int32_t *length, *row_start, *table;
     int64_t requests, table_ld, rows, max_rows;

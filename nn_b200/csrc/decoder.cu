@@ -1351,7 +1351,7 @@ nnq_status nnq_decoder_set_cache(nnq_decoder *d, int format, int block) {
     if (s == NNQ_OK) s = dev_alloc(ctx, (void **)&k.krot, (size_t)d->lkv * 128 * 4, "decoder buffer");
     if (s == NNQ_OK) {
         k.layer0 = {format, d->lkv, 128, block, blocks, k.mem, k.mem + codes, k.mem + 2 * codes, k.mem + 2 * codes + exps};
-        const nnq_kv_batch b = {k.ints, k.ints, k.ints, 1, blocks, 1, 1};
+        const nnq_kv_batch b = {k.ints, k.ints, k.ints, 1, blocks, c.max_seq, c.max_seq};
         s = nnq_kv_attention_workspace(ctx, &k.layer0, &b, d->lh, &k.work_bytes);
     }
     if (s == NNQ_OK) s = dev_alloc(ctx, &k.work, k.work_bytes, "attention workspace");

@@ -28,9 +28,9 @@
 
 namespace nnq {
 
-constexpr int kKvWarps = 8, kKvCols = 8, kKvStep = 16, kKvStages = 3;
+constexpr int kKvWarps = 8, kKvCols = 8, kKvStep = 16, kKvStages = 2;
 constexpr int kKvMinSteps = kKvWarps;   // of a CTA's part
-constexpr int kKvPad = 16;
+constexpr int kKvPad = 32;
 constexpr int kFew = 64;   // see nnq_kv_attention
 constexpr int kNothing = INT32_MIN;   // in place of a block: no key of the step is seen
 constexpr float kKvLog2E = 1.4426950408889634f;
@@ -239,7 +239,7 @@ __global__ void __launch_bounds__(kKvWarps * 32, D <= 128 ? 2 : 1) kv_attn_kerne
         __syncthreads();   // the records of the item before have been read
         int blk = block_of(lane), ke, ve;
         fetch(0, __shfl_sync(0xFFFFFFFFu, blk, 0));
-        fetch(1, __shfl_sync(0xFFFFFFFFu, blk, 1));
+
         bytes_of(blk, ke, ve);
         int blk1 = kNothing, ke1 = 127, ve1 = 127;
 
@@ -321,10 +321,10 @@ __global__ void __launch_bounds__(kKvWarps * 32, D <= 128 ? 2 : 1) kv_attn_kerne
                 blk1 = n > j + 32 ? block_of(j + 32 + lane) : kNothing;
             }
             if ((j & 31) == 16 && n > (j | 31)) bytes_of(blk1, ke1, ve1);
-            fetch(j + 2, __shfl_sync(0xFFFFFFFFu, (j & 31) < 30 ? blk : blk1, (j + 2) & 31));
+            fetch(j + 1, __shfl_sync(0xFFFFFFFFu, (j & 31) < 31 ? blk : blk1, (j + 1) & 31));
             const int b = __shfl_sync(0xFFFFFFFFu, blk, j & 31);
             const float kf = pow2_byte(__shfl_sync(0xFFFFFFFFu, ke, j & 31)), vexp = (float)(__shfl_sync(0xFFFFFFFFu, ve, j & 31) - 127);
-            asm volatile("cp.async.wait_group 2;" ::: "memory");
+            asm volatile("cp.async.wait_group 1;" ::: "memory");
             __syncwarp();
             if (b >= 0 && b < a.blocks) {
                 const uint32_t k_s = ring + (uint32_t)(j % kKvStages) * STEP, v_s = k_s + kKvStep * D;
@@ -563,7 +563,8 @@ static size_t kv_records_bytes(nnq_ctx *ctx, int dim) { return (size_t)kv_parts(
 template <int FMT, int D, int QT>
 static nnq_status launch_kv_attn(nnq_ctx *ctx, const KvAttn &a, float *records, cudaStream_t st) {
     constexpr int smem = kv_smem_bytes<D>();
-    nnq_status s = check_cuda(ctx, cudaFuncSetAttribute(kv_attn_kernel<FMT, D, QT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), "attention shared memory");
+    static std::atomic<uint64_t> done;
+    nnq_status s = allow_smem(ctx, kv_attn_kernel<FMT, D, QT>, smem, done);
     if (s != NNQ_OK) return s;
     const int parts = kv_parts(ctx, D);
     KvJoin *joins = reinterpret_cast<KvJoin *>(reinterpret_cast<uint8_t *>(records) + kv_records_bytes(ctx, D));
@@ -588,6 +589,9 @@ static nnq_status launch_kv_attn(nnq_ctx *ctx, const KvAttn &a, float *records, 
     }
 }
 
+// Can the batch have requests for the tensor-core kernel?
+static bool tc_rows(int dim, int group, int64_t max_rows) { return kv_attn_tc_supported(dim) && max_rows > kFew / group; }
+
 static nnq_status check_batch(nnq_ctx *ctx, const nnq_kv_cache *c, const nnq_kv_batch *b, int heads) {
     nnq_status s = check_kv_cache(ctx, c);
     if (s != NNQ_OK) return s;
@@ -609,7 +613,8 @@ nnq_status nnq_kv_attention_workspace(nnq_ctx *ctx, const nnq_kv_cache *c, const
     if (!bytes) return fail(ctx, NNQ_ERR_INVALID_ARG, "NULL result");
     nnq_status s = check_batch(ctx, c, b, heads);
     if (s != NNQ_OK) return s;
-    *bytes = std::max(kv_records_bytes(ctx, c->dim) + kv_parts(ctx, c->dim) * sizeof(KvJoin), kv_attn_tc_workspace(ctx, c->dim));
+    *bytes = kv_records_bytes(ctx, c->dim) + kv_parts(ctx, c->dim) * sizeof(KvJoin);
+    if (tc_rows(c->dim, heads / c->kv_heads, b->max_rows)) *bytes = std::max(*bytes, kv_attn_tc_workspace(ctx, c->dim));
     return NNQ_OK;
 }
 
@@ -635,7 +640,7 @@ nnq_status nnq_kv_attention(nnq_ctx *ctx, const nnq_kv_cache *c, const nnq_kv_ba
                       c->kv_heads, heads / c->kv_heads, c->dim, log2_of(c->block), window, (int)q_dt, (int)y_dt, INT32_MAX, scale, ctx->d_status};
     // Requests of more than kFew query vectors per key / value head go to the tensor-core kernel where there can be any; the rest of the
     // batch, down to single tokens beside a prompt, to this file's.
-    if (kv_attn_tc_supported(a) && b->max_rows > kFew / a.group) {
+    if (tc_rows(a.dim, a.group, b->max_rows)) {
         a.few = b->requests == 1 ? 0 : kFew;   // (a request alone is a prompt)
         if ((s = launch_kv_attn_tc(ctx, a, c->format, (float *)workspace, (cudaStream_t)stream)) != NNQ_OK || a.few == 0) return s;
     }

@@ -116,7 +116,7 @@ __device__ __forceinline__ void kv_split(float x, float y, uint32_t &hi, uint32_
 }
 
 // kv_attn_tc.cu: requests of more than a.few query vectors per key / value head
-bool kv_attn_tc_supported(const KvAttn &a);
+bool kv_attn_tc_supported(int dim);
 size_t kv_attn_tc_workspace(nnq_ctx *ctx, int dim);
 nnq_status launch_kv_attn_tc(nnq_ctx *ctx, const KvAttn &a, int fmt, float *records, cudaStream_t st);
 

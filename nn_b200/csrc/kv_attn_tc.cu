@@ -720,14 +720,15 @@ __global__ void __launch_bounds__(kTcCols) kv_tc_join_kernel(const KvAttn a, con
     }
 }
 
-bool kv_attn_tc_supported(const KvAttn &a) { return a.dim == 64 || a.dim == 128; }
+bool kv_attn_tc_supported(int dim) { return dim == 64 || dim == 128; }
 static size_t tc_records_bytes(nnq_ctx *ctx, int dim) { return (size_t)ctx->sm_count * 2 * tc_record_floats(dim) * 4; }
 size_t kv_attn_tc_workspace(nnq_ctx *ctx, int dim) { return tc_records_bytes(ctx, dim) + ctx->sm_count * sizeof(TcJoin); }
 
 template <int FMT, int D, int T>
 static nnq_status launch_tc(nnq_ctx *ctx, const KvAttn &a, float *records, cudaStream_t st) {
     constexpr int smem = TcShared<D, T>::bytes;
-    nnq_status s = check_cuda(ctx, cudaFuncSetAttribute(kv_attn_tc_kernel<FMT, D, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), "attention shared memory");
+    static std::atomic<uint64_t> done;
+    nnq_status s = allow_smem(ctx, kv_attn_tc_kernel<FMT, D, T>, smem, done);
     if (s != NNQ_OK) return s;
     TcJoin *joins = reinterpret_cast<TcJoin *>(reinterpret_cast<uint8_t *>(records) + tc_records_bytes(ctx, D));
     launch_pdl_smem(kv_attn_tc_kernel<FMT, D, T>, dim3(ctx->sm_count), dim3(kTcThreads), smem, st, a, records, joins);

@@ -12,6 +12,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <atomic>
+
 #include "nnq_internal.h"
 #include "pdl.cuh"
 
@@ -54,6 +56,17 @@ inline nnq_status check_kv_cache(nnq_ctx *ctx, const nnq_kv_cache *c) {
     if (!c->k || !c->v || !c->k_exp || !c->v_exp) return fail(ctx, NNQ_ERR_INVALID_ARG, "NULL tensor in a cache");
     if (((uintptr_t)c->k | (uintptr_t)c->v) & 15u) return fail(ctx, NNQ_ERR_INVALID_ARG, "codes of a cache must be 16-byte aligned");
     return NNQ_OK;
+}
+
+// Dynamic shared memory of a kernel beyond the default, asked for once per device (a call of its own takes about 1 us): `done` is a
+// static of the caller's, one for each kernel.
+template <typename K>
+inline nnq_status allow_smem(nnq_ctx *ctx, K kernel, size_t bytes, std::atomic<uint64_t> &done) {
+    const uint64_t bit = 1ull << (ctx->device & 63);
+    if (done.load(std::memory_order_relaxed) & bit) return NNQ_OK;
+    nnq_status s = check_cuda(ctx, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes), "shared memory of a kernel");
+    if (s == NNQ_OK && ctx->device < 64) done.fetch_or(bit, std::memory_order_relaxed);
+    return s;
 }
 
 inline int log2_of(int x) { return 31 - __builtin_clz((unsigned)x); }

@@ -118,7 +118,7 @@ class KvCache:
         z = lambda *s: torch.zeros(s, dtype=torch.uint8, device=self.device)  # noqa: E731
         self.k, self.v = z(blocks, kv_heads, block, dim), z(blocks, kv_heads, block, dim)
         self.k_exp, self.v_exp = z(blocks, kv_heads).fill_(127), z(blocks, kv_heads).fill_(127)
-        self._need = {}   # workspace by the number of query heads
+        self._need = {}   # workspace by numbers of query heads and rows
         self._c = _Cache(self.fmt, self.kv_heads, self.dim, self.block, self.blocks, self.k.data_ptr(), self.v.data_ptr(), self.k_exp.data_ptr(), self.v_exp.data_ptr())
         self._ref = ctypes.byref(self._c)
 
@@ -194,11 +194,11 @@ class KvCache:
         if batch.block != self.block or batch.backend.device != b.device:
             raise api.InvalidArgument(f"a batch of blocks of {batch.block} on {batch.device} for a cache of blocks of {self.block} on {self.device}")
         c = _Batch(batch.length.data_ptr(), batch.row_start.data_ptr(), batch.table.data_ptr(), batch.requests, batch.table.shape[1], n, max(int(max_rows), 1))
-        need = self._need.get(heads)
-        if need is None:   # (depends on the cache and the heads alone)
+        need = self._need.get((heads, c.max_rows))
+        if need is None:
             size = ctypes.c_size_t()
             b.check(b._lib.nnq_kv_attention_workspace(b._ctx, self._ref, ctypes.byref(c), heads, ctypes.byref(size)))
-            need = self._need[heads] = size.value
+            need = self._need[heads, c.max_rows] = size.value
         work = torch.empty(need, dtype=torch.uint8, device=self.device)
         st = b._lib.nnq_kv_attention(b._ctx, self._ref, ctypes.byref(c), q.data_ptr(), api._dtype_code(q), q.stride(0) if n > 1 else ld, heads,
                                      1.0 / math.sqrt(self.dim) if scale is None else float(scale), int(window), out.data_ptr(), api._dtype_code(out),

@@ -37,16 +37,18 @@ def token_logprobs(logits, tokens, top: int = 0, backend: Optional[api.Backend] 
         logits = logits.contiguous()
     if tokens.dtype != torch.int32:
         tokens = tokens.clamp(-1, 2 ** 31 - 1).to(torch.int32)
-    tokens = tokens.contiguous()
+    if not tokens.is_contiguous():
+        tokens = tokens.contiguous()
     if top < 0 or top > min(32, vocab):
         raise api.Unsupported(f"{top} alternatives: at most 32 and the vocabulary's size")
-    # one allocation: log probabilities, entropies, then both tables of alternatives
-    mem = torch.empty((2 + 2 * top) * rows, dtype=torch.float32, device=logits.device)
-    at = mem.data_ptr()
-    st = b._lib.nnq_token_logprobs(b._ctx, logits.data_ptr(), api._dtype_code(logits), rows, vocab, logits.stride(0) if rows > 1 else vocab, tokens.data_ptr(), int(top),
-                                   at, at + 4 * rows, at + 8 * rows if top else None, at + 4 * (2 + top) * rows if top else None, api._stream_ptr(None, b.device))
+    dev = logits.device
+    pair = torch.empty((2, rows), dtype=torch.float32, device=dev)
+    at = pair.data_ptr()
+    tt = tl = None
+    if top:
+        tt, tl = torch.empty((rows, top), dtype=torch.int32, device=dev), torch.empty((rows, top), dtype=torch.float32, device=dev)
+    st = b._lib.nnq_token_logprobs(b._ctx, logits.data_ptr(), api._dtype_code(logits), rows, vocab, logits.stride(0) if rows > 1 else vocab, tokens.data_ptr(), top,
+                                   at, at + 4 * rows, tt.data_ptr() if top else None, tl.data_ptr() if top else None, api._stream_ptr(None, b.device))
     if st:
         b.check(st)
-    if not top:
-        return TokenLogprobs(mem[:rows], mem[rows:])
-    return TokenLogprobs(mem[:rows], mem[rows:2 * rows], mem[2 * rows:(2 + top) * rows].view(torch.int32).view(rows, top), mem[(2 + top) * rows:].view(rows, top))
+    return TokenLogprobs(*pair.unbind(0), tt, tl)
