@@ -341,7 +341,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attn_tc_kernel(const KvAttn 
                         }
                     }
                 };
-#pragma unroll
+#pragma unroll 1
                 for (int c = 0; c < D / 32; c++) {
                     float x[32];
                     part(c, x);
@@ -349,7 +349,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attn_tc_kernel(const KvAttn 
                     for (int i = 0; i < 32; i++) big = max(big, __float_as_uint(x[i]) & 0x7FFFFFFFu);
                 }
                 const float sc = kv_top_scale(big);
-#pragma unroll
+#pragma unroll 1
                 for (int c = 0; c < D / 32; c++) {
                     float x[32];
                     part(c, x);
@@ -502,7 +502,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attn_tc_kernel(const KvAttn 
             if (whole) {
                 const float inv = none ? 0.0f : exp2f(mv - m) * Codes::unscale / l;
                 const int64_t to = (int64_t)(it.row0 + row) * a.y_ld + (int64_t)qhead * D;
-#pragma unroll
+#pragma unroll 1
                 for (int c = 0; c < D / 32; c++) {
                     uint32_t x[32];
                     tmem_ld32(o_t + 32 * c, x);
@@ -525,7 +525,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attn_tc_kernel(const KvAttn 
                 float4 *rec = reinterpret_cast<float4 *>(records + ((int64_t)blockIdx.x * 2 + (it.s0 == 0 ? 1 : 0)) * tc_record_floats(D));
                 const int v = w * 128 + me;
                 if (mine) rec[v] = make_float4(none ? -INFINITY : thr > -INFINITY ? m : l, mv, l, 0.0f);   // (l: scores that are all NaN)
-#pragma unroll
+#pragma unroll 1
                 for (int c = 0; c < D / 32; c++) {
                     uint32_t x[32];
                     tmem_ld32(o_t + 32 * c, x);
