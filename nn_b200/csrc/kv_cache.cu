@@ -414,7 +414,7 @@ nnq_status nnq_kv_append(nnq_ctx *ctx, const nnq_kv_cache *c, const void *k_dev,
     if (!rows_aligned(k_dev, k_ld, dt) || !rows_aligned(v_dev, v_ld, dt)) return fail(ctx, NNQ_ERR_INVALID_ARG, "rows of keys and values must start at multiples of 16 bytes");
     if ((s = check_cuda(ctx, cudaSetDevice(ctx->device), "cudaSetDevice")) != NNQ_OK) return s;
     const AppendArgs a = {{k_dev, k_ld, (uint8_t *)c->k, c->k_exp}, {v_dev, v_ld, (uint8_t *)c->v, c->v_exp}, slot_dev, rows, c->blocks * c->block, c->kv_heads, c->dim,
-                          log2_of(c->block), rows > 1024 ? 8 : 1, ctx->d_status};   // (few rows are single tokens more often than not: a warp each)
+                          log2_of(c->block), rows > 1024 ? 16 : 1, ctx->d_status};   // (few rows are single tokens more often than not: a warp each)
     const int64_t warps = (rows + a.tile - 1) / a.tile * 2 * c->kv_heads;
     if (warps / kAppWarps >= INT32_MAX) return fail(ctx, NNQ_ERR_UNSUPPORTED, "%lld rows of %d heads", (long long)rows, c->kv_heads);
     const dim3 grid((unsigned)((warps + kAppWarps - 1) / kAppWarps)), block(kAppWarps * 32);

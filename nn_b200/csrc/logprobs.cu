@@ -93,7 +93,7 @@ __device__ __forceinline__ void each_logit(const Slice<F32, kLpThreads> &s, F f)
 }
 
 template <bool F32, int kLpThreads>
-__global__ void __launch_bounds__(kLpThreads, kLpThreads == 256 ? 3 : 2) logprobs_kernel(const LogprobArgs a) {
+__global__ void __launch_bounds__(kLpThreads, kLpThreads == 256 ? 4 : 2) logprobs_kernel(const LogprobArgs a) {
     extern __shared__ float group_max[];   // [groups of a thread][threads]
     constexpr int kLpWarps = kLpThreads / 32;
     __shared__ Stats warp_stats[kLpWarps], cta_stats;
