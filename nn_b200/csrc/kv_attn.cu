@@ -15,7 +15,10 @@
 // and outputs are of f32 accuracy. A block's scales stay outside: the key's multiplies the scores, the value's goes into the exponent
 // of the weight, w = 2^(s - mv + e_v), which has a reference mv of its own beside the maximum m of the sum (l = sum 2^(s - m)): weights
 // stay between 0 and 2^8 whatever the scales are. Both references move only when a score passes them by 8, so most steps have one vote
-// in place of the maxima's exchange.
+// in place of the maxima's exchange. The tensor core cuts off what its f32 sums cannot hold, always towards zero, so chains in it are
+// kept short: 32 dimensions of a score, kKvFlush steps of an output, which then join sums in shared memory (2 requests of 130001
+// positions, f32: all steps in one chain 113.5 us and an error of the outputs against 64 bits of 2.3e-6, chains of 16 steps 114.8 us and
+// 0.86e-6, of 8 steps 116.6 us and 0.65e-6; torch in f32: 1.24e-6).
 //
 // Work is dealt in steps of 16 keys: all steps of all (request, head, vectors) items in one row, cut into equal parts, one for each
 // CTA, whatever the requests' lengths are. An item counts kKvPad steps more than it has, about what beginning and ending one takes, so
@@ -31,7 +34,7 @@ namespace nnq {
 constexpr int kKvWarps = 8, kKvCols = 8, kKvStep = 16, kKvStages = 2;
 constexpr int kKvMinSteps = kKvWarps;   // of a CTA's part
 constexpr int kKvPad = 32;
-constexpr int kFew = 64;   // see nnq_kv_attention
+constexpr int kKvFlush = 16;
 constexpr int kNothing = INT32_MIN;   // in place of a block: no key of the step is seen
 constexpr float kKvLog2E = 1.4426950408889634f;
 constexpr float kKvSlack = 8.0f;   // a score may pass the reference by this power of two: weights up to 256 in f16
@@ -53,7 +56,7 @@ struct KvPlan {
 
 // Steps of an item of the request (the same for all its heads and vectors), and its items of one head.
 __device__ __forceinline__ int item_steps(const KvAttn &a, const KvRequest &q) {
-    if (q.rows == 0 || q.rows * a.group > a.few) return 0;
+    if (q.rows == 0 || kv_many(a, q)) return 0;
     const int lo = row_first(a, max(row_pos(q, 0), 0)), steps = (q.length + kKvStep - 1) / kKvStep - lo / kKvStep;
     return max(steps, 1) + kKvPad;
 }
@@ -152,11 +155,10 @@ __device__ __forceinline__ uint2 lds64(uint32_t p) {
 __device__ __forceinline__ uint32_t chunk_at(int row, int c) { return (uint32_t)((row >> 1) * 128 + (((((row & 1) << 2) | c) ^ (((row >> 1) & 3) << 1)) << 4)); }
 
 template <int D>
-constexpr int kv_ring_bytes() { return kKvWarps * kKvStages * 2 * kKvStep * D; }
+constexpr int kKvRing = kKvWarps * kKvStages * 2 * kKvStep * D;
 template <int D>
 constexpr int kv_smem_bytes() {
-    const int merge = kKvWarps * kKvCols * (4 + D) * 4;
-    return kv_ring_bytes<D>() > merge ? kv_ring_bytes<D>() : merge;
+    return kKvRing<D> + kKvWarps * kKvCols * (4 + D) * 4;
 }
 
 __device__ __forceinline__ void store_out(const KvAttn &a, int64_t at, float y) {
@@ -166,12 +168,12 @@ __device__ __forceinline__ void store_out(const KvAttn &a, int64_t at, float y) 
 
 template <int FMT, int D, int QT>
 __global__ void __launch_bounds__(kKvWarps * 32, D <= 128 ? 2 : 1) kv_attn_kernel(const KvAttn a, float *records, KvJoin *joins) {
-    extern __shared__ __align__(128) uint8_t kv_smem[];   // the warps' rings; at the end of an item a record of every warp and column
+    extern __shared__ __align__(128) uint8_t kv_smem[];   // the warps' rings, then a record of every warp and column
     typedef CodePairs<FMT> Codes;
     constexpr int REC = 4 + D, STEP = 2 * kKvStep * D;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
     const uint32_t ring = smem_u32(kv_smem) + warp * kKvStages * STEP;
-    float *sm = reinterpret_cast<float *>(kv_smem);
+    float *sm = reinterpret_cast<float *>(kv_smem + kKvRing<D>);
     pdl_prologue();
     pdl_release();
     const KvPlan plan = kv_plan(a, gridDim.x);
@@ -310,6 +312,27 @@ __global__ void __launch_bounds__(kKvWarps * 32, D <= 128 ? 2 : 1) kv_attn_kerne
             for (int j = 0; j < 4; j++) acc[i][j] = 0.0f;
         float m[2] = {0.0f, 0.0f}, mv[2] = {0.0f, 0.0f}, l[2] = {0.0f, 0.0f};
         float thr[2] = {-INFINITY, -INFINITY}, thv[2] = {-INFINITY, -INFINITY};   // what makes the references move
+        float kept[2] = {-INFINITY, -INFINITY};   // reference of the sums in shared memory (-inf: none yet)
+        auto flush = [&]() {
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+                if (2 * t + j >= vecs || thr[j] == -INFINITY) continue;
+                float *rec = sm + (warp * kKvCols + 2 * t + j) * REC + 4 + 8 * g;
+                const float f = kv_ex2(kept[j] - mv[j]);
+#pragma unroll
+                for (int i = 0; i < D / 16; i += 2) {
+                    float4 *p = reinterpret_cast<float4 *>(rec + (i >> 2) * 64 + (i & 2) * 2);
+                    float4 o = make_float4(acc[i][j], acc[i][j + 2], acc[i + 1][j], acc[i + 1][j + 2]);
+                    if (kept[j] != -INFINITY) {
+                        const float4 q = *p;
+                        o = make_float4(fmaf(q.x, f, o.x), fmaf(q.y, f, o.y), fmaf(q.z, f, o.z), fmaf(q.w, f, o.w));
+                    }
+                    *p = o;
+                    acc[i][j] = acc[i][j + 2] = acc[i + 1][j] = acc[i + 1][j + 2] = 0.0f;
+                }
+                kept[j] = mv[j];
+            }
+        };
 
         for (int j = 0; j < n; j++) {
             if ((j & 31) == 0) {
@@ -329,7 +352,6 @@ __global__ void __launch_bounds__(kKvWarps * 32, D <= 128 ? 2 : 1) kv_attn_kerne
             if (b >= 0 && b < a.blocks) {
                 const uint32_t k_s = ring + (uint32_t)(j % kKvStages) * STEP, v_s = k_s + kKvStep * D;
                 // ---- scores
-                // (sums of 32 dimensions each: the tensor core cuts off what its f32 sums cannot hold, and long chains of that lean one way)
                 float part[D / 32][4];
 #pragma unroll
                 for (int c = 0; c < D / 64; c++) {
@@ -418,28 +440,22 @@ __global__ void __launch_bounds__(kKvWarps * 32, D <= 128 ? 2 : 1) kv_attn_kerne
                     }
                 }
             }
+            if ((j & (kKvFlush - 1)) == kKvFlush - 1) flush();
             __syncwarp();   // the stage may be written again
         }
+        flush();
         asm volatile("cp.async.wait_group 0;" ::: "memory");
 
-        // ---- the warps' sums in shared memory: a record per warp and column (m = -inf: nothing seen)
-        __syncthreads();
+        // ---- the rest of the warps' records (m = -inf: nothing seen)
 #pragma unroll
         for (int j = 0; j < 2; j++) {
 #pragma unroll
             for (int o = 4; o < 32; o <<= 1) l[j] += __shfl_xor_sync(0xFFFFFFFFu, l[j], o);
-            if (2 * t + j >= vecs) continue;
+            if (2 * t + j >= vecs || g > 0) continue;
             float *rec = sm + (warp * kKvCols + 2 * t + j) * REC;
-            if (g == 0) {
-                rec[0] = thr[j] > -INFINITY ? m[j] : (l[j] == 0.0f ? -INFINITY : l[j]);   // (scores that are all NaN move no reference)
-                rec[1] = mv[j];
-                rec[2] = l[j];
-            }
-            if (thr[j] > -INFINITY) {
-#pragma unroll
-                for (int i = 0; i < D / 16; i += 2)
-                    *reinterpret_cast<float4 *>(rec + 4 + (i >> 2) * 64 + 8 * g + (i & 2) * 2) = make_float4(acc[i][j], acc[i][j + 2], acc[i + 1][j], acc[i + 1][j + 2]);
-            }
+            rec[0] = thr[j] > -INFINITY ? m[j] : (l[j] == 0.0f ? -INFINITY : l[j]);   // (scores that are all NaN move no reference)
+            rec[1] = mv[j];
+            rec[2] = l[j];
         }
         __syncthreads();
         const bool whole = v0 == 0 && v1 == spi;
@@ -589,8 +605,8 @@ static nnq_status launch_kv_attn(nnq_ctx *ctx, const KvAttn &a, float *records, 
     }
 }
 
-// Can the batch have requests for the tensor-core kernel?
-static bool tc_rows(int dim, int group, int64_t max_rows) { return kv_attn_tc_supported(dim) && max_rows > kFew / group; }
+// Can the batch have requests for the tensor-core kernel, whatever their lengths are?
+static bool tc_rows(int dim, int group, int64_t max_rows) { return kv_attn_tc_supported(dim) && max_rows > kKvFew / group; }
 
 static nnq_status check_batch(nnq_ctx *ctx, const nnq_kv_cache *c, const nnq_kv_batch *b, int heads) {
     nnq_status s = check_kv_cache(ctx, c);
@@ -638,10 +654,13 @@ nnq_status nnq_kv_attention(nnq_ctx *ctx, const nnq_kv_cache *c, const nnq_kv_ba
     if ((s = check_cuda(ctx, cudaSetDevice(ctx->device), "cudaSetDevice")) != NNQ_OK) return s;
     KvAttn a = {(const uint8_t *)c->k, (const uint8_t *)c->v, c->k_exp, c->v_exp, b->length, b->row_start, b->table, q_dev, y_dev, c->blocks, b->table_ld, b->requests, q_ld, y_ld, b->rows,
                       c->kv_heads, heads / c->kv_heads, c->dim, log2_of(c->block), window, (int)q_dt, (int)y_dt, INT32_MAX, scale, ctx->d_status};
-    // Requests of more than kFew query vectors per key / value head go to the tensor-core kernel where there can be any; the rest of the
-    // batch, down to single tokens beside a prompt, to this file's.
-    if (tc_rows(a.dim, a.group, b->max_rows)) {
-        a.few = b->requests == 1 ? 0 : kFew;   // (a request alone is a prompt)
+    // The batch's requests are dealt between the two kernels on the device (kv_many). The tensor-core kernel is not launched where the
+    // rows, the table's width and the window leave it none; a prompt alone goes to it wholly.
+    const bool prompt = b->max_rows > 2 * kKvFew / a.group;
+    int64_t keys = std::min<int64_t>(b->table_ld * c->block, INT32_MAX);
+    if (window > 0) keys = std::min(keys, window + std::min(b->max_rows, b->rows));
+    if (tc_rows(a.dim, a.group, b->max_rows) && (prompt || keys * a.kv_heads >= (kKvManyKeys + b->requests - 1) / b->requests)) {
+        a.few = prompt && b->requests == 1 ? 0 : kKvFew;
         if ((s = launch_kv_attn_tc(ctx, a, c->format, (float *)workspace, (cudaStream_t)stream)) != NNQ_OK || a.few == 0) return s;
     }
     return c->format == NNQ_KV_INT8 ? launch_kv_attn<NNQ_KV_INT8>(ctx, a, (float *)workspace, (cudaStream_t)stream)

@@ -12,7 +12,7 @@ struct KvAttn {
     int64_t blocks, table_ld, requests, q_ld, y_ld, rows;
     int kv_heads, group, dim, shift, window;   // window 0: every earlier position
     int q_dt, y_dt;
-    int few;   // query vectors of a request and key / value head up to which kv_attn_kernel takes it; beyond: kv_attn_tc_kernel
+    int few;   // see kv_many: 0 (all requests go to kv_attn_tc_kernel), kKvFew or INT32_MAX (none goes)
     float scale;
     int *status;
 };
@@ -35,6 +35,25 @@ __device__ __forceinline__ KvRequest kv_request(const KvAttn &a, int64_t r) {
 // position of row i, and the first position it sees
 __device__ __forceinline__ int row_pos(const KvRequest &q, int i) { return q.length - q.rows + i; }
 __device__ __forceinline__ int row_first(const KvAttn &a, int pos) { return a.window > 0 && pos >= a.window ? pos - a.window + 1 : 0; }
+
+// Which kernel a request goes to. kv_attn_tc_kernel takes 256 query vectors of a key / value head for the price of one, but begins
+// slowly and deals a batch in coarser parts; kv_attn_kernel reads the keys again for every 8 vectors. Heads of 128, int8, bf16, group 4,
+// 8 key / value heads, us of kv_attn_kernel / kv_attn_tc_kernel:
+//   vectors           40             56             80            112
+//   2 x 500      18.0 / 27.4    19.8 / 28.0    22.7 / 28.3    23.7 / 29.6
+//   2 x 4000     29.1 / 40.6    36.3 / 41.6    46.2 / 42.9    58.6 / 44.7
+//   16 x 500     43.1 / 36.1    50.4 / 36.5    67.1 / 37.4    85.3 / 37.9
+//   2 x 30000     119 / 110      161 / 111      224 / 112      306 / 115
+//   16 x 4000     142 / 117      191 / 118      267 / 122      362 / 124
+//   16 x 30000    929 / 638     1233 / 619     1949 / 626     2715 / 635
+// and up to 32 vectors the first wins everywhere. So: beyond 64, and beyond 32 if the batch has 2^16 keys of all heads and requests
+// (taken for as long as this one).
+constexpr int kKvFew = 32;
+constexpr int64_t kKvManyKeys = 1 << 16;
+__device__ __forceinline__ bool kv_many(const KvAttn &a, const KvRequest &q) {
+    const int64_t vecs = (int64_t)q.rows * a.group, keys = q.length - row_first(a, max(row_pos(q, 0), 0));
+    return vecs > 2 * (int64_t)a.few || (vecs > a.few && (float)keys * (float)a.kv_heads * (float)a.requests >= (float)kKvManyKeys);
+}
 
 // Two f16 numbers of two codes that lie in the bytes of a 16-bit half each: int8 exactly, e4m3 times 2^-8 (its bits moved to their
 // place in an f16 number, subnormal ones included).

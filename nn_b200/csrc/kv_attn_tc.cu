@@ -53,7 +53,7 @@ __device__ __forceinline__ TcRequest tc_request(const KvAttn &a, int64_t r) {
     q.row0 = k.row0;
     q.rows = k.rows;
     q.length = k.length;
-    if (k.rows * a.group > a.few) q.cbs = (k.rows * a.group + kTcCols - 1) / kTcCols;
+    if (kv_many(a, k)) q.cbs = (k.rows * a.group + kTcCols - 1) / kTcCols;
     return q;
 }
 template <int KT>

@@ -395,6 +395,25 @@ def test_attention_of_prompts(fmt, group, dim, dtype, window):
     check_attend(c, table, lengths, start, q, b, window=window)
 
 
+@pytest.mark.parametrize("group,dim,rows", [(71, 64, 1), (128, 128, 1), (65, 192, 1), (33, 128, 2), (16, 64, 4), (13, 64, 5)])
+def test_attention_of_many_heads_to_one(group, dim, rows):
+    """Up to 64 query vectors of a request and key / value head, and more: single tokens of many heads among them."""
+    rng = np.random.default_rng(group)
+    lengths = [100, 7, 33]
+    c, table, start, q, b = serving(rng, 1, lengths, [rows, 1, rows], heads=group, kv=1, dim=dim, block=32, dtype=torch.bfloat16)
+    check_attend(c, table, lengths, start, q, b)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows,window", [(5, 0), (8, 0), (5, 2044)])
+def test_attention_of_a_few_rows_of_long_requests(rows, window, dtype):
+    """33 to 64 query vectors: requests of 2^16 keys (times heads and requests) and more take another kernel than shorter ones do."""
+    rng = np.random.default_rng(rows)
+    lengths = [2100, 2047, 2048, 5]
+    c, table, start, q, b = serving(rng, 1, lengths, [rows, rows, rows, 5], heads=64, kv=8, dim=64, block=64, dtype=dtype)
+    check_attend(c, table, lengths, start, q, b, window=window)
+
+
 @pytest.mark.parametrize("count,length", [(1, 6001), (3, 2500), (200, 40)])
 def test_attention_that_is_cut_into_parts(count, length):
     """Long requests in many parts, and many short ones in one."""
@@ -545,6 +564,38 @@ def test_attention_on_another_stream_and_in_two_graphs(rows):
                 g.replay()
         torch.cuda.synchronize()
         assert torch.equal(outs[0], want[0]) and torch.equal(outs[1], want[1])
+
+
+def test_a_step_captured_whole():
+    """Tables that advance, append and attention in one graph: twenty tokens of two requests against one call with all of them."""
+    rng = np.random.default_rng(21)
+    block, n = 16, 2
+    c = kv_cache.KvCache(12, 2, 64, block)
+    b = kv_cache.KvBatch(n, 6, n, block)
+    k, v, q = (torch.from_numpy(rng.standard_normal((20, n, h, 64)).astype(np.float32)).to(DEV) for h in (2, 2, 4))
+    now = [torch.zeros_like(x[0]) for x in (k, v, q)]
+    one, free = i32([1, 1]), i32(rng.permutation(12))
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=stream):
+            b.build(b.length, one, free, b.used)
+            c.append(now[0], now[1], b.slot)
+            y = c.attend(now[2], b)
+        outs = []
+        for t in range(20):
+            for dst, src in zip(now, (k, v, q)):
+                dst.copy_(src[t])
+            g.replay()
+            outs.append(y.clone())
+    torch.cuda.synchronize()
+    assert b.length.tolist() == [20, 20] and int(b.used) == 4
+    kk, vv = values_of(c)
+    want, mag, top = ref.attend(now[2].double().cpu().numpy(), kk, vv, b.table.cpu().numpy(), [20, 20], [0, 1, 2], block, 0.125, 0)
+    got = outs[-1].double().cpu().numpy()
+    assert (np.abs(got - want) <= bound(mag, want, top, 64, 20, torch.float32, np.abs(vv).max(), False)).all()
+    c.backend.device_status()
 
 
 def test_attention_refuses_wrong_tensors():
