@@ -772,7 +772,7 @@ NNQ_API nnq_status nnq_kv_append(nnq_ctx *ctx, const nnq_kv_cache *cache, const 
 /* The values of given slots, k and v [rows, kv_heads, dim] f32 or bf16 (exact in both); zeros for slot -1. */
 NNQ_API nnq_status nnq_kv_read(nnq_ctx *ctx, const nnq_kv_cache *cache, const int32_t *slot_dev, int64_t rows, void *k_dev, void *v_dev, nnq_dtype dt, void *stream);
 
-/* The batch as attention reads it: what nnq_kv_tables writes. max_rows: rows of the request with the most, as far as the
+/* The batch as attention reads it: what nnq_kv_tables writes (a table's blocks * block must stay below 2^31 - 1024). max_rows: rows of the request with the most, as far as the
  * host knows; it decides which kernels run and how much workspace they need, not what they compute. */
 typedef struct nnq_kv_batch {
     const int32_t *length, *row_start, *table;

@@ -614,7 +614,9 @@ static nnq_status check_batch(nnq_ctx *ctx, const nnq_kv_cache *c, const nnq_kv_
     if (!b) return fail(ctx, NNQ_ERR_INVALID_ARG, "batch is NULL");
     if (heads < 1 || heads % c->kv_heads) return fail(ctx, NNQ_ERR_SHAPE_MISMATCH, "%d query heads over %d key / value heads", heads, c->kv_heads);
     if (b->requests < 1 || b->rows < 0 || b->table_ld < 1 || b->max_rows < 1) return fail(ctx, NNQ_ERR_INVALID_ARG, "bad sizes of a batch");
-    if (b->requests > INT32_MAX / 2 || b->rows > INT32_MAX / heads || b->table_ld > INT32_MAX) return fail(ctx, NNQ_ERR_UNSUPPORTED, "a batch of %lld requests and %lld rows", (long long)b->requests, (long long)b->rows);
+    // (positions are counted in 32 bits, up to a tile beyond the last)
+    if (b->table_ld > (INT32_MAX - 1024) / c->block) return fail(ctx, NNQ_ERR_UNSUPPORTED, "tables of %lld blocks of %d tokens", (long long)b->table_ld, c->block);
+    if (b->requests > INT32_MAX / 2 || b->rows > INT32_MAX / heads) return fail(ctx, NNQ_ERR_UNSUPPORTED, "a batch of %lld requests and %lld rows", (long long)b->requests, (long long)b->rows);
     return NNQ_OK;
 }
 
@@ -657,7 +659,7 @@ nnq_status nnq_kv_attention(nnq_ctx *ctx, const nnq_kv_cache *c, const nnq_kv_ba
     // The batch's requests are dealt between the two kernels on the device (kv_many). The tensor-core kernel is not launched where the
     // rows, the table's width and the window leave it none; a prompt alone goes to it wholly.
     const bool prompt = b->max_rows > 2 * kKvFew / a.group;
-    int64_t keys = std::min<int64_t>(b->table_ld * c->block, INT32_MAX);
+    int64_t keys = b->table_ld * c->block;
     if (window > 0) keys = std::min(keys, window + std::min(b->max_rows, b->rows));
     if (tc_rows(a.dim, a.group, b->max_rows) && (prompt || keys * a.kv_heads >= (kKvManyKeys + b->requests - 1) / b->requests)) {
         a.few = prompt && b->requests == 1 ? 0 : kKvFew;

@@ -76,7 +76,7 @@ def test_reads_that_are_refused(lib, ctx, change, status):
     (dict(q_dt=3), {}, INVALID), (dict(y_dt=-1), {}, INVALID), (dict(heads=3), {}, SHAPE), (dict(heads=0), {}, SHAPE), (dict(scale=0.0), {}, RANGE),
     (dict(scale=-1.0), {}, RANGE), (dict(scale=float("nan")), {}, RANGE), (dict(scale=float("inf")), {}, RANGE), (dict(window=-1), {}, INVALID),
     (dict(q=None), {}, INVALID), (dict(y=None), {}, INVALID), (dict(q=P + 8), {}, INVALID), (dict(q_ld=511), {}, SHAPE), (dict(y_ld=513), {}, INVALID),
-    (dict(work=None), {}, INVALID), (dict(work=P + 4), {}, INVALID), (dict(), dict(requests=0), INVALID), (dict(), dict(table_ld=0), INVALID),
+    (dict(work=None), {}, INVALID), (dict(work=P + 4), {}, INVALID), (dict(), dict(requests=0), INVALID), (dict(), dict(table_ld=0), INVALID), (dict(), dict(table_ld=1 << 27), UNSUPPORTED),
     (dict(), dict(rows=-1), INVALID), (dict(), dict(max_rows=0), INVALID), (dict(), dict(rows=1 << 30), UNSUPPORTED), (dict(), dict(length=None), INVALID),
     (dict(), dict(row_start=None), INVALID), (dict(), dict(table=None), INVALID)])
 def test_attention_that_is_refused(lib, ctx, change, batch, status):
