@@ -59,7 +59,7 @@ __device__ __forceinline__ TcRequest tc_request(const KvAttn &a, int64_t r) {
 template <int KT>
 __device__ __forceinline__ void tc_range(const KvAttn &a, const TcRequest &q, int cb, int &first, int &steps) {
     const int base = q.length - q.rows, r0 = base + cb * kTcCols / a.group, r1 = base + (min((cb + 1) * kTcCols, q.rows * a.group) - 1) / a.group;
-    const int lo = a.window > 0 ? max(r0 - a.window + 1, 0) : 0;
+    const int lo = row_first(a, r0);
     first = r1 < 0 ? 0 : lo / KT;
     steps = r1 < 0 ? 1 : r1 / KT - first + 1;
 }
@@ -368,7 +368,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attn_tc_kernel(const KvAttn 
             group_sync(w);
             if (me == 0) mbar_arrive(qf + 8 * w);
             const int pos = it.length - it.rows + row;
-            const int low = a.window > 0 ? max(pos - a.window + 1, 0) : 0;
+            const int low = row_first(a, pos);
             const float fac = a.scale * kTcLog2E * Codes::unscale * kv_top_unscale(big);
             float m = 0.0f, mv = 0.0f, l = 0.0f, thr = -INFINITY, thv = -INFINITY;
             // the weights of the group's tile number `t` are in tensor memory

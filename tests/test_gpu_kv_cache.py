@@ -414,6 +414,17 @@ def test_attention_of_a_few_rows_of_long_requests(rows, window, dtype):
     check_attend(c, table, lengths, start, q, b, window=window)
 
 
+@pytest.mark.parametrize("window", [1, 2 ** 31 - 1])
+def test_attention_of_rows_before_the_first_position(window):
+    """A request of more rows than positions: the rows before position 0 see nothing, whatever the window is."""
+    rng = np.random.default_rng(3)
+    lengths = [90, 100]
+    c, table, start, q, b = serving(rng, 1, lengths, [90, 100], heads=8, kv=2, dim=64, block=32, dtype=torch.float32)
+    check_attend(c, table, lengths, start, q, b, window=window)
+    b.length[0] = 20
+    check_attend(c, table, [20, 100], start, q, b, window=window)
+
+
 @pytest.mark.parametrize("count,length", [(1, 6001), (3, 2500), (200, 40)])
 def test_attention_that_is_cut_into_parts(count, length):
     """Long requests in many parts, and many short ones in one."""
