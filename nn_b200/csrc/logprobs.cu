@@ -347,8 +347,10 @@ nnq_status nnq_token_logprobs(nnq_ctx *ctx, const void *logits_dev, nnq_dtype dt
     // shared memory: a float per thread and group of its vectors (vocabularies of many millions take more than there is)
     const int64_t groups = (slice / v + threads * kLpUnroll - 1) / (threads * kLpUnroll);
     const size_t smem = top > 0 ? (size_t)groups * threads * 4 : 0;
-    if (smem > 160 * 1024) return fail(ctx, NNQ_ERR_UNSUPPORTED, "alternatives among %lld tokens", (long long)vocab);
-    if (smem > 16 * 1024 && (s = check_cuda(ctx, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem), "shared memory")) != NNQ_OK) return s;
+    constexpr size_t most_smem = 160 * 1024;
+    static std::atomic<uint64_t> allowed[4];   // (one size for all calls: others of other threads may lie between asking and launching)
+    if (smem > most_smem) return fail(ctx, NNQ_ERR_UNSUPPORTED, "alternatives among %lld tokens", (long long)vocab);
+    if (smem > 16 * 1024 && (s = allow_smem(ctx, kernel, most_smem, allowed[(dt == NNQ_F32) * 2 + (threads == 256)])) != NNQ_OK) return s;
     const int64_t most = 65535;   // rows of a launch
     for (int64_t r0 = 0; r0 < rows; r0 += most) {
         LogprobArgs a = {(const uint8_t *)logits_dev + r0 * ld * (dt == NNQ_F32 ? 4 : 2), token_dev ? token_dev + r0 : nullptr, logprob_dev ? logprob_dev + r0 : nullptr,

@@ -145,3 +145,33 @@ def test_wrong_tensors_are_refused():
         with pytest.raises(api.TensorError):
             token_logprobs(*args)
     assert token_logprobs(x[:0], t[:0], 2).top_tokens.shape == (0, 2)
+
+
+def test_two_threads_with_other_vocabularies():
+    """Two contexts in two threads, one with a large vocabulary, the other with a small one, call after call."""
+    import threading
+
+    x = {v: torch.randn(1, v, device=DEV) for v in (151936, 60000)}
+    t = torch.zeros(1, dtype=torch.int32, device=DEV)
+    want = {v: token_logprobs(x[v], t, 5) for v in x}
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(v):
+        b = api.Backend()
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(300):
+                    r = token_logprobs(x[v], t, 5, b)
+                torch.cuda.current_stream().synchronize()
+            if not (torch.equal(r.logprob, want[v].logprob) and torch.equal(r.top_tokens, want[v].top_tokens)):
+                wrong.append(v)
+        except Exception as e:   # noqa: BLE001
+            wrong.append(e)
+
+    threads = [threading.Thread(target=work, args=(v,)) for v in x]
+    for th in threads:
+        th.start()
+    for th in threads:
+        th.join()
+    assert not wrong
