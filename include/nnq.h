@@ -801,8 +801,8 @@ NNQ_API nnq_status nnq_token_logprobs(nnq_ctx *ctx, const void *logits_dev, nnq_
                                       float *logprob_dev, float *entropy_dev, int32_t *top_token_dev, float *top_logprob_dev, void *stream);
 
 /* A Qwen3 decoder (nnq_decoder_create) with its keys and values in 8 bits, in blocks of `block` tokens (see nnq_kv_cache): a quarter of the
- * memory of the f32 cache, which is given back. Before the first token. A step appends and attends through the calls above, so it is not
- * fused with its products. With this cache nnq_decoder_buffers gives NULL for the f32 ones; nnq_decoder_cache gives a layer's,
+ * memory of the f32 cache, which is given back. Before the first token. A step appends and attends through the calls above, which takes
+ * four launches a layer in place of one. With this cache nnq_decoder_buffers gives NULL for the f32 ones; nnq_decoder_cache gives a layer's,
  * whose position p is slot p. */
 NNQ_API nnq_status nnq_decoder_set_cache(nnq_decoder *d, int format, int block);
 NNQ_API nnq_status nnq_decoder_cache(nnq_decoder *d, int layer, nnq_kv_cache *out);

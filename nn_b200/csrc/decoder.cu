@@ -1707,10 +1707,11 @@ static nnq_status rows_blocks(nnq_decoder *d, int n, int pos0, cudaStream_t st) 
 }
 
 // One GPU, bf16 activations and the Q4_K kernels for the products: norms, rotation, activation and residual sums are parts of the
-// kernels around them (five launches a layer instead of nine).
+// kernels around them (five launches a layer instead of nine; with an 8-bit cache, which has rotation, append, attention and its joining
+// as launches of their own, eight instead of eleven: a token of the Qwen3-8B shape behind 2048 others 2764 -> 2375 us).
 static bool step_is_fused(const nnq_decoder *d) {
     const nnq_decoder_config &c = d->cfg;
-    if (d->blocks || d->kv8 || d->comm || c.tp_world > 1 || d->act_dt != NNQ_BF16 || d->ctx->path != NNQ_PATH_AUTO || c.head_dim != 128) return false;
+    if (d->blocks || d->comm || c.tp_world > 1 || d->act_dt != NNQ_BF16 || d->ctx->path != NNQ_PATH_AUTO || c.head_dim != 128) return false;
     for (int l = 0; l < c.n_layers; l++) {
         const nnq_decoder::Layer &L = d->layers[l];
         for (const nnq_weight *w : {L.q, L.k, L.v, L.gate, L.up})

@@ -117,8 +117,8 @@ class Decoder:
 
     def set_cache(self, fmt: int, block: int = 32):
         """Keys and values in 8 bits (kv_cache.INT8 or E4M3), a scale for each `block` tokens and head, in place of f32: a quarter of the
-        memory, and steps behind long contexts read a quarter of the bytes; steps behind short ones take longer, as they are no
-        longer fused. Before the first token; Qwen3 decoders."""
+        memory, and steps behind long contexts read a quarter of the bytes; steps behind short ones take longer, as attention is
+        four launches (Qwen3-8B shape, a token behind 2048 / 32768 others: f32 1.89 / 3.34 ms, int8 2.38 / 2.92 ms). Before the first token; Qwen3 decoders."""
         self.backend.check(self.backend._lib.nnq_decoder_set_cache(self._handle, int(fmt), int(block)))
 
     def cache(self, layer: int):

@@ -9,6 +9,7 @@ from nn_b200 import api, decoder, kv_cache
 from nn_b200.formats import QuantFormat as Q
 from oracle import qwen3_ref as ref
 from tests import kv_reference as kvref
+from tests import test_gpu_fused_step as fused
 
 pytestmark = pytest.mark.gpu
 HIDDEN, FFN, VOCAB, EPS = 128, 192, 160, 1e-6
@@ -125,6 +126,40 @@ def test_generation_replayed_from_a_graph_and_again(act_dtype):
         dec.backend.device_status()
         dec.release()
     assert out[0] == out[1]
+
+
+@pytest.mark.parametrize("fmt", [kv_cache.INT8, kv_cache.E4M3])
+@pytest.mark.parametrize("heads,kv", [(2, 2), (16, 8), (16, 2)])
+def test_fused_steps_over_an_8_bit_cache(fmt, heads, kv):
+    """A bf16 decoder of Q4_K weights, whose step keeps norms, activation and residual sums in the products' kernels, against the step
+    with kernels of their own: 1e-2 in the 2-norm as with an f32 cache. A difference d of a new key or value may also turn its code by a
+    step s, which adds d s to its mean square: d = 2^-9 and s = 2^-6 of the largest value, elements of a third of it, sqrt(d s) * 3 =
+    1.7e-2 where the new token is all there is, 1.7e-2 / sqrt(16) behind 15 others."""
+    dec, b = fused._model(heads, kv, 2, 600), api.gpu_backend()
+    dec.set_cache(fmt, 32)
+    logits, caches = dec.buffers()[2], [dec.cache(i) for i in range(2)]
+    g = torch.Generator(device="cuda").manual_seed(5)
+    past = [[torch.randint(0, 120, t.shape, device="cuda", generator=g, dtype=torch.uint8) if t.dim() == 4 else torch.full_like(t, 121) for t in c] for c in caches]
+    for at in (0, 1, 15, 32, 599):
+        got = []
+        for path in (api.PATH_AUTO, api.PATH_SKINNY):
+            for c, old in zip(caches, past):
+                for t, o in zip(c, old):
+                    t.copy_(o)
+            b.set_path(path)
+            try:
+                dec.reset(7, at)
+                before = b.launch_count()
+                dec.step()
+                launches = b.launch_count() - before
+            finally:
+                b.set_path(api.PATH_AUTO)
+            torch.cuda.synchronize()
+            b.device_status()
+            got.append((launches, logits[:].clone()))
+        assert got[0][0] < got[1][0]   # (the fused step is what ran)
+        assert float((got[0][1] - got[1][1]).norm() / got[1][1].norm()) < 1e-2 + 1.7e-2 / (at + 1) ** 0.5, at
+    dec.release()
 
 
 def test_the_end_of_the_context_with_an_8_bit_cache():
