@@ -4,8 +4,8 @@
 //   y = sum_j p_j v_j / sum_j p_j,  p_j = exp(scale q . k_j - m),  over the positions that a row sees.
 //
 // What bounds it is the reading of the cache, 2 dim bytes per key and head once for all query heads of the group. The codes go from
-// global memory by cp.async into a ring of a warp's own, two steps of 16 keys ahead of the one that is worked on (128 KB under way on an
-// SM), and from there as bytes into the operand registers of mma.sync (m16n8k16, f16):
+// global memory by cp.async into a ring of a warp's own, one step of 16 keys ahead of the one that is worked on (64 KB under way on an
+// SM; two ahead, with the records in the ring: 2 requests of 130001 positions 111.0 us, one ahead 106.8), and from there as bytes into the operand registers of mma.sync (m16n8k16, f16):
 //   scores   S^T [16 keys x 8 vectors] = K [16 x dim] Q^T: lane (g, t) of a warp reads 16 bytes of keys g and g + 8 at a time; which
 //            dimension stands at which place of k is free as long as the queries agree.
 //   values   O^T [dim x 8 vectors] += V^T [dim x 16 keys] P^T: lane (g, t) reads 8 neighbouring bytes of the four keys whose
@@ -24,6 +24,9 @@
 // CTA, whatever the requests' lengths are. An item counts kKvPad steps more than it has, about what beginning and ending one takes, so
 // that many short requests in one part weigh what they cost. An item inside one part is written directly; of an item that is cut every part
 // leaves a record (m, mv, l, O), and kv_join_kernel joins them in their order.
+// Measured (heads of 128, with the joining): 2 requests of 130001 positions, int8, 8 key / value heads of 5 f32 query heads, 115 us (4.6 TB/s of
+// codes); 40 requests of up to 12000, e4m3, 8 heads of 4 bf16 query heads, 90 us (4.0 TB/s); one of 2001 positions 12.5 us, of which the
+// two launches, the first loads behind the table and the joining are nearly all.
 #include <algorithm>
 
 #include "kv_attn.cuh"
@@ -32,8 +35,8 @@
 namespace nnq {
 
 constexpr int kKvWarps = 8, kKvCols = 8, kKvStep = 16, kKvStages = 2;
-constexpr int kKvMinSteps = kKvWarps;   // of a CTA's part
-constexpr int kKvPad = 32;
+constexpr int kKvMinSteps = kKvWarps;   // of a CTA's part (one request of 2001 positions: 1 / 8 steps 14.3 / 12.5 us)
+constexpr int kKvPad = 32;              // (us with 8 / 16 / 32 / 64: 40 ragged requests 107.7 / 90.7 / 85.3 / 97.4; 2 long ones 116.0 / 111.3 with 32 / 64)
 constexpr int kKvFlush = 16;
 constexpr int kNothing = INT32_MIN;   // in place of a block: no key of the step is seen
 constexpr float kKvLog2E = 1.4426950408889634f;

@@ -12,9 +12,13 @@
 //   warps 16, 17:   (two more complete their group) a lane of each issues the MMAs of one softmax group: S(t + 1), then O += P(t) V(t). They
 //                   run in the order they are issued, so S(t + 1) may overwrite the weights of t - 1, whose product stands in front
 //                   of it. (One warp for both groups took 100 clocks an MMA beside the scheduler's other warps and set the pace.)
-// What bounds it is the softmax: of the exponentials a thread forms, the special function unit takes 16 a clock and SM. Codes are exact in f16. T = 1 (bf16 queries and outputs): a query vector is
-// exact under its power of two, a weight is one f16 number, off by up to 2^-11 of itself where the output's own rounding is 2^-8 of it. T = 2 (f32
-// on either side): both have two terms, 22 bits.
+// What bounds it is the softmax: some 6100 instructions of a scheduler's warps per tile of both groups, the exponentials among them (the
+// special function unit takes 16 a clock and SM), and the hand-over between softmax and MMA. Measured: 2000 rows behind 2100, e4m3, 8 key /
+// value heads of 4 bf16 query heads of 128, 189 us with the joining, 537 TFLOP/s of the 102 GFLOP that a causal prompt takes; counters of an
+// earlier form of 182 us: tensor pipe 30 % active, logic and FMA pipes 38 %, special functions 32 %. Slower were 128 keys a tile with both
+// MMA warps on each (217 us) and four converter warps in favour of more registers for the softmax (186 beside 182).
+// Codes are exact in f16. T = 1 (bf16 queries and outputs): a query vector is exact under its power of two, a weight is one f16 number, off
+// by up to 2^-11 of itself where the output's own rounding is 2^-8 of it. T = 2 (f32 on either side): both have two terms, 22 bits.
 // Scales: a block's key exponent multiplies its scores in f32. Its value exponent enters the weight, w = p 2^(m - mv + e_v) with a
 // reference mv of its own, the largest score + e_v as m is that of the scores: one factor per vector and 16 keys, and weights
 // between 0 and 2^8 whatever the scales are.
@@ -598,69 +602,69 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attn_tc_kernel(const KvAttn 
     } else {
         tc_registers<48>();
         if (warp < 18) {
-        // ---------------- MMA issuers (a warp waits together, one lane issues) ----------------
-        const int w = warp - 16;
-        const uint32_t id_s = (1u << 4) | ((uint32_t)(KT >> 3) << 17) | ((128u >> 4) << 24);                 // both operands f16
-        const uint32_t id_o = (1u << 4) | (1u << 16) | ((uint32_t)(D >> 3) << 17) | ((128u >> 4) << 24);     // B is MN-major
-        const uint32_t qa = smem_u32(smem + w * T * ATOMS * Sh::q_atom), o_t = tmem + 256 * w;
-        int nw = 0, items = 0;
-        TcJoin join = {-1, 0, 0, 0, 0, {0, 0, 0}};
-        auto wait = [&](uint32_t bar, int count) {
-            ok = ok && __all_sync(0xFFFFFFFFu, mbar_wait_fast(bar, count & 1));
-            return ok;
-        };
-        while (ok && walk.next(it)) {
-            const int steps = it.s1 - it.s0;
-            if (it.s0 > 0 && it.s1 == it.steps) join = {(int)((plan.begin - it.s0) / plan.chunk), it.vecs, it.row0 + it.vec0 / a.group, it.head * a.group, it.vec0 % a.group, {0, 0, 0}};
-            if (w * 128 >= it.vecs) {   // nothing for the second group: its word for the stages alone
-                for (int s = 0; s < steps && ok; s++, n++)
-                    if (wait(full + 8 * (n % STAGES), n / STAGES) && lane == 0) mbar_arrive(empty + 8 * (n % STAGES));
-                continue;
-            }
-            wait(qf + 8 * w, items++);
-            for (int s = -1; s < steps && ok; s++) {
-                if (s + 1 < steps) {   // the next tile's scores
-                    const int st = (n + s + 1) % STAGES, place = (nw + 1 + s) & 1;
-                    if (!wait(full + 8 * st, (n + s + 1) / STAGES)) break;
+            // ---------------- MMA issuers (a warp waits together, one lane issues) ----------------
+            const int w = warp - 16;
+            const uint32_t id_s = (1u << 4) | ((uint32_t)(KT >> 3) << 17) | ((128u >> 4) << 24);                 // both operands f16
+            const uint32_t id_o = (1u << 4) | (1u << 16) | ((uint32_t)(D >> 3) << 17) | ((128u >> 4) << 24);     // B is MN-major
+            const uint32_t qa = smem_u32(smem + w * T * ATOMS * Sh::q_atom), o_t = tmem + 256 * w;
+            int nw = 0, items = 0;
+            TcJoin join = {-1, 0, 0, 0, 0, {0, 0, 0}};
+            auto wait = [&](uint32_t bar, int count) {
+                ok = ok && __all_sync(0xFFFFFFFFu, mbar_wait_fast(bar, count & 1));
+                return ok;
+            };
+            while (ok && walk.next(it)) {
+                const int steps = it.s1 - it.s0;
+                if (it.s0 > 0 && it.s1 == it.steps) join = {(int)((plan.begin - it.s0) / plan.chunk), it.vecs, it.row0 + it.vec0 / a.group, it.head * a.group, it.vec0 % a.group, {0, 0, 0}};
+                if (w * 128 >= it.vecs) {   // nothing for the second group: its word for the stages alone
+                    for (int s = 0; s < steps && ok; s++, n++)
+                        if (wait(full + 8 * (n % STAGES), n / STAGES) && lane == 0) mbar_arrive(empty + 8 * (n % STAGES));
+                    continue;
+                }
+                wait(qf + 8 * w, items++);
+                for (int s = -1; s < steps && ok; s++) {
+                    if (s + 1 < steps) {   // the next tile's scores
+                        const int st = (n + s + 1) % STAGES, place = (nw + 1 + s) & 1;
+                        if (!wait(full + 8 * st, (n + s + 1) / STAGES)) break;
+                        tc_fence_after();
+                        if (elect_one()) {
+                            const uint32_t ka = smem_u32(stages + st * Sh::stage);
+    #pragma unroll
+                            for (int x = T - 1; x >= 0; x--)   // the small products first, so that their sums are rounded at their size
+    #pragma unroll
+                                for (int i = 0; i < ATOMS; i++) {
+                                    const uint64_t dq = smem_desc(qa + (x * ATOMS + i) * Sh::q_atom), dk = smem_desc(ka + i * Sh::k_atom);
+    #pragma unroll
+                                    for (int k = 0; k < 4; k++) umma_bf16(o_t + 128 + 64 * place, dq + 2 * k, dk + 2 * k, id_s, x < T - 1 || (i | k) != 0);
+                                }
+                            umma_commit(sf + 8 * (2 * w + place));
+                        }
+                        __syncwarp();
+                    }
+                    if (s < 0) continue;
+                    const int st = (n + s) % STAGES, place = (nw + s) & 1;
+                    if (!wait(pf + 8 * (2 * w + place), (nw + s) >> 1)) break;
                     tc_fence_after();
                     if (elect_one()) {
-                        const uint32_t ka = smem_u32(stages + st * Sh::stage);
-#pragma unroll
-                        for (int x = T - 1; x >= 0; x--)   // the small products first, so that their sums are rounded at their size
-#pragma unroll
-                            for (int i = 0; i < ATOMS; i++) {
-                                const uint64_t dq = smem_desc(qa + (x * ATOMS + i) * Sh::q_atom), dk = smem_desc(ka + i * Sh::k_atom);
-#pragma unroll
-                                for (int k = 0; k < 4; k++) umma_bf16(o_t + 128 + 64 * place, dq + 2 * k, dk + 2 * k, id_s, x < T - 1 || (i | k) != 0);
-                            }
-                        umma_commit(sf + 8 * (2 * w + place));
+                        const uint32_t va = smem_u32(stages + st * Sh::stage) + ATOMS * Sh::k_atom, pa = o_t + 128 + 64 * place;
+                        const uint64_t dv = tc_desc_mn(va, Sh::k_atom);
+    #pragma unroll
+                        for (int x = T - 1; x >= 0; x--)
+    #pragma unroll
+                            for (int k = 0; k < KT / 16; k++) umma_ts(o_t, pa + 32 * x + 8 * k, dv + (2048 >> 4) * k, id_o, s > 0 || x < T - 1 || k != 0);
+                        umma_commit(of + 8 * (2 * w + place));
+                        umma_commit(empty + 8 * st);
                     }
                     __syncwarp();
                 }
-                if (s < 0) continue;
-                const int st = (n + s) % STAGES, place = (nw + s) & 1;
-                if (!wait(pf + 8 * (2 * w + place), (nw + s) >> 1)) break;
-                tc_fence_after();
-                if (elect_one()) {
-                    const uint32_t va = smem_u32(stages + st * Sh::stage) + ATOMS * Sh::k_atom, pa = o_t + 128 + 64 * place;
-                    const uint64_t dv = tc_desc_mn(va, Sh::k_atom);
-#pragma unroll
-                    for (int x = T - 1; x >= 0; x--)
-#pragma unroll
-                        for (int k = 0; k < KT / 16; k++) umma_ts(o_t, pa + 32 * x + 8 * k, dv + (2048 >> 4) * k, id_o, s > 0 || x < T - 1 || k != 0);
-                    umma_commit(of + 8 * (2 * w + place));
-                    umma_commit(empty + 8 * st);
-                }
-                __syncwarp();
+                n += steps;
+                nw += steps;
             }
-            n += steps;
-            nw += steps;
-        }
-        if (w == 0 && lane == 0) joins[blockIdx.x] = join;
-        // MMAs that were issued may still read shared memory and write tensor memory
-        if (elect_one()) umma_commit(drain + 8 * w);
-        __syncwarp();
-        ok = __all_sync(0xFFFFFFFFu, mbar_wait(drain + 8 * w, 0)) && ok;
+            if (w == 0 && lane == 0) joins[blockIdx.x] = join;
+            // MMAs that were issued may still read shared memory and write tensor memory
+            if (elect_one()) umma_commit(drain + 8 * w);
+            __syncwarp();
+            ok = __all_sync(0xFFFFFFFFu, mbar_wait(drain + 8 * w, 0)) && ok;
         }
     }
     if (!ok && lane == 0) atomicExch(a.status, 1);

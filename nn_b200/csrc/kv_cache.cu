@@ -13,7 +13,8 @@ namespace nnq {
 // One launch of one cluster: every CTA sums the counts of all requests, in portions of kTabChunk that lie in shared memory, and writes
 // its share of the tables: entry i of the portion's new blocks, row i of its rows, found by bisection of the sums. The cluster meets
 // between the reading of a portion and the writing, so lengths may be written where the old ones lie. What bounds it is latency:
-// the requests' loads, the sums, the bisection, one dependent load for a block that was there before.
+// the requests' loads, the sums, the bisection, one dependent load for a block that was there before. Measured: 8 single tokens 2.4 us,
+// 300 requests with some 32000 rows 10.2 us.
 constexpr int kTabChunk = 2048;
 
 struct TableArgs {
@@ -136,7 +137,7 @@ __global__ void __launch_bounds__(1024) kv_tables_kernel(const TableArgs a) {
 // left out), the exponent byte, the codes; codes the block held before are rounded again where the exponent grew. The first pieces of
 // eight values of a lane stay in registers in between.
 // What bounds it is latency: the chain slot -> values -> codes, which a warp goes through alone (a CTA per run, with a barrier in it:
-// 12000 rows of 8 heads of 128, bf16, 43 us).
+// 12000 rows of 8 heads of 128, bf16, 43 us). Measured: those 32 us, 48 single f32 rows with the read behind them 4.4 us.
 constexpr int kAppWarps = 8;
 
 struct AppendArgs {
@@ -328,7 +329,8 @@ struct ReadArgs {
     int *status;
 };
 
-// A thread has 16 values of a row: one load, two or four stores. Rows of no slot are zeros.
+// A thread has 16 values of a row: one load, two or four stores. Rows of no slot are zeros. Bound by the stores: 12000 rows of 8 heads of
+// 128 to bf16 16.6 us (4.4 TB/s both ways).
 template <int FMT, bool F32>
 __global__ void __launch_bounds__(256) kv_read_kernel(const ReadArgs a) {
     pdl_prologue();
@@ -383,6 +385,8 @@ nnq_status nnq_kv_tables(nnq_ctx *ctx, const int32_t *past_dev, const int32_t *c
     nnq_status s = check_cuda(ctx, cudaSetDevice(ctx->device), "cudaSetDevice");
     if (s != NNQ_OK) return s;
     const TableArgs a = {past_dev, count_dev, free_dev, skip_dev, table_dev, length_dev, row_start_dev, slot_dev, position_dev, used_dev, requests, n_free, table_ld, rows, log2_of(block)};
+    // one CTA of 256 threads for what it does in a pass or four, else a cluster of up to 8 CTAs of 1024, one for 2048 rows (us, small / large:
+    // 8 requests of a row 2.4 / 4.9, 300 requests of some 32000 rows 84 / 10.2)
     const bool small = requests <= 256 && rows <= 1024;
     cudaLaunchConfig_t cfg = {};
     cfg.blockDim = dim3(small ? 256 : 1024);
@@ -414,7 +418,8 @@ nnq_status nnq_kv_append(nnq_ctx *ctx, const nnq_kv_cache *c, const void *k_dev,
     if (!rows_aligned(k_dev, k_ld, dt) || !rows_aligned(v_dev, v_ld, dt)) return fail(ctx, NNQ_ERR_INVALID_ARG, "rows of keys and values must start at multiples of 16 bytes");
     if ((s = check_cuda(ctx, cudaSetDevice(ctx->device), "cudaSetDevice")) != NNQ_OK) return s;
     const AppendArgs a = {{k_dev, k_ld, (uint8_t *)c->k, c->k_exp}, {v_dev, v_ld, (uint8_t *)c->v, c->v_exp}, slot_dev, rows, c->blocks * c->block, c->kv_heads, c->dim,
-                          log2_of(c->block), rows > 1024 ? 16 : 1, ctx->d_status};   // (few rows are single tokens more often than not: a warp each)
+                          log2_of(c->block), rows > 1024 ? 16 : 1, ctx->d_status};   // (few rows are single tokens more often than not: a warp each.
+                          // us with the read behind, 1 / 16 rows: 48 single tokens 4.4 / 17.6, three prompts of some 4000 rows 79 / 48; 4 / 8 rows 54 / 50)
     const int64_t warps = (rows + a.tile - 1) / a.tile * 2 * c->kv_heads;
     if (warps / kAppWarps >= INT32_MAX) return fail(ctx, NNQ_ERR_UNSUPPORTED, "%lld rows of %d heads", (long long)rows, c->kv_heads);
     const dim3 grid((unsigned)((warps + kAppWarps - 1) / kAppWarps)), block(kAppWarps * 32);

@@ -12,7 +12,8 @@
 // meets more equal values than there is room for, or a NaN, the largest element below the one before is looked for `top` times. Order:
 // larger value first, then the lower index.
 // What bounds it: bf16 rows 12 elements per clock and SM at the copy rate, where the special function unit forms 16 exponentials;
-// single rows the way through the cluster.
+// single rows the way through the cluster. Measured: 2000 bf16 rows of 128259 with one alternative 123 us (4.2 TB/s), 129 f32 rows of
+// 151936 with 20 of them from memory 25 us (3.1 TB/s), one row 11 us.
 // The reference turns logits into probabilities on the host (crates/nn-core/src/layers/generation/autoregressive_sampling.rs:14-21 and
 // the samplers beside it).
 #include <algorithm>
@@ -336,11 +337,13 @@ nnq_status nnq_token_logprobs(nnq_ctx *ctx, const void *logits_dev, nnq_dtype dt
     if ((uintptr_t)logits_dev % (dt == NNQ_F32 ? 4 : 2)) return fail(ctx, NNQ_ERR_INVALID_ARG, "misaligned logits");
     nnq_status s = check_cuda(ctx, cudaSetDevice(ctx->device), "cudaSetDevice");
     if (s != NNQ_OK) return s;
-    // CTAs of a row: as many as give every SM one, but no slices below 4096 elements
+    // CTAs of a row: as many as there are SMs for, but no slices below 4096 elements. us with as many / up to twice as many, rows from
+    // memory: 30 bf16 rows of 151936 13.2 / 16.1, 140 bf16 rows of 32000 9.9 / 12.5, 19 f32 rows of 151936 13.9 / 15.9, but 80 of them 23.7 / 22.0;
+    // rows in the L2 cache: 129 f32 rows 18.8 / 23.2. One row of 151936 by one CTA 15.8, by eight 10.9.
     int ctas = 1;
-    while (ctas < 8 && rows * ctas < ctx->sm_count && vocab / (2 * ctas) >= 4096) ctas *= 2;
+    while (ctas < 8 && rows * 2 * ctas <= ctx->sm_count && vocab / (2 * ctas) >= 4096) ctas *= 2;
     // threads: four CTAs of 256 on an SM are in different phases of their rows where there are many; a row's few parts are read faster by
-    // 512 (us, 256 / 512: 2000 bf16 rows of 128259 128 / 145, 129 f32 rows of 151936 26.7 / 22.7)
+    // 512 (us, 256 / 512: 2000 bf16 rows of 128259 123 / 145, 129 f32 rows of 151936 26.7 / 22.7 with two CTAs a row)
     const int threads = rows >= 2 * ctx->sm_count ? 256 : 512;
     auto kernel = dt == NNQ_F32 ? (threads == 256 ? logprobs_kernel<true, 256> : logprobs_kernel<true, 512>) : (threads == 256 ? logprobs_kernel<false, 256> : logprobs_kernel<false, 512>);
     const int slice = (int)(((vocab + ctas - 1) / ctas + 7) / 8 * 8), v = dt == NNQ_F32 ? 4 : 8;
