@@ -772,8 +772,8 @@ NNQ_API nnq_status nnq_kv_append(nnq_ctx *ctx, const nnq_kv_cache *cache, const 
 /* The values of given slots, k and v [rows, kv_heads, dim] f32 or bf16 (exact in both); zeros for slot -1. */
 NNQ_API nnq_status nnq_kv_read(nnq_ctx *ctx, const nnq_kv_cache *cache, const int32_t *slot_dev, int64_t rows, void *k_dev, void *v_dev, nnq_dtype dt, void *stream);
 
-/* The batch as attention reads it: what nnq_kv_tables writes (a table's blocks * block must stay below 2^31 - 1024). max_rows: rows of the request with the most, as far as the
- * host knows; it decides which kernels run and how much workspace they need, not what they compute. */
+/* The batch as attention reads it: what nnq_kv_tables writes (table_ld * block must stay below 2^31 - 1024). max_rows: rows of
+ * the request with the most, as far as the host knows; it decides which kernels run and how much workspace they need, not what they compute. */
 typedef struct nnq_kv_batch {
     const int32_t *length, *row_start, *table;
     int64_t requests, table_ld, rows, max_rows;
@@ -781,8 +781,8 @@ typedef struct nnq_kv_batch {
 
 /* Softmax attention over the cache: row i of request r stands at position length[r] - (rows of r) + i and sees the positions up to
  * its own, with window > 0 the last `window` of them; query head h reads key / value head h / (heads / kv_heads).
- * q [rows, heads, dim] and y in the same layout, f32 or bf16, rows q_ld / y_ld elements apart, 16-byte aligned. A row that sees
- * nothing is zero; rows behind the last request are left as they were. Scores, softmax and sums are f32, codes exact, queries
+ * q [rows, heads, dim] and y in the same layout, f32 or bf16, rows q_ld / y_ld elements apart, 16-byte aligned, apart from each
+ * other. A row that sees nothing is zero; rows behind the last request are left as they were. Scores, softmax and sums are f32, codes exact, queries
  * and weights enter the products with 22 bits (bf16 queries exactly; with bf16 queries and outputs the weights of requests of more than
  * 32 query vectors per key / value head, dim 64 and 128, are rounded to 11 bits). A block number outside the cache is not read: its positions
  * count as unseen, and nnq_device_status reports NNQ_ERR_INVALID_ARG. The workspace (nnq_kv_attention_workspace; 16-byte

@@ -46,8 +46,8 @@ __device__ __forceinline__ int row_first(const KvAttn &a, int pos) { return a.wi
 //   2 x 30000     119 / 110      161 / 111      224 / 112      306 / 115
 //   16 x 4000     142 / 117      191 / 118      267 / 122      362 / 124
 //   16 x 30000    929 / 638     1233 / 619     1949 / 626     2715 / 635
-// and up to 32 vectors the first wins everywhere. So: beyond 64, and beyond 32 if the batch has 2^16 keys of all heads and requests
-// (taken for as long as this one).
+// 32 vectors: 2 x 30000 98 / 108, 16 x 4000 117 / 115, 16 x 30000 702 / 605, with f32 queries 111 / 153, 131 / 164, 820 / 959. So: beyond
+// 64, and beyond 32 if the batch has 2^16 keys of all heads and requests (taken for as long as this one).
 constexpr int kKvFew = 32;
 constexpr int64_t kKvManyKeys = 1 << 16;
 __device__ __forceinline__ bool kv_many(const KvAttn &a, const KvRequest &q) {
