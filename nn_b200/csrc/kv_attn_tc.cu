@@ -21,7 +21,7 @@
 // by up to 2^-11 of itself where the output's own rounding is 2^-8 of it. T = 2 (f32 on either side): both have two terms, 22 bits.
 // The sums in tensor memory run through all tiles of a part, and the tensor core cuts off what they cannot hold: outputs lean towards zero
 // by some 2^-26 for every 16 keys and term (f32, heads of 64: 3054 keys, error against 64 bits 5.0e-6; shorter chains would need a second
-// place for the sums, which heads of 128 leave no columns for). With bf16 outputs that is below their rounding up to millions of keys.
+// place for the sums, which heads of 128 leave no columns for). With bf16 outputs that is below their rounding up to a million keys.
 // Scales: a block's key exponent multiplies its scores in f32. Its value exponent enters the weight, w = p 2^(m - mv + e_v) with a
 // reference mv of its own, the largest score + e_v as m is that of the scores: one factor per vector and 16 keys, and weights
 // between 0 and 2^8 whatever the scales are.
