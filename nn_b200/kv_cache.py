@@ -69,7 +69,7 @@ class KvBatch:
         self.table, self.length = _int32(table, "table", table.shape, b.device), _int32(length, "length", (n,), b.device)
         self.row_start = _int32(row_start, "row_start", (n + 1,), b.device)
         self.slot = None if slot is None else _int32(slot, "slot", (slot.numel(),), b.device)
-        self.position = None if position is None else _int32(position, "position", (position.numel(),), b.device)
+        self.position = None if position is None else _int32(position, "position", (position.numel() if slot is None else slot.numel(),), b.device)
         self.rows = 0 if slot is None else slot.numel()
         self.used = torch.zeros(1, dtype=torch.int32, device=self.device)
         return self

@@ -2,11 +2,13 @@
 call, so a context of zeros is enough to reach it. And the 64-bit reference of the GPU tests against itself."""
 import ctypes
 
+from types import SimpleNamespace
+
 import numpy as np
 import pytest
 
-from nn_b200 import _lib
-from nn_b200.kv_cache import _Batch, _Cache
+from nn_b200 import _lib, api
+from nn_b200.kv_cache import KvBatch, _Batch, _Cache
 from tests import kv_reference as ref
 
 P = 1 << 20   # a pointer that nothing follows: aligned, not NULL
@@ -125,3 +127,30 @@ def test_the_reference_keeps_every_code(fmt):
     for amax in (127.0, 127.5, 448.0, 448.5, 1.0, 3e-20, 2e38):
         e = ref.least_exponent(fmt, amax)
         assert amax <= ref.TOP[fmt] * 2.0 ** (e - 127) and (e == 7 or amax > ref.TOP[fmt] * 2.0 ** (e - 128))
+
+
+class DeviceInts:
+    """What a batch asks of an int32 tensor on the device, without one."""
+
+    def __init__(self, *shape):
+        torch = pytest.importorskip("torch")
+        self.shape, self.dtype, self.is_cuda, self.device = torch.Size(shape), torch.int32, True, "cuda:0"
+
+    def dim(self):
+        return len(self.shape)
+
+    def numel(self):
+        return int(np.prod(self.shape))
+
+    def get_device(self):
+        return 0
+
+    def is_contiguous(self):
+        return True
+
+
+@pytest.mark.parametrize("slots,positions", [(10, 5), (10, 0), (3, 4)])
+def test_a_batch_has_a_position_for_every_slot(slots, positions):
+    """`build` writes both for as many rows as there are slots."""
+    with pytest.raises(api.ShapeMismatch):
+        KvBatch.from_tensors(DeviceInts(2, 4), DeviceInts(2), DeviceInts(3), 16, slot=DeviceInts(slots), position=DeviceInts(positions), backend=SimpleNamespace(device=0))
