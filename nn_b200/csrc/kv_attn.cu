@@ -619,7 +619,8 @@ static nnq_status check_batch(nnq_ctx *ctx, const nnq_kv_cache *c, const nnq_kv_
     if (b->requests < 1 || b->rows < 0 || b->table_ld < 1 || b->max_rows < 1) return fail(ctx, NNQ_ERR_INVALID_ARG, "bad sizes of a batch");
     // (positions are counted in 32 bits, up to a tile beyond the last)
     if (b->table_ld > (INT32_MAX - 1024) / c->block) return fail(ctx, NNQ_ERR_UNSUPPORTED, "tables of %lld blocks of %d tokens", (long long)b->table_ld, c->block);
-    if (b->requests > INT32_MAX / 2 || b->rows > INT32_MAX / heads) return fail(ctx, NNQ_ERR_UNSUPPORTED, "a batch of %lld requests and %lld rows", (long long)b->requests, (long long)b->rows);
+    // (so are query vectors, up to an item beyond the last)
+    if (b->requests > INT32_MAX / 2 || b->rows > (INT32_MAX - 1024) / heads) return fail(ctx, NNQ_ERR_UNSUPPORTED, "a batch of %lld requests and %lld rows", (long long)b->requests, (long long)b->rows);
     return NNQ_OK;
 }
 

@@ -72,14 +72,16 @@ __device__ __forceinline__ void tc_range(const KvAttn &a, const TcRequest &q, in
 }
 // tiles of one head of a request, by a whole warp
 template <int KT>
-__device__ __forceinline__ int tc_head_steps(const KvAttn &a, const TcRequest &q) {
-    int n = 0;
+__device__ __forceinline__ int64_t tc_head_steps(const KvAttn &a, const TcRequest &q) {
+    int64_t n = 0;   // (a prompt of some million rows passes 32 bits)
     for (int cb = threadIdx.x & 31; cb < q.cbs; cb += 32) {
         int f, s;
         tc_range<KT>(a, q, cb, f, s);
         n += s;
     }
-    return __reduce_add_sync(0xFFFFFFFFu, n);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xFFFFFFFFu, (long long)n, o);
+    return n;
 }
 
 struct TcPlan {
@@ -99,8 +101,8 @@ __device__ TcPlan tc_plan(const KvAttn &a, int parts, int *found, int64_t *sums)
         for (uint32_t m = __ballot_sync(0xFFFFFFFFu, q.cbs > 0); m; m &= m - 1) {
             const int src = __ffs(m) - 1;
             const TcRequest o = {__shfl_sync(0xFFFFFFFFu, q.row0, src), __shfl_sync(0xFFFFFFFFu, q.rows, src), __shfl_sync(0xFFFFFFFFu, q.length, src), __shfl_sync(0xFFFFFFFFu, q.cbs, src)};
-            const int n = tc_head_steps<KT>(a, o);
-            if (lane == src) mine = (int64_t)n * a.kv_heads;
+            const int64_t n = tc_head_steps<KT>(a, o);
+            if (lane == src) mine = n * a.kv_heads;
         }
         long long x = mine;
 #pragma unroll
@@ -137,10 +139,10 @@ __device__ TcPlan tc_plan(const KvAttn &a, int parts, int *found, int64_t *sums)
     __syncthreads();
     if (warp == 0) {   // head and vectors within the request
         const TcRequest q = tc_request(a, found[0]);
-        const int per_head = tc_head_steps<KT>(a, q);
-        const int64_t off = sums[32];
+        const int64_t per_head = tc_head_steps<KT>(a, q), off = sums[32];
         const int head = (int)(off / per_head);
-        int rest = (int)(off - (int64_t)head * per_head), sum = 0;
+        const int64_t rest = off - head * per_head;
+        int64_t sum = 0;
         for (int c0 = 0; c0 < q.cbs; c0 += 32) {
             int f, s = 0;
             if (c0 + lane < q.cbs) tc_range<KT>(a, q, c0 + lane, f, s);
@@ -153,7 +155,7 @@ __device__ TcPlan tc_plan(const KvAttn &a, int parts, int *found, int64_t *sums)
             if (rest >= sum + x - s && rest < sum + x) {
                 found[1] = head;
                 found[2] = c0 + lane;
-                found[3] = rest - (sum + x - s);
+                found[3] = (int)(rest - (sum + x - s));
             }
             sum += __shfl_sync(0xFFFFFFFFu, x, 31);
         }

@@ -154,3 +154,12 @@ def test_a_batch_has_a_position_for_every_slot(slots, positions):
     """`build` writes both for as many rows as there are slots."""
     with pytest.raises(api.ShapeMismatch):
         KvBatch.from_tensors(DeviceInts(2, 4), DeviceInts(2), DeviceInts(3), 16, slot=DeviceInts(slots), position=DeviceInts(positions), backend=SimpleNamespace(device=0))
+
+
+@pytest.mark.parametrize("over,status", [(0, UNSUPPORTED), (1100, 0)])
+def test_query_vectors_are_counted_in_32_bits(lib, ctx, over, status):
+    """Up to an item of 256 vectors beyond the last, so the last thousand numbers of the range are left out."""
+    need, heads = ctypes.c_size_t(), 4
+    b = _Batch(P, P, P, 1, 4, ((1 << 31) - 1 - over) // heads, 1)
+    c = cache(kv_heads=1)
+    assert lib.nnq_kv_attention_workspace(ctx, ctypes.byref(c), ctypes.byref(b), heads, ctypes.byref(need)) == status
