@@ -783,7 +783,8 @@ typedef struct nnq_kv_batch {
  * its own, with window > 0 the last `window` of them; query head h reads key / value head h / (heads / kv_heads).
  * q [rows, heads, dim] and y in the same layout, f32 or bf16, rows q_ld / y_ld elements apart, 16-byte aligned, apart from each
  * other. A row that sees nothing is zero; rows behind the last request are left as they were. Scores, softmax and sums are f32, codes exact, queries
- * and weights enter the products with 22 bits (bf16 queries exactly; with bf16 queries and outputs the weights of requests of more than
+ * and weights enter the products with 22 bits (bf16 queries exactly), weights below some 2^-10 of the largest of a vector with fewer: no weight
+ * is off by more than 2^-32 of the largest (with bf16 queries and outputs the weights of requests of more than
  * 32 query vectors per key / value head, dim 64 and 128, are rounded to 11 bits; with f32 ones their sums of products lean towards zero, 5e-6 of an output
  * at 3000 positions and in proportion beyond). A block number outside the cache is not read: its positions
  * count as unseen, and nnq_device_status reports NNQ_ERR_INVALID_ARG. The workspace (nnq_kv_attention_workspace; 16-byte

@@ -13,12 +13,16 @@
 // Keys as the 16 rows waste none of the tensor core on missing query vectors. Codes are exact in f16; a query vector enters under a
 // power of two (one f16 term for bf16 queries, which is exact; two for f32), weights as two f16 terms (22 bits), so that scores, sums
 // and outputs are of f32 accuracy. A block's scales stay outside: the key's multiplies the scores, the value's goes into the exponent
-// of the weight, w = 2^(s - mv + e_v), which has a reference mv of its own beside the maximum m of the sum (l = sum 2^(s - m)): weights
-// stay between 0 and 2^8 whatever the scales are. Both references move only when a score passes them by 8, so most steps have one vote
-// in place of the maxima's exchange. The tensor core cuts off what its f32 sums cannot hold, always towards zero, so chains in it are
-// kept short: 32 dimensions of a score, kKvFlush steps of an output, which then join sums in shared memory (2 requests of 130001
-// positions, f32: all steps in one chain 113.5 us and an error of the outputs against 64 bits of 2.3e-6, chains of 16 steps 114.8 us and
-// 0.86e-6, of 8 steps 116.6 us and 0.65e-6; torch in f32: 1.24e-6).
+// of the weight, w = 2^(s - mv + e_v), which has a reference mv of its own beside the maximum m of the sum (l = sum 2^(s - m)), whatever
+// the scales are. It stands 2^11 below the largest s + e_v, so that the largest weight is 2^11 to 2^15, next to the end of f16: the second
+// term ends at multiples of 2^-24, which is then 2^-35 of the largest weight and scale. Both references move only when a score passes
+// them by 2^4, so most steps have one vote in place of the maxima's exchange. (References at the largest score itself and moves by 2^8
+// leave 2^-24: the outputs of 1100 keys 16 / 20 nats under a first one whose value is zero are then off by 9e-3 / 0.13 of the largest in place
+// of 4e-6 / 1.3e-4, in the same time.)
+// The tensor core cuts off what its f32 sums cannot hold, always towards zero, so chains in it are kept short: 32 dimensions of a
+// score, kKvFlush steps of an output, which then join sums in shared memory (2 requests of 130001 positions, f32: all steps in one chain
+// 113.5 us and an error of the outputs against 64 bits of 2.3e-6, chains of 16 steps 114.8 us and 0.86e-6, of 8 steps 116.6 us and
+// 0.65e-6; torch in f32: 1.24e-6).
 //
 // Work is dealt in steps of 16 keys: all steps of all (request, head, vectors) items in one row, cut into equal parts, one for each
 // CTA, whatever the requests' lengths are. An item counts kKvPad steps more than it has, about what beginning and ending one takes, so
@@ -40,7 +44,7 @@ constexpr int kKvPad = 32;              // (us with 8 / 16 / 32 / 64: 40 ragged 
 constexpr int kKvFlush = 16;
 constexpr int kNothing = INT32_MIN;   // in place of a block: no key of the step is seen
 constexpr float kKvLog2E = 1.4426950408889634f;
-constexpr float kKvSlack = 8.0f;   // a score may pass the reference by this power of two: weights up to 256 in f16
+constexpr float kKvSlack = 4.0f, kKvLow = 11.0f;   // a score may pass the references by 2^4; mv is 2^11 lower: weights up to 2^15 in f16
 
 // records: [part][began before, begins here][column]: m, mv, l, unused, then O[dim]; behind them what every part has to join
 __host__ __device__ inline int kv_record_floats(int dim) { return 4 + dim; }
@@ -398,7 +402,7 @@ __global__ void __launch_bounds__(kKvWarps * 32, D <= 128 ? 2 : 1) kv_attn_kerne
                     for (int i = 0; i < 2; i++) {
                         if (big[i] == -INFINITY) continue;   // nothing seen yet or here
                         const bool none = thr[i] == -INFINITY;   // a first reference: the sums are zero
-                        const float mn = none ? big[i] : fmaxf(m[i], big[i]), vn = none ? big[i] + vexp : fmaxf(mv[i], big[i] + vexp);
+                        const float mn = none ? big[i] : fmaxf(m[i], big[i]), vn = none ? big[i] + vexp - kKvLow : fmaxf(mv[i], big[i] + vexp - kKvLow);
                         const float f = none ? 1.0f : kv_ex2(mv[i] - vn);
                         l[i] *= none ? 1.0f : kv_ex2(m[i] - mn);
 #pragma unroll
@@ -409,7 +413,7 @@ __global__ void __launch_bounds__(kKvWarps * 32, D <= 128 ? 2 : 1) kv_attn_kerne
                         m[i] = mn;
                         mv[i] = vn;
                         thr[i] = mn + kKvSlack;
-                        thv[i] = vn + kKvSlack;
+                        thv[i] = vn + (kKvLow + kKvSlack);
                     }
                 }
                 // ---- weights
@@ -482,8 +486,8 @@ __global__ void __launch_bounds__(kKvWarps * 32, D <= 128 ? 2 : 1) kv_attn_kerne
             }
             if (whole) {
                 const int v = vec0 + col, row = v / a.group;
-                // (the values' factor of e4m3 codes; exponents of both references are far inside the range. No key seen: 0; NaN: l is)
-                const float y = ll == 0.0f ? 0.0f : o * (exp2f(mvv - mm) * Codes::unscale) / ll;
+                // (2^(mv - m) in two halves: it can lie below the numbers where the output does not. No key seen: 0; NaN: l is)
+                const float h = exp2f(0.5f * (mvv - mm)), y = ll == 0.0f ? 0.0f : o * Codes::unscale / ll * h * h;
                 store_out(a, (int64_t)(rq.row0 + row) * a.y_ld + (int64_t)(head * a.group + v - row * a.group) * D + d, y);
             } else {
                 float *rec = records + (((int64_t)blockIdx.x * 2 + (v0 == 0 ? 1 : 0)) * kKvCols + col) * REC;
@@ -568,12 +572,12 @@ __global__ void __launch_bounds__(256) kv_join_kernel(const KvAttn a, const floa
         s.w += x.w;
         l += part_l[w].x;
     }
-    const float f = l == 0.0f ? 0.0f : exp2f(mv - mm) * CodePairs<FMT>::unscale / l;
+    const float h = exp2f(0.5f * (mv - mm)), f = l == 0.0f ? 0.0f : CodePairs<FMT>::unscale / l;
     const int v = j.rest + col, row = v / a.group;
     const int64_t to = (int64_t)(j.group_row + row) * a.y_ld + (int64_t)(j.head * a.group + v - row * a.group) * a.dim + 4 * q;
     const float y[4] = {s.x, s.y, s.z, s.w};
 #pragma unroll
-    for (int i = 0; i < 4; i++) store_out(a, to + i, l == 0.0f ? 0.0f : y[i] * f);
+    for (int i = 0; i < 4; i++) store_out(a, to + i, l == 0.0f ? 0.0f : y[i] * f * h * h);
 }
 
 static int kv_parts(nnq_ctx *ctx, int dim) { return (dim <= 128 ? 2 : 1) * ctx->sm_count; }

@@ -23,8 +23,9 @@
 // by some 2^-26 for every 16 keys and term (f32, heads of 64: 3054 keys, error against 64 bits 5.0e-6; shorter chains would need a second
 // place for the sums, which heads of 128 leave no columns for). With bf16 outputs that is below their rounding up to a million keys.
 // Scales: a block's key exponent multiplies its scores in f32. Its value exponent enters the weight, w = p 2^(m - mv + e_v) with a
-// reference mv of its own, the largest score + e_v as m is that of the scores: one factor per vector and 16 keys, and weights
-// between 0 and 2^8 whatever the scales are.
+// reference mv of its own, 2^7 below the largest score + e_v as m is the largest score: one factor per vector and 16 keys, and weights
+// up to 2^15 whatever the scales are, as in kv_attn.cu. References move for 2^8 here, not 2^4, as the sums are scaled in tensor memory
+// (prompt of 2000 rows behind 2100, moves for 2^4 / 2^6 / 2^7 / 2^8: 216 / 204 / 194 / 192 us).
 //
 // Work: the key tiles of all (request, head, 256 vectors) items in one row, cut into equal parts, one per SM: causal rows and
 // long contexts load all SMs alike. An item inside a part is written directly, of one that is cut every part leaves a record, and
@@ -39,7 +40,7 @@ namespace nnq {
 
 constexpr int kTcCols = 256, kTcThreads = 20 * 32, kTcKeys = 64, kTcMinSteps = 8;
 constexpr int kTcNone = INT32_MIN;   // in place of a block: no such key
-constexpr float kTcLog2E = 1.4426950408889634f, kTcSlack = 8.0f;
+constexpr float kTcLog2E = 1.4426950408889634f, kTcSlack = 8.0f, kTcLow = 7.0f;   // weights up to 2^15
 
 struct TcItem {
     int r, head, cb;              // request, key / value head, number of the 256 vectors
@@ -431,7 +432,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attn_tc_kernel(const KvAttn 
                     float f = 1.0f;
                     if (moves) {
                         const bool none = thr == -INFINITY;   // a first reference: the sums are zero
-                        const float mn = none ? mt : fmaxf(m, mt), vn = none ? vt : fmaxf(mv, vt);
+                        const float mn = none ? mt : fmaxf(m, mt), vn = none ? vt - kTcLow : fmaxf(mv, vt - kTcLow);
                         if (!none) {
                             l *= exp2f(m - mn);
                             f = exp2f(mv - vn);
@@ -439,7 +440,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attn_tc_kernel(const KvAttn 
                         m = mn;
                         mv = vn;
                         thr = mn + kTcSlack;
-                        thv = vn + kTcSlack;
+                        thv = vn + (kTcLow + kTcSlack);
                     }
                     if (!first && __any_sync(0xFFFFFFFFu, f != 1.0f)) {
                         ok = __all_sync(0xFFFFFFFFu, mbar_wait_fast(of + 8 * (2 * w + ((nw - 1) & 1)), ((nw - 1) >> 1) & 1));
@@ -509,7 +510,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attn_tc_kernel(const KvAttn 
             tc_fence_after();
             const bool whole = it.s0 == 0 && it.s1 == it.steps, mine = w * 128 + me < it.vecs, none = !(thr > -INFINITY) && l == 0.0f;
             if (whole) {
-                const float inv = none ? 0.0f : exp2f(mv - m) * Codes::unscale / l;
+                const float h = exp2f(0.5f * (mv - m)), inv = none ? 0.0f : Codes::unscale / l;   // (in two halves as in kv_attn.cu)
                 const int64_t to = (int64_t)(it.row0 + row) * a.y_ld + (int64_t)qhead * D;
 #pragma unroll 1
                 for (int c = 0; c < D / 32; c++) {
@@ -518,7 +519,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attn_tc_kernel(const KvAttn 
                     if (!mine) continue;
                     float y[32];
 #pragma unroll
-                    for (int i = 0; i < 32; i++) y[i] = none ? 0.0f : __uint_as_float(x[i]) * inv;
+                    for (int i = 0; i < 32; i++) y[i] = none ? 0.0f : __uint_as_float(x[i]) * inv * h * h;
                     if (a.y_dt == NNQ_F32) {
                         float4 *p = reinterpret_cast<float4 *>(reinterpret_cast<float *>(a.y) + to + 32 * c);
 #pragma unroll
@@ -719,11 +720,11 @@ __global__ void __launch_bounds__(kTcCols) kv_tc_join_kernel(const KvAttn a, con
         }
     }
     const int64_t to = (int64_t)(j.row + row) * a.y_ld + (int64_t)(j.head + vec - row * a.group) * a.dim;
-    const float inv = l == 0.0f ? 0.0f : exp2f(mv - mm) * unscale / l;   // (l is NaN where only NaN scores came)
+    const float inv = l == 0.0f ? 0.0f : unscale / l, h = l == 0.0f ? 0.0f : exp2f(0.5f * (mv - mm));   // (l is NaN where only NaN scores came)
 #pragma unroll
     for (int q = 0; q < Q; q++) {
         if (q0 + q >= quads) break;
-        const float4 y = make_float4(o[q].x * inv, o[q].y * inv, o[q].z * inv, o[q].w * inv);
+        const float4 y = make_float4(o[q].x * inv * h * h, o[q].y * inv * h * h, o[q].z * inv * h * h, o[q].w * inv * h * h);
         if (a.y_dt == NNQ_F32) *reinterpret_cast<float4 *>(reinterpret_cast<float *>(a.y) + to + 4 * (q0 + q)) = y;
         else *reinterpret_cast<uint2 *>(reinterpret_cast<__nv_bfloat16 *>(a.y) + to + 4 * (q0 + q)) = make_uint2(pack_bf16(y.x, y.y), pack_bf16(y.z, y.w));
     }

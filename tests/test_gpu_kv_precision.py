@@ -1,0 +1,57 @@
+"""How many digits attention over the 8-bit cache keeps where they are easily lost: keys that weigh little beside one that weighs nearly all."""
+import numpy as np
+import pytest
+
+torch = pytest.importorskip("torch")
+
+from nn_b200 import kv_cache
+from tests import kv_reference as ref
+from tests.test_gpu_kv_cache import DEV, FORMATS, i32, serving, values_of
+
+pytestmark = pytest.mark.gpu
+
+
+def bound(mag, want, top, dim, keys, out_dtype, largest, one_term=False):
+    """How far an output may be off, element by element: mag = sum p |v|, top the largest scale sum |q||k| of a vector, keys those that it sees.
+
+    A score: products exact or of two f16 terms (2^-21), dim / 16 sums of 2^-23 each, scaling and reference 2^-23: delta = top (2^-20 +
+    dim / 16 2^-23), which counts twice (weight and normalisation); exponentials 2^-21, weights of two terms 2^-22, the joining of warps and
+    parts 2^-20: 2^-19 in all; the sums over keys 2^-23 for every 16 of them. A factor of two on all. A weight of two terms ends at a multiple of
+    2^-24 under a reference that gives the largest 2^7 or more: off by 2^-25 at most, 2^-32 of the largest. Outputs are rounded once.
+    one_term: weights of one f16 number, half a step of which is 2^-12 to 2^-11 of them and 2^-32 of the largest at least."""
+    eps = 2 * top * (2.0 ** -20 + dim / 16 * 2.0 ** -23) + 2.0 ** -19 + keys / 16 * 2.0 ** -23
+    half_step = 2.0 ** -8 if out_dtype == torch.bfloat16 else 2.0 ** -24
+    return (2 * eps + (2.0 ** -11 if one_term else 0.0)) * mag + half_step * np.abs(want) + keys * 2.0 ** -32 * largest
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows,requests", [(1, 64), (40, 16)])
+@pytest.mark.parametrize("nats", [8.0, 16.0, 17.5, 20.0])
+def test_keys_under_a_sink(fmt, dtype, rows, requests, nats):
+    """The first key of every request is `nats` above the others and its value is zero, as models come to use the first token of a context:
+    what is attended to in earnest has weights of e^-nats, and all of the output is theirs."""
+    rng = np.random.default_rng(int(nats * 2) + rows)
+    lengths, heads, dim, block = [1100] * requests, 4, 64, 16
+    c, table, start, q, b = serving(rng, fmt, lengths, [rows] * requests, heads=heads, kv=heads, dim=dim, block=block, dtype=dtype)
+    one = 1.0 if fmt == kv_cache.INT8 else 4.0   # (values of 64 to 127 for int8, 256 to 448 for e4m3)
+    kinds = np.arange(256)[(ref.VALUES[fmt] >= 64 * one) & (ref.VALUES[fmt] <= ref.TOP[fmt])].astype(np.uint8)
+    small = np.arange(256)[np.abs(ref.VALUES[fmt]) <= 16 * one].astype(np.uint8)
+    k, v = rng.choice(small, c.k.shape), rng.choice(kinds, c.v.shape)
+    k[..., 0] = 0
+    first = table[:, 0]
+    k[first, :, 0] = 0
+    k[first, :, 0, 0] = np.argmax(np.where(ref.VALUES[fmt] <= ref.TOP[fmt], ref.VALUES[fmt], 0))
+    v[first, :, 0] = 0
+    c.k.copy_(torch.from_numpy(k))
+    c.v.copy_(torch.from_numpy(v))
+    for e in (c.k_exp, c.v_exp):
+        e.fill_(121 if fmt == kv_cache.INT8 else 119)   # values up to about two
+    q[:, :, 0] = nats * dim ** 0.5 / float(ref.TOP[fmt] * 2.0 ** (-6 if fmt == kv_cache.INT8 else -8))
+    y = c.attend(q, b, max_rows=rows)
+    want, mag, top = ref.attend(q.double().cpu().numpy(), *values_of(c), table, lengths, start, block, dim ** -0.5, 0)
+    lim = bound(mag, want, top, dim, 1100, dtype, 2.0, dtype == torch.bfloat16 and rows > 1)
+    off = np.abs(y.double().cpu().numpy() - want)
+    print(f"largest error {off.max() / np.abs(want).max():.2e} of the largest output")
+    assert (off <= lim).all(), (off.max(), (off / lim).max())
+    c.backend.device_status()
