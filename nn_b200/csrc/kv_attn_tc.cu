@@ -19,9 +19,11 @@
 // MMA warps on each (217 us) and four converter warps in favour of more registers for the softmax (186 beside 182).
 // Codes are exact in f16. T = 1 (bf16 queries and outputs): a query vector is exact under its power of two, a weight is one f16 number, off
 // by up to 2^-11 of itself where the output's own rounding is 2^-8 of it. T = 2 (f32 on either side): both have two terms, 22 bits.
-// The sums in tensor memory run through all tiles of a part, and the tensor core cuts off what they cannot hold: outputs lean towards zero
-// by some 2^-26 for every 16 keys and term (f32, heads of 64: 3054 keys, error against 64 bits 5.0e-6; shorter chains would need a second
-// place for the sums, which heads of 128 leave no columns for). With bf16 outputs that is below their rounding up to a million keys.
+// The tensor core cuts off what its f32 sums cannot hold, towards zero, so a chain of products in tensor memory ends after kTcChain tiles and its sums
+// join others in the item's record in the workspace, in f32 (a second place in tensor memory would need columns that heads of 128 leave
+// none of). Mean error of f32 outputs over 3000 / 12001 / 32000 positions, heads of 128, e4m3: in one chain 3.2e-6 / 1.4e-5 / 3.8e-5, of 8 tiles
+// 2.0e-6 (3000), of 4 tiles 1.1e-6 / 1.2e-6 / 1.2e-6; 2000 f32 rows behind 2100: 264, 308, 346 us. With bf16 outputs chains of 64 tiles, some 2e-5 of an
+// output, which is far below its rounding, and 1.0 of the time of one chain.
 // Scales: a block's key exponent multiplies its scores in f32. Its value exponent enters the weight, w = p 2^(m - mv + e_v) with a
 // reference mv of its own, 2^7 below the largest score + e_v as m is the largest score: one factor per vector and 16 keys, and weights
 // up to 2^15 whatever the scales are, as in kv_attn.cu. References move for 2^8 here, not 2^4, as the sums are scaled in tensor memory
@@ -39,6 +41,7 @@
 namespace nnq {
 
 constexpr int kTcCols = 256, kTcThreads = 20 * 32, kTcKeys = 64, kTcMinSteps = 8;
+constexpr int kTcChain = 4, kTcChainBf16 = 64;   // tiles of a chain, by the outputs' type; powers of two
 constexpr int kTcNone = INT32_MIN;   // in place of a block: no such key
 constexpr float kTcLog2E = 1.4426950408889634f, kTcSlack = 8.0f, kTcLow = 7.0f;   // weights up to 2^15
 
@@ -307,6 +310,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attn_tc_kernel(const KvAttn 
     tc_fence_after();
     const uint32_t tmem = __shfl_sync(0xFFFFFFFFu, tmem_s, 0);   // of group w: O at 256 w, S and P at 256 w + 128 and 64 on
     uint8_t *stages = smem + Sh::q_bytes;
+    const int chain = a.y_dt == NNQ_F32 ? kTcChain : kTcChainBf16;
     bool ok = true;
     TcWalk<KT> walk(a, plan, found);
     TcItem it;
@@ -388,7 +392,42 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attn_tc_kernel(const KvAttn 
                 __syncwarp();
                 if (elect_one()) mbar_arrive(pf + 8 * (2 * w + (t & 1)));
             };
+            // Products add up in tensor memory for `chain` tiles at most, then join the sums in the item's record, of which a thread has one vector as well.
+            float4 *rec = reinterpret_cast<float4 *>(records + ((int64_t)blockIdx.x * 2 + (it.s0 == 0 ? 1 : 0)) * tc_record_floats(D)) + w * 128 + me;
+            float kept = -INFINITY;   // reference of the record's sums (-inf: they are zero)
+            auto join_sums = [&](int c, uint32_t (&x)[32]) {   // 32 dimensions
+                const float f = exp2f(kept - mv);
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    const float4 q = rec[kTcCols * (1 + 8 * c + i)];
+                    x[4 * i] = __float_as_uint(fmaf(q.x, f, __uint_as_float(x[4 * i])));
+                    x[4 * i + 1] = __float_as_uint(fmaf(q.y, f, __uint_as_float(x[4 * i + 1])));
+                    x[4 * i + 2] = __float_as_uint(fmaf(q.z, f, __uint_as_float(x[4 * i + 2])));
+                    x[4 * i + 3] = __float_as_uint(fmaf(q.w, f, __uint_as_float(x[4 * i + 3])));
+                }
+            };
+            auto keep_sums = [&](int c, const uint32_t (&x)[32]) {
+#pragma unroll
+                for (int i = 0; i < 8; i++)
+                    rec[kTcCols * (1 + 8 * c + i)] = make_float4(__uint_as_float(x[4 * i]), __uint_as_float(x[4 * i + 1]), __uint_as_float(x[4 * i + 2]), __uint_as_float(x[4 * i + 3]));
+            };
+            // the weights of the chain's last tile are handed over here, and the tile behind it begins as an item's first one does
+            auto drain_sums = [&](bool again) {
+                hand_over(nw - 1);
+                ok = __all_sync(0xFFFFFFFFu, mbar_wait_fast(of + 8 * (2 * w + ((nw - 1) & 1)), ((nw - 1) >> 1) & 1));
+                if (!ok) return;
+                tc_fence_after();
+#pragma unroll 1
+                for (int c = 0; c < D / 32; c++) {
+                    uint32_t x[32];
+                    tmem_ld32(o_t + 32 * c, x);
+                    if (again) join_sums(c, x);
+                    keep_sums(c, x);
+                }
+                kept = thr > -INFINITY ? mv : -INFINITY;
+            };
             // A tile of keys, starting at key0; CLEAR: every vector of the warp sees all of it.
+            // (`first` of a chain: no weights to hand over, no sums to scale)
             auto tile = [&](auto clear, const int2 *sub, int key0, bool first) {
                 const uint32_t s_t = o_t + 128 + 64 * (nw & 1);
                 constexpr bool CLEAR = decltype(clear)::value;
@@ -498,17 +537,22 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attn_tc_kernel(const KvAttn 
                 ok = __all_sync(0xFFFFFFFFu, mbar_wait_fast(sf + 8 * (2 * w + (nw & 1)), (nw >> 1) & 1) && mbar_wait_fast(full + 8 * st, (n / STAGES) & 1));
                 if (!ok) break;
                 tc_fence_after();
+                const bool first = ((s - it.s0) & (chain - 1)) == 0;
+                if (first && s > it.s0) {
+                    drain_sums(s - it.s0 > chain);
+                    if (!ok) break;
+                }
                 const int2 *sub = sub_info[st];
                 const int4 i0 = *reinterpret_cast<const int4 *>(sub), i1 = *reinterpret_cast<const int4 *>(sub + 2);
-                if (__all_sync(0xFFFFFFFFu, pos - key0 >= KT - 1 && low <= key0 && (i0.x | i0.z | i1.x | i1.z) >= 0)) tile(std::true_type(), sub, key0, s == it.s0);
-                else tile(std::false_type(), sub, key0, s == it.s0);
+                if (__all_sync(0xFFFFFFFFu, pos - key0 >= KT - 1 && low <= key0 && (i0.x | i0.z | i1.x | i1.z) >= 0)) tile(std::true_type(), sub, key0, first);
+                else tile(std::false_type(), sub, key0, first);
             }
             if (!ok) break;
             hand_over(nw - 1);
             ok = __all_sync(0xFFFFFFFFu, mbar_wait_fast(of + 8 * (2 * w + ((nw - 1) & 1)), ((nw - 1) >> 1) & 1));
             if (!ok) break;
             tc_fence_after();
-            const bool whole = it.s0 == 0 && it.s1 == it.steps, mine = w * 128 + me < it.vecs, none = !(thr > -INFINITY) && l == 0.0f;
+            const bool whole = it.s0 == 0 && it.s1 == it.steps, mine = w * 128 + me < it.vecs, none = !(thr > -INFINITY) && l == 0.0f, drained = it.s1 - it.s0 > chain;
             if (whole) {
                 const float h = exp2f(0.5f * (mv - m)), inv = none ? 0.0f : Codes::unscale / l;   // (in two halves as in kv_attn.cu)
                 const int64_t to = (int64_t)(it.row0 + row) * a.y_ld + (int64_t)qhead * D;
@@ -517,6 +561,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attn_tc_kernel(const KvAttn 
                     uint32_t x[32];
                     tmem_ld32(o_t + 32 * c, x);
                     if (!mine) continue;
+                    if (drained) join_sums(c, x);
                     float y[32];
 #pragma unroll
                     for (int i = 0; i < 32; i++) y[i] = none ? 0.0f : __uint_as_float(x[i]) * inv * h * h;
@@ -532,17 +577,14 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attn_tc_kernel(const KvAttn 
                     }
                 }
             } else {
-                float4 *rec = reinterpret_cast<float4 *>(records + ((int64_t)blockIdx.x * 2 + (it.s0 == 0 ? 1 : 0)) * tc_record_floats(D));
-                const int v = w * 128 + me;
-                if (mine) rec[v] = make_float4(none ? -INFINITY : thr > -INFINITY ? m : l, mv, l, 0.0f);   // (l: scores that are all NaN)
+                if (mine) rec[0] = make_float4(none ? -INFINITY : thr > -INFINITY ? m : l, mv, l, 0.0f);   // (l: scores that are all NaN)
 #pragma unroll 1
                 for (int c = 0; c < D / 32; c++) {
                     uint32_t x[32];
                     tmem_ld32(o_t + 32 * c, x);
                     if (!mine) continue;
-#pragma unroll
-                    for (int i = 0; i < 8; i++)
-                        rec[kTcCols * (1 + 8 * c + i) + v] = make_float4(__uint_as_float(x[4 * i]), __uint_as_float(x[4 * i + 1]), __uint_as_float(x[4 * i + 2]), __uint_as_float(x[4 * i + 3]));
+                    if (drained) join_sums(c, x);
+                    keep_sums(c, x);
                 }
             }
             tc_fence_before();
@@ -657,7 +699,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attn_tc_kernel(const KvAttn 
     #pragma unroll
                         for (int x = T - 1; x >= 0; x--)
     #pragma unroll
-                            for (int k = 0; k < KT / 16; k++) umma_ts(o_t, pa + 32 * x + 8 * k, dv + (2048 >> 4) * k, id_o, s > 0 || x < T - 1 || k != 0);
+                            for (int k = 0; k < KT / 16; k++) umma_ts(o_t, pa + 32 * x + 8 * k, dv + (2048 >> 4) * k, id_o, (s & (chain - 1)) != 0 || x < T - 1 || k != 0);
                         umma_commit(of + 8 * (2 * w + place));
                         umma_commit(empty + 8 * st);
                     }

@@ -55,3 +55,38 @@ def test_keys_under_a_sink(fmt, dtype, rows, requests, nats):
     print(f"largest error {off.max() / np.abs(want).max():.2e} of the largest output")
     assert (off <= lim).all(), (off.max(), (off / lim).max())
     c.backend.device_status()
+
+
+def exact(c, table, q, length, rows):
+    """A single request's outputs and sum p |v| in 64 bits, on the device."""
+    values = torch.from_numpy(ref.VALUES[c.fmt]).to(DEV)
+    p = torch.arange(length, device=DEV)
+    blk, off, e = i32(table[0]).long()[p // c.block], p % c.block, torch.arange(-127, 129, device=DEV).double()
+    k, v = (values[t[blk, :, off].long()] * torch.exp2(e)[x[blk].long()][:, :, None] for t, x in ((c.k, c.k_exp), (c.v, c.v_exp)))   # [length, kv, dim]
+    group = q.shape[1] // c.kv_heads
+    y, mag = torch.empty(q.shape, dtype=torch.float64, device=DEV), torch.empty(q.shape, dtype=torch.float64, device=DEV)
+    unseen = p[None] > torch.arange(length - rows, length, device=DEV)[:, None]
+    for h in range(q.shape[1]):
+        s = (q[:, h].double() @ k[:, h // group].T * c.dim ** -0.5).masked_fill_(unseen, -float("inf"))
+        w = torch.softmax(s, 1)
+        y[:, h], mag[:, h] = w @ v[:, h // group], w @ v[:, h // group].abs()
+    return y, mag
+
+
+@pytest.mark.parametrize("fmt,dim", [(kv_cache.INT8, 64), (kv_cache.E4M3, 128)])
+@pytest.mark.parametrize("rows", [1, 72])
+@pytest.mark.parametrize("length", [3000, 12001, 32000])
+def test_sums_in_f32_do_not_lean_with_the_length(fmt, dim, rows, length):
+    """Values of one sign, 32 heads (so that a part of the work is hundreds of keys): whatever the tensor core cuts off its sums shows in
+    the mean error. A product added to a sum loses half a unit of 2^-23 of it on average, the sum grows from nothing, and at most 64 are added
+    (two terms of a weight, 16 keys each): 64 * 2^-24 / 2 = 1.9e-6. Other roundings are as often up as down."""
+    rng = np.random.default_rng(length + rows)
+    c, table, start, q, b = serving(rng, fmt, [length], [rows], heads=32, kv=32, dim=dim, block=64)
+    c.v.bitwise_and_(0x7F)   # positive codes (e4m3's 0x7F reads as 480)
+    y = c.attend(q, b, max_rows=rows).double()
+    want, mag = exact(c, table, q, length, rows)
+    off = (y - want) / mag
+    print(f"mean {float(off.mean()):.2e}, root mean square {float(off.square().mean().sqrt()):.2e}, largest {float(off.abs().max()):.2e}")
+    assert abs(float(off.mean())) <= 2e-6
+    assert float(off.square().mean().sqrt()) <= 2.5e-6   # (the lean and what is left of some hundred roundings of 2^-23)
+    c.backend.device_status()
