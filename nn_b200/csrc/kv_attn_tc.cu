@@ -14,11 +14,12 @@
 //                   of it. (One warp for both groups took 100 clocks an MMA beside the scheduler's other warps and set the pace.)
 // What bounds it is the softmax: some 6100 instructions of a scheduler's warps per tile of both groups, the exponentials among them (the
 // special function unit takes 16 a clock and SM), and the hand-over between softmax and MMA. Measured: 2000 rows behind 2100, e4m3, 8 key /
-// value heads of 4 bf16 query heads of 128, 189 us with the joining, 537 TFLOP/s of the 102 GFLOP that a causal prompt takes; counters of an
+// value heads of 4 bf16 query heads of 128, 215 us with the joining, 474 TFLOP/s of the 102 GFLOP that a causal prompt takes; counters of an
 // earlier form of 182 us: tensor pipe 30 % active, logic and FMA pipes 38 %, special functions 32 %. Slower were 128 keys a tile with both
 // MMA warps on each (217 us) and four converter warps in favour of more registers for the softmax (186 beside 182).
-// Codes are exact in f16. T = 1 (bf16 queries and outputs): a query vector is exact under its power of two, a weight is one f16 number, off
-// by up to 2^-11 of itself where the output's own rounding is 2^-8 of it. T = 2 (f32 on either side): both have two terms, 22 bits.
+// Codes are exact in f16. A query vector is one f16 term under its power of two where that is exact (T = 1: bf16 queries and outputs), else two (T = 2); a
+// weight is always two, 22 bits (with one, 11 bits and 188 us for the prompt above, a bf16 output differed from the rounded exact one by 9e-4 in the
+// 2-norm, now by 2e-4).
 // The tensor core cuts off what its f32 sums cannot hold, towards zero, so a chain of products in tensor memory ends after kTcChain tiles and its sums
 // join others in the item's record in the workspace, in f32 (a second place in tensor memory would need columns that heads of 128 leave
 // none of). Mean error of f32 outputs over 3000 / 12001 / 32000 positions, heads of 128, e4m3: in one chain 3.2e-6 / 1.4e-5 / 3.8e-5, of 8 tiles
@@ -519,13 +520,12 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attn_tc_kernel(const KvAttn 
                                 }
                                 const float2 v = make_float2(kv_ex2(y.x), kv_ex2(y.y));
                                 sum = __fadd2_rn(sum, v);
-                                if (T == 2) kv_split(v.x, v.y, hw[k / 2], lw[k / 2]);
-                                else hw[k / 2] = half_bits(__floats2half2_rn(v.x, v.y));
+                                kv_split(v.x, v.y, hw[k / 2], lw[k / 2]);
                             }
                             l = fmaf(sum.x + sum.y, kv_ex2(-lf[2 * c + b]), l);
                         }
                         tc_st(s_t + 16 * c, hw);
-                        if (T == 2) tc_st(s_t + 32 + 16 * c, lw);
+                        tc_st(s_t + 32 + 16 * c, lw);
                     }
                 }
             };
@@ -697,9 +697,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attn_tc_kernel(const KvAttn 
                         const uint32_t va = smem_u32(stages + st * Sh::stage) + ATOMS * Sh::k_atom, pa = o_t + 128 + 64 * place;
                         const uint64_t dv = tc_desc_mn(va, Sh::k_atom);
     #pragma unroll
-                        for (int x = T - 1; x >= 0; x--)
+                        for (int x = 1; x >= 0; x--)
     #pragma unroll
-                            for (int k = 0; k < KT / 16; k++) umma_ts(o_t, pa + 32 * x + 8 * k, dv + (2048 >> 4) * k, id_o, (s & (chain - 1)) != 0 || x < T - 1 || k != 0);
+                            for (int k = 0; k < KT / 16; k++) umma_ts(o_t, pa + 32 * x + 8 * k, dv + (2048 >> 4) * k, id_o, (s & (chain - 1)) != 0 || x == 0 || k != 0);
                         umma_commit(of + 8 * (2 * w + place));
                         umma_commit(empty + 8 * st);
                     }

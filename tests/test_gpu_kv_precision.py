@@ -11,17 +11,16 @@ from tests.test_gpu_kv_cache import DEV, FORMATS, i32, serving, values_of
 pytestmark = pytest.mark.gpu
 
 
-def bound(mag, want, top, dim, keys, out_dtype, largest, one_term=False):
+def bound(mag, want, top, dim, keys, out_dtype, largest):
     """How far an output may be off, element by element: mag = sum p |v|, top the largest scale sum |q||k| of a vector, keys those that it sees.
 
     A score: products exact or of two f16 terms (2^-21), dim / 16 sums of 2^-23 each, scaling and reference 2^-23: delta = top (2^-20 +
     dim / 16 2^-23), which counts twice (weight and normalisation); exponentials 2^-21, weights of two terms 2^-22, the joining of warps and
     parts 2^-20: 2^-19 in all; the sums over keys 2^-23 for every 16 of them. A factor of two on all. A weight of two terms ends at a multiple of
-    2^-24 under a reference that gives the largest 2^7 or more: off by 2^-25 at most, 2^-32 of the largest. Outputs are rounded once.
-    one_term: weights of one f16 number, half a step of which is 2^-12 to 2^-11 of them and 2^-32 of the largest at least."""
+    2^-24 under a reference that gives the largest 2^7 or more: off by 2^-25 at most, 2^-32 of the largest. Outputs are rounded once."""
     eps = 2 * top * (2.0 ** -20 + dim / 16 * 2.0 ** -23) + 2.0 ** -19 + keys / 16 * 2.0 ** -23
     half_step = 2.0 ** -8 if out_dtype == torch.bfloat16 else 2.0 ** -24
-    return (2 * eps + (2.0 ** -11 if one_term else 0.0)) * mag + half_step * np.abs(want) + keys * 2.0 ** -32 * largest
+    return 2 * eps * mag + half_step * np.abs(want) + keys * 2.0 ** -32 * largest
 
 
 @pytest.mark.parametrize("fmt", FORMATS)
@@ -50,7 +49,7 @@ def test_keys_under_a_sink(fmt, dtype, rows, requests, nats):
     q[:, :, 0] = nats * dim ** 0.5 / float(ref.TOP[fmt] * 2.0 ** (-6 if fmt == kv_cache.INT8 else -8))
     y = c.attend(q, b, max_rows=rows)
     want, mag, top = ref.attend(q.double().cpu().numpy(), *values_of(c), table, lengths, start, block, dim ** -0.5, 0)
-    lim = bound(mag, want, top, dim, 1100, dtype, 2.0, dtype == torch.bfloat16 and rows > 1)
+    lim = bound(mag, want, top, dim, 1100, dtype, 2.0)
     off = np.abs(y.double().cpu().numpy() - want)
     print(f"largest error {off.max() / np.abs(want).max():.2e} of the largest output")
     assert (off <= lim).all(), (off.max(), (off / lim).max())
@@ -89,4 +88,22 @@ def test_sums_in_f32_do_not_lean_with_the_length(fmt, dim, rows, length):
     print(f"mean {float(off.mean()):.2e}, root mean square {float(off.square().mean().sqrt()):.2e}, largest {float(off.abs().max()):.2e}")
     assert abs(float(off.mean())) <= 2e-6
     assert float(off.square().mean().sqrt()) <= 2.5e-6   # (the lean and what is left of some hundred roundings of 2^-23)
+    c.backend.device_status()
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("rows,dim", [(1, 64), (40, 64), (40, 128), (150, 128)])
+@pytest.mark.parametrize("window", [2, 5, 40])
+def test_outputs_in_bf16_are_the_exact_ones_rounded(fmt, rows, dim, window):
+    """Whatever a request's rows are: no rounding to fewer bits stands in front of the one to bf16. Few keys, so that none averages away."""
+    rng = np.random.default_rng(window + rows)
+    lengths = [300, 200]
+    c, table, start, q, b = serving(rng, fmt, lengths, [rows, rows], heads=8, kv=2, dim=dim, block=32, dtype=torch.bfloat16)
+    y = c.attend(q, b, window=window, max_rows=rows).cpu()
+    k, v = values_of(c)
+    want, mag, top = ref.attend(q.double().cpu().numpy(), k, v, table, lengths, start, 32, dim ** -0.5, window)
+    lim = bound(mag, want, top, dim, window, torch.float32, np.abs(v).max())
+    low, high = (torch.from_numpy(x).to(torch.bfloat16) for x in (want - lim, want + lim))
+    wrong = ~((low <= y) & (y <= high))
+    assert not wrong.any(), (int(wrong.sum()), wrong.numel())
     c.backend.device_status()
