@@ -600,10 +600,12 @@ __global__ void __launch_bounds__(kTcThreads, 1) kv_attn_tc_kernel(const KvAttn 
             uint4 k[ATOMS], v[ATOMS];
             int2 info = make_int2(-1, 127);
             int blk, info_blk;   // of the next tile: this thread's key's, and (threads 0 .. SUBS - 1) that of 16 keys
+            // keys in front of what the first row sees and behind the last row are not looked for (their blocks may have been given back), by 16
+            const int base = it.length - it.rows, lo = row_first(a, base + it.vec0 / a.group) & ~15, hi = base + (it.vec0 + it.vecs - 1) / a.group;
             auto blocks = [&](int s) {
                 const int key0 = (it.first + s) * KT, key = key0 + key_of, key16 = key0 + 16 * pt;
-                blk = s < it.s1 && key < it.length ? table[key >> a.shift] : kTcNone;
-                info_blk = pt < SUBS && s < it.s1 && key16 < it.length ? table[key16 >> a.shift] : kTcNone;
+                blk = s < it.s1 && key >= lo && key <= hi ? table[key >> a.shift] : kTcNone;
+                info_blk = pt < SUBS && s < it.s1 && key16 >= lo && key16 <= hi ? table[key16 >> a.shift] : kTcNone;
             };
             auto load = [&](int s) {
                 const bool there = blk >= 0 && blk < a.blocks;

@@ -620,6 +620,20 @@ def test_attention_refuses_wrong_tensors():
             c.attend(*args, **kw)
 
 
+@pytest.mark.parametrize("rows", [1, 40, 150])
+@pytest.mark.parametrize("window,block", [(20, 16), (70, 16), (100, 16), (20, 32), (70, 32), (100, 64)])
+def test_blocks_behind_every_window_may_have_been_given_back(rows, window, block):
+    """Entries of blocks that no row of a request sees any more are -1: nothing reads them, and nothing is reported."""
+    rng = np.random.default_rng(rows + window)
+    lengths = [333, 150, 201]
+    c, table, start, q, b = serving(rng, 1, lengths, [rows] * 3, heads=8, kv=2, dim=64, block=block)
+    for r, n in enumerate(lengths):
+        table[r, :max(0, n - rows - window + 1) // block] = -1
+    assert (table[0, :1] == -1).all() and window > 1
+    b.table.copy_(i32(table))
+    check_attend(c, table, lengths, start, q, b, window=window)
+
+
 # ------------------------------------------------------------------------------------------
 # together
 # ------------------------------------------------------------------------------------------
