@@ -8,7 +8,9 @@
 // A row is dealt to a cluster of CTAs where the rows are few, and every CTA's sums meet in the first one's shared memory, in order.
 // The most probable tokens: the pass leaves the largest element of every group (four 16-byte vectors of a thread) in shared memory. The
 // threads of each of 32 lanes have seen disjoint parts of the slice, so at least 32 elements are not below the least of these parts'
-// maxima: the groups from there on (about a hundred) are ranked, and the `top` best are read again, element by element. Where that
+// maxima: the groups from there on (about a hundred) are ranked, and the `top` best are read again, element by element. Where one of these
+// parts is all -inf (few tokens are allowed), all groups with anything above -inf are (64 rows of 151936 with 20 such tokens, 20 alternatives:
+// 20 us as for other rows, 264 us by the search below). Where that
 // meets more equal values than there is room for, or a NaN, the largest element below the one before is looked for `top` times. Order:
 // larger value first, then the lower index.
 // What bounds it: bf16 rows 12 elements per clock and SM at the copy rate, where the special function unit forms 16 exponentials;
@@ -17,6 +19,7 @@
 // The reference turns logits into probabilities on the host (crates/nn-core/src/layers/generation/autoregressive_sampling.rs:14-21 and
 // the samplers beside it).
 #include <algorithm>
+#include <cfloat>
 
 #include "kv_cache.cuh"
 #include "tcgen05.cuh"
@@ -200,7 +203,9 @@ __global__ void __launch_bounds__(kLpThreads, kLpThreads == 256 ? 4 : 2) logprob
     if (a.top > 0) {
         bool few = !(cta_stats.l != cta_stats.l);   // (a NaN hides from the groups' maxima)
         if (few) {
-            const float bound = bound_s;
+            // (a lane may have seen nothing but -inf, where few tokens are allowed: then every group with something above it)
+            const float bound = fmaxf(bound_s, -FLT_MAX);
+            const bool rest = bound_s == -INFINITY;
             for (int g = 0; g < groups; g++)
                 if ((g * kLpUnroll * kLpThreads) + tid < sl.vecs && group_max[g * kLpThreads + tid] >= bound) {
                     const int at = atomicAdd(&found, 1);
@@ -225,9 +230,9 @@ __global__ void __launch_bounds__(kLpThreads, kLpThreads == 256 ? 4 : 2) logprob
                 const int groups_read = chosen, per = kLpUnroll * V;
                 if (tid == 0) found = 0;
                 __syncthreads();
-                auto offer = [&](int idx) {
+                auto offer = [&](int idx, bool masked) {
                     const float v = logit<F32>(x, idx);
-                    if (order_bits(v) >= least) {
+                    if (order_bits(v) >= least && (v == -INFINITY) == masked) {
                         const int at = atomicAdd(&found, 1);
                         if (at < kLpRoom) room[at] = order_key(v, idx);
                     }
@@ -235,9 +240,11 @@ __global__ void __launch_bounds__(kLpThreads, kLpThreads == 256 ? 4 : 2) logprob
 #pragma unroll 2
                 for (int i = tid; i < groups_read * per; i += kLpThreads) {
                     const int q = pick[i / per], e = i % per, u = (q / kLpThreads * kLpUnroll + e / V) * kLpThreads + q % kLpThreads;
-                    if (u < sl.vecs) offer(sl.head + u * V + e % V);
+                    if (u < sl.vecs) offer(sl.head + u * V + e % V, false);
                 }
-                for (int i = tid; i < sl.edges(); i += kLpThreads) offer(sl.edge(i));
+                for (int i = tid; i < sl.edges(); i += kLpThreads) offer(sl.edge(i), false);
+                // fewer than `top` above -inf: the first ones at -inf, which are among the first `top` of the slice
+                if (rest && sl.lo + tid < min(sl.hi, sl.lo + a.top)) offer(sl.lo + tid, true);
                 __syncthreads();
                 few = found <= kLpRoom;
             }

@@ -175,3 +175,59 @@ def test_two_threads_with_other_vocabularies():
     for th in threads:
         th.join()
     assert not wrong
+
+
+def masked_rows(rows, vocab, allowed, dtype, seed=0):
+    """Logits of a grammar: all but `allowed` tokens of a row are -inf."""
+    rng = np.random.default_rng(seed + vocab + allowed)
+    x = np.full((rows, vocab), -np.inf, np.float32)
+    for r in range(rows):
+        at = rng.choice(vocab, allowed, replace=False)
+        x[r, at] = rng.standard_normal(allowed) * 3
+    return torch.from_numpy(x).to("cuda:0", dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows,vocab", [(1, 151936), (3, 32003), (5, 700), (300, 5001)])
+@pytest.mark.parametrize("allowed", [1, 5, 20, 31, 33, 200])
+@pytest.mark.parametrize("top", [1, 20, 32])
+def test_alternatives_where_few_tokens_are_allowed(dtype, rows, vocab, allowed, top):
+    """Those that are allowed, then the lowest of the others at -inf."""
+    x = masked_rows(rows, vocab, allowed, dtype)
+    x[0, :3] = -float("inf")
+    if rows > 1:
+        x[1, :3], x[-1, -2:] = 1.5, 2.5   # next to the slice's edges
+    if not x.isfinite().any(1).all():
+        x[0, 3] = 0.5
+    token = x.float().argmax(1)
+    lp, ent, order, tl = ref.logprobs(x.double().cpu().numpy(), token.cpu().numpy(), top)
+    r = token_logprobs(x, token, top)
+    assert np.array_equal(r.top_tokens.cpu().numpy(), order)
+    got, there = r.top_logprobs.double().cpu().numpy(), np.isfinite(tl)
+    lim = (2.0 ** -20 + (vocab / 512 + 64) * 2.0 ** -24) * (1 + np.log(vocab))   # (as in `check`)
+    assert (got[~there] == -np.inf).all() and (np.abs(got[there] - tl[there]) <= lim + 2.0 ** -22 * np.abs(tl[there])).all()
+    assert (np.abs(r.logprob.double().cpu().numpy() - lp) <= lim + 2.0 ** -22 * np.abs(lp)).all()
+    assert (np.abs(r.entropy.double().cpu().numpy() - ent) <= 2 * lim).all()
+
+
+def test_masked_rows_cost_what_others_do():
+    """They are not read again for every alternative."""
+    x = torch.randn(64, 151936, device="cuda:0")
+    few = masked_rows(64, 151936, 20, torch.float32)
+    token = torch.zeros(64, dtype=torch.int32, device="cuda:0")
+
+    def shortest(t):
+        best = 1e9
+        for _ in range(10):
+            a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            a.record()
+            for _ in range(5):
+                token_logprobs(t, token, 20)
+            b.record()
+            b.synchronize()
+            best = min(best, a.elapsed_time(b))
+        return best
+
+    plain, masked = shortest(x), shortest(few)
+    print(f"{plain * 200:.1f} and {masked * 200:.1f} us")
+    assert masked <= 3 * plain
