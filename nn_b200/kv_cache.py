@@ -191,6 +191,8 @@ class KvCache:
             out = torch.empty(q.shape, dtype=q.dtype, device=self.device)
         elif out.shape != q.shape or out.device != self.device or out.dtype not in (torch.float32, torch.bfloat16) or out.stride(2) != 1 or out.stride(1) != self.dim:
             raise api.ShapeMismatch(f"out: expected {tuple(q.shape)}, heads next to each other, on {self.device}")
+        if not 0 <= window < 1 << 31:   # (the C call would take what is left of it in 32 bits)
+            raise api.InvalidArgument(f"a window of {window}")
         if batch.block != self.block or batch.backend.device != b.device:
             raise api.InvalidArgument(f"a batch of blocks of {batch.block} on {batch.device} for a cache of blocks of {self.block} on {self.device}")
         c = _Batch(batch.length.data_ptr(), batch.row_start.data_ptr(), batch.table.data_ptr(), batch.requests, batch.table.shape[1], n, max(int(max_rows), 1))

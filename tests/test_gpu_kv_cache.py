@@ -634,6 +634,13 @@ def test_blocks_behind_every_window_may_have_been_given_back(rows, window, block
     check_attend(c, table, lengths, start, q, b, window=window)
 
 
+@pytest.mark.parametrize("window", [-1, 2 ** 31, 2 ** 32, 2 ** 32 + 5])
+def test_windows_beyond_31_bits_are_refused(window):
+    c, b = kv_cache.KvCache(4, 2, 64), kv_cache.KvBatch(1, 4, 1, 16)
+    with pytest.raises(api.InvalidArgument):
+        c.attend(torch.zeros(1, 4, 64, device=DEV), b, window=window)
+
+
 # ------------------------------------------------------------------------------------------
 # together
 # ------------------------------------------------------------------------------------------
