@@ -42,19 +42,27 @@ def _int32(t, name: str, shape, index: int):
     return t
 
 
+def _fixed(name: str):
+    """A tensor whose memory the calls rely on: filled in place (``copy_``), not replaced."""
+    return property(lambda self: getattr(self, "_" + name))
+
+
 class KvBatch:
-    """Block tables [requests, max_blocks], lengths, packed rows (row_start), and slot and position of every row, on the device."""
+    """Block tables [requests, max_blocks], lengths, packed rows (row_start), and slot and position of every row, on the device. The tensors
+    are filled in place, not replaced."""
+
+    table, length, row_start, slot, position, used = map(_fixed, ("table", "length", "row_start", "slot", "position", "used"))
 
     def __init__(self, requests: int, max_blocks: int, rows: int, block: int = 16, backend: Optional[api.Backend] = None):
         if requests < 1 or max_blocks < 1 or rows < 0:
             raise api.InvalidArgument(f"a batch of {requests} requests, {max_blocks} blocks each, {rows} rows")
         torch = api._torch()
         b = backend or api.gpu_backend()
-        self.backend, self.block, self.rows = b, int(block), int(rows)
+        self.backend, self.block = b, int(block)
         self.device = torch.device("cuda", b.device)
         z = lambda *s: torch.zeros(s, dtype=torch.int32, device=self.device)  # noqa: E731
-        self.table = torch.full((requests, max_blocks), -1, dtype=torch.int32, device=self.device)
-        self.length, self.row_start, self.slot, self.position, self.used = z(requests), z(requests + 1), z(rows), z(rows), z(1)
+        self._table = torch.full((requests, max_blocks), -1, dtype=torch.int32, device=self.device)
+        self._length, self._row_start, self._slot, self._position, self._used = z(requests), z(requests + 1), z(rows), z(rows), z(1)
 
     @classmethod
     def from_tensors(cls, table, length, row_start, block: int, slot=None, position=None, backend: Optional[api.Backend] = None) -> "KvBatch":
@@ -66,17 +74,20 @@ class KvBatch:
         if table.dim() != 2 or table.shape[0] < 1 or table.shape[1] < 1:
             raise api.ShapeMismatch(f"table: expected [requests, blocks], got {tuple(table.shape)}")
         n = table.shape[0]
-        self.table, self.length = _int32(table, "table", table.shape, b.device), _int32(length, "length", (n,), b.device)
-        self.row_start = _int32(row_start, "row_start", (n + 1,), b.device)
-        self.slot = None if slot is None else _int32(slot, "slot", (slot.numel(),), b.device)
-        self.position = None if position is None else _int32(position, "position", (position.numel() if slot is None else slot.numel(),), b.device)
-        self.rows = 0 if slot is None else slot.numel()
-        self.used = torch.zeros(1, dtype=torch.int32, device=self.device)
+        self._table, self._length = _int32(table, "table", table.shape, b.device), _int32(length, "length", (n,), b.device)
+        self._row_start = _int32(row_start, "row_start", (n + 1,), b.device)
+        self._slot = None if slot is None else _int32(slot, "slot", (slot.numel(),), b.device)
+        self._position = None if position is None else _int32(position, "position", (position.numel() if slot is None else slot.numel(),), b.device)
+        self._used = torch.zeros(1, dtype=torch.int32, device=self.device)
         return self
 
     @property
     def requests(self) -> int:
         return self.table.shape[0]
+
+    @property
+    def rows(self) -> int:
+        return 0 if self._slot is None else self._slot.numel()
 
     def build(self, past, count, free, skip=None):
         """Tables and slots for `count` new tokens behind `past` ones, int32 [requests] each. `free`: numbers of free blocks (int32), of which
@@ -100,7 +111,9 @@ class KvBatch:
 
 class KvCache:
     """One layer's keys and values: codes uint8 [blocks, kv_heads, block, dim] (``k``, ``v``) and exponent bytes uint8 [blocks, kv_heads]
-    (``k_exp``, ``v_exp``); value = code * 2^(byte - 127)."""
+    (``k_exp``, ``v_exp``); value = code * 2^(byte - 127). A saved cache is brought back with ``copy_`` into these tensors."""
+
+    k, v, k_exp, v_exp = map(_fixed, ("k", "v", "k_exp", "v_exp"))
 
     def __init__(self, blocks: int, kv_heads: int, dim: int, block: int = 16, fmt: int = INT8, backend: Optional[api.Backend] = None):
         torch = api._torch()
@@ -116,8 +129,8 @@ class KvCache:
         self.blocks, self.kv_heads, self.dim, self.block, self.fmt = int(blocks), int(kv_heads), int(dim), int(block), int(fmt)
         self.device = torch.device("cuda", b.device)
         z = lambda *s: torch.zeros(s, dtype=torch.uint8, device=self.device)  # noqa: E731
-        self.k, self.v = z(blocks, kv_heads, block, dim), z(blocks, kv_heads, block, dim)
-        self.k_exp, self.v_exp = z(blocks, kv_heads).fill_(127), z(blocks, kv_heads).fill_(127)
+        self._k, self._v = z(blocks, kv_heads, block, dim), z(blocks, kv_heads, block, dim)
+        self._k_exp, self._v_exp = z(blocks, kv_heads).fill_(127), z(blocks, kv_heads).fill_(127)
         self._need = {}   # workspace by numbers of query heads and rows
         self._c = _Cache(self.fmt, self.kv_heads, self.dim, self.block, self.blocks, self.k.data_ptr(), self.v.data_ptr(), self.k_exp.data_ptr(), self.v_exp.data_ptr())
         self._ref = ctypes.byref(self._c)

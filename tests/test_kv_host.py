@@ -8,7 +8,7 @@ import numpy as np
 import pytest
 
 from nn_b200 import _lib, api
-from nn_b200.kv_cache import KvBatch, _Batch, _Cache
+from nn_b200.kv_cache import KvBatch, KvCache, _Batch, _Cache
 from tests import kv_reference as ref
 
 P = 1 << 20   # a pointer that nothing follows: aligned, not NULL
@@ -163,3 +163,11 @@ def test_query_vectors_are_counted_in_32_bits(lib, ctx, over, status):
     b = _Batch(P, P, P, 1, 4, ((1 << 31) - 1 - over) // heads, 1)
     c = cache(kv_heads=1)
     assert lib.nnq_kv_attention_workspace(ctx, ctypes.byref(c), ctypes.byref(b), heads, ctypes.byref(need)) == status
+
+
+@pytest.mark.parametrize("kind,names", [(KvCache, ("k", "v", "k_exp", "v_exp")), (KvBatch, ("table", "length", "row_start", "slot", "position", "used", "rows"))])
+def test_tensors_that_calls_rely_on_are_not_replaced(kind, names):
+    """A cache's addresses go into every call, and a batch writes as many rows as its first slot map has."""
+    for name in names:
+        with pytest.raises(AttributeError):
+            setattr(kind.__new__(kind), name, None)
