@@ -753,8 +753,8 @@ typedef struct nnq_kv_cache {
  * row_start[r] .. row_start[r + 1] - 1); for each of `rows` packed rows its slot and position, -1 for rows behind the last
  * request; *used_dev (may be NULL) = *skip_dev + blocks taken. Where the list or a table's row ends, the entry and the slots of
  * its tokens are -1 and *used_dev says more than n_free. length_dev may be past_dev, used_dev may be
- * skip_dev: a captured step then advances the batch. Negative counts are taken as 0. One launch; neither
- * allocates nor synchronises, as all calls of this section. */
+ * skip_dev: a captured step then advances the batch. Negative counts are taken as 0. One launch. The nnq_kv_* calls
+ * and nnq_token_logprobs neither allocate nor synchronise and can be captured in a graph; the decoder's calls at the end of this section do both. */
 NNQ_API nnq_status nnq_kv_tables(nnq_ctx *ctx, const int32_t *past_dev, const int32_t *count_dev, int64_t requests, const int32_t *free_dev, int64_t n_free,
                                  const int32_t *skip_dev, int block, int32_t *table_dev, int64_t table_ld, int32_t *length_dev, int32_t *row_start_dev,
                                  int32_t *slot_dev, int32_t *position_dev, int64_t rows, int32_t *used_dev, void *stream);
@@ -773,7 +773,9 @@ NNQ_API nnq_status nnq_kv_append(nnq_ctx *ctx, const nnq_kv_cache *cache, const 
 NNQ_API nnq_status nnq_kv_read(nnq_ctx *ctx, const nnq_kv_cache *cache, const int32_t *slot_dev, int64_t rows, void *k_dev, void *v_dev, nnq_dtype dt, void *stream);
 
 /* The batch as attention reads it: what nnq_kv_tables writes (table_ld * block must stay below 2^31 - 1024). max_rows: rows of
- * the request with the most, as far as the host knows; it decides which kernels run and how much workspace they need, not what they compute. */
+ * the request with the most, as far as the host knows; it decides which kernels run and how much workspace they need, not what they compute: a
+ * number that is too small is right too, but slow (the keys of a prompt are then read again for every 8 query vectors). The kernel of a request
+ * and the parts that it is cut into follow from the whole batch: beside other requests the last bits of an output may differ, within what is said below. */
 typedef struct nnq_kv_batch {
     const int32_t *length, *row_start, *table;
     int64_t requests, table_ld, rows, max_rows;
@@ -803,14 +805,15 @@ NNQ_API nnq_status nnq_token_logprobs(nnq_ctx *ctx, const void *logits_dev, nnq_
                                       float *logprob_dev, float *entropy_dev, int32_t *top_token_dev, float *top_logprob_dev, void *stream);
 
 /* A Qwen3 decoder (nnq_decoder_create) with its keys and values in 8 bits, in blocks of `block` tokens (see nnq_kv_cache): a quarter of the
- * memory of the f32 cache, which is given back. Before the first token. A step appends and attends through the calls above, which takes
+ * memory of the f32 cache, which is given back. Before the first token; allocates, copies and waits for the device, so it cannot be captured. A step appends and attends through the calls above, which takes
  * four launches a layer in place of one. With this cache nnq_decoder_buffers gives NULL for the f32 ones; nnq_decoder_cache gives a layer's,
  * whose position p is slot p. */
 NNQ_API nnq_status nnq_decoder_set_cache(nnq_decoder *d, int format, int block);
 NNQ_API nnq_status nnq_decoder_cache(nnq_decoder *d, int layer, nnq_kv_cache *out);
 /* nnq_decoder_extend with log probabilities in place of the logits: after the `n_want` tokens want[] (at least one), the log probability of
  * given_host[i] (a negative one: 0), the entropy and the `top` most probable tokens as in nnq_token_logprobs, to host arrays [n_want]
- * and [n_want, top]. For both kinds of decoder. */
+ * and [n_want, top]. For both kinds of decoder. Allocates on its first call and waits for the stream behind every portion of tokens: it cannot be
+ * captured, as nnq_decoder_extend cannot. */
 NNQ_API nnq_status nnq_decoder_score(nnq_decoder *d, const int32_t *tokens_host, int count, int start_pos, const int32_t *want, int n_want, const int32_t *given_host, int top,
                                      float *logprob_host, float *entropy_host, int32_t *top_token_host, float *top_logprob_host, void *stream);
 

@@ -193,8 +193,9 @@ class KvCache:
 
     def attend(self, q, batch: KvBatch, scale: Optional[float] = None, window: int = 0, max_rows: int = 1, out=None):
         """Softmax attention of the batch's packed rows q [rows, heads, dim] to the positions up to their own (the last `window` of them, 0:
-        all), in q's dtype or out's. `scale` defaults to dim^-1/2. `max_rows`: rows of the request with the most, for the choice
-        of kernels. `out` must not overlap q. Rows behind the last request are left as `out` has them."""
+        all), in out's dtype, without one in q's where that is float32 or bfloat16 (others are taken as float32). `scale` defaults to dim^-1/2.
+        `max_rows`: rows of the request with the most, for the choice of kernels: with the default a prompt is right but many times slower.
+        `out` must not overlap q. Rows behind the last request are left as `out` has them."""
         torch = api._torch()
         b = self.backend
         heads = q.shape[1] if q.dim() == 3 else 0

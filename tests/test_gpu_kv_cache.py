@@ -634,6 +634,15 @@ def test_blocks_behind_every_window_may_have_been_given_back(rows, window, block
     check_attend(c, table, lengths, start, q, b, window=window)
 
 
+@pytest.mark.parametrize("dtype,want", [(torch.float32, torch.float32), (torch.bfloat16, torch.bfloat16), (torch.float16, torch.float32), (torch.float64, torch.float32)])
+def test_types_of_queries_and_outputs(dtype, want):
+    rng = np.random.default_rng(22)
+    c, table, start, q, b = serving(rng, 0, [40, 30], [1, 1], heads=4, kv=2, dim=64, block=16)
+    y = check_attend(c, table, [40, 30], start, q.to(dtype), b)
+    assert y.dtype == want
+    check_attend(c, table, [40, 30], start, q.to(dtype), b, out=torch.empty(2, 4, 64, dtype=torch.bfloat16, device=DEV))
+
+
 @pytest.mark.parametrize("window", [-1, 2 ** 31, 2 ** 32, 2 ** 32 + 5])
 def test_windows_beyond_31_bits_are_refused(window):
     c, b = kv_cache.KvCache(4, 2, 64), kv_cache.KvBatch(1, 4, 1, 16)
