@@ -262,3 +262,18 @@ def test_scores_of_a_block_decoder():
     lp, ent, order, _ = kvref.logprobs(logits, np.append(ids[1:], 0), 3)
     assert np.abs(r.logprob[:-1] - lp[:-1]).max() <= 1e-5 and np.abs(r.entropy - ent).max() <= 1e-5 and np.array_equal(r.top_tokens, order)
     dec.release()
+
+
+@pytest.mark.parametrize("fmt,block", [(kv_cache.INT8, 32), (kv_cache.E4M3, 64)])
+@pytest.mark.parametrize("group", [1, 4])
+def test_long_prompts_over_an_8_bit_cache(f32_products, fmt, block, group):
+    """Prompts of several tiles of the prompt attention's, in two portions, the second far behind the first one's start."""
+    count, cut = 640, 411
+    dec, model = _decoder(group, count + 2)
+    dec.set_cache(fmt, block)
+    want, ids = Restated(model, fmt, block), np.random.default_rng(group).integers(0, VOCAB, count + 2)
+    for a, e in ((0, cut), (cut, count), (count, count + 1), (count + 1, count + 2)):
+        got, exact = dec.extend(ids[a:e], a, list(range(e - a))), want.rows(ids[a:e])
+        assert np.abs(got - exact).max() <= 2e-3 * np.abs(exact).max(), (a, e, np.abs(got - exact).max() / np.abs(exact).max())
+    dec.backend.device_status()
+    dec.release()
