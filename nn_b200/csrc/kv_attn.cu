@@ -30,7 +30,9 @@
 // leaves a record (m, mv, l, O), and kv_join_kernel joins them in their order.
 // Measured (heads of 128, with the joining): 2 requests of 130001 positions, int8, 8 key / value heads of 5 f32 query heads, 115 us (4.6 TB/s of
 // codes); 40 requests of up to 12000, e4m3, 8 heads of 4 bf16 query heads, 90 us (4.0 TB/s); one of 2001 positions 12.5 us, of which the
-// two launches, the first loads behind the table and the joining are nearly all.
+// two launches, the first loads behind the table and the joining are nearly all. Counters of the first two: issue slots 58 / 64 % used, logic
+// pipe 44 / 52 %, tensor pipe 29 / 19 %: the codes' way to the operands stands beside the reading. Heads of 128 with f32 queries spill (128 registers, 192
+// bytes of stores: 1 % of the instructions).
 #include <algorithm>
 
 #include "kv_attn.cuh"
@@ -613,7 +615,7 @@ static nnq_status launch_kv_attn(nnq_ctx *ctx, const KvAttn &a, float *records, 
 }
 
 // Can the batch have requests for the tensor-core kernel, whatever their lengths are?
-static bool tc_rows(int dim, int group, int64_t max_rows) { return kv_attn_tc_supported(dim) && max_rows > kKvFew / group; }
+static bool tc_rows(int dim, int group, int64_t max_rows, int few) { return kv_attn_tc_supported(dim) && max_rows > few / group; }
 
 static nnq_status check_batch(nnq_ctx *ctx, const nnq_kv_cache *c, const nnq_kv_batch *b, int heads) {
     nnq_status s = check_kv_cache(ctx, c);
@@ -640,7 +642,7 @@ nnq_status nnq_kv_attention_workspace(nnq_ctx *ctx, const nnq_kv_cache *c, const
     nnq_status s = check_batch(ctx, c, b, heads);
     if (s != NNQ_OK) return s;
     *bytes = kv_records_bytes(ctx, c->dim) + kv_parts(ctx, c->dim) * sizeof(KvJoin);
-    if (tc_rows(c->dim, heads / c->kv_heads, b->max_rows)) *bytes = std::max(*bytes, kv_attn_tc_workspace(ctx, c->dim));
+    if (tc_rows(c->dim, heads / c->kv_heads, b->max_rows, kKvFew)) *bytes = std::max(*bytes, kv_attn_tc_workspace(ctx, c->dim));
     return NNQ_OK;
 }
 
@@ -663,15 +665,18 @@ nnq_status nnq_kv_attention(nnq_ctx *ctx, const nnq_kv_cache *c, const nnq_kv_ba
         return fail(ctx, NNQ_ERR_INVALID_ARG, "the workspace must be %zu bytes, 16-byte aligned (got %zu)", need, workspace ? workspace_bytes : (size_t)0);
     if ((s = check_cuda(ctx, cudaSetDevice(ctx->device), "cudaSetDevice")) != NNQ_OK) return s;
     KvAttn a = {(const uint8_t *)c->k, (const uint8_t *)c->v, c->k_exp, c->v_exp, b->length, b->row_start, b->table, q_dev, y_dev, c->blocks, b->table_ld, b->requests, q_ld, y_ld, b->rows,
-                      c->kv_heads, heads / c->kv_heads, c->dim, log2_of(c->block), window, (int)q_dt, (int)y_dt, INT32_MAX, scale, ctx->d_status};
+                      c->kv_heads, heads / c->kv_heads, c->dim, log2_of(c->block), window, (int)q_dt, (int)y_dt, INT32_MAX, INT32_MAX, scale, ctx->d_status};
     // The batch's requests are dealt between the two kernels on the device (kv_many). The tensor-core kernel is not launched where the
     // rows, the table's width and the window leave it none; a prompt alone goes to it wholly.
-    const bool prompt = b->max_rows > 2 * kKvFew / a.group;
+    const bool prompt = b->max_rows > kKvAlways / a.group;
+    const int few = q_dt == NNQ_BF16 && y_dt == NNQ_BF16 ? kKvFew : kKvFewF32;
     int64_t keys = b->table_ld * c->block;
     if (window > 0) keys = std::min(keys, window + std::min(b->max_rows, b->rows));
-    if (tc_rows(a.dim, a.group, b->max_rows) && (prompt || keys * a.kv_heads >= (kKvManyKeys + b->requests - 1) / b->requests)) {
-        a.few = prompt && b->requests == 1 ? 0 : kKvFew;
-        if ((s = launch_kv_attn_tc(ctx, a, c->format, (float *)workspace, (cudaStream_t)stream)) != NNQ_OK || a.few == 0) return s;
+    if (tc_rows(a.dim, a.group, b->max_rows, few) && (prompt || keys * a.kv_heads >= (kKvManyKeys + b->requests - 1) / b->requests)) {
+        const bool all = prompt && b->requests == 1;
+        a.few = all ? 0 : few;
+        a.many = all ? 0 : kKvAlways;
+        if ((s = launch_kv_attn_tc(ctx, a, c->format, (float *)workspace, (cudaStream_t)stream)) != NNQ_OK || all) return s;
     }
     return c->format == NNQ_KV_INT8 ? launch_kv_attn<NNQ_KV_INT8>(ctx, a, (float *)workspace, (cudaStream_t)stream)
                                     : launch_kv_attn<NNQ_KV_E4M3>(ctx, a, (float *)workspace, (cudaStream_t)stream);

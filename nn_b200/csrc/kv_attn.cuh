@@ -12,7 +12,7 @@ struct KvAttn {
     int64_t blocks, table_ld, requests, q_ld, y_ld, rows;
     int kv_heads, group, dim, shift, window;   // window 0: every earlier position
     int q_dt, y_dt;
-    int few;   // see kv_many: 0 (all requests go to kv_attn_tc_kernel), kKvFew or INT32_MAX (none goes)
+    int few, many;   // see kv_many; both 0: all requests go to kv_attn_tc_kernel, both INT32_MAX: none goes
     float scale;
     int *status;
 };
@@ -37,22 +37,28 @@ __device__ __forceinline__ int row_pos(const KvRequest &q, int i) { return q.len
 __device__ __forceinline__ int row_first(const KvAttn &a, int pos) { return a.window > 0 && pos >= a.window ? pos - a.window + 1 : 0; }
 
 // Which kernel a request goes to. kv_attn_tc_kernel takes 256 query vectors of a key / value head for the price of one, but begins
-// slowly and deals a batch in coarser parts; kv_attn_kernel reads the keys again for every 8 vectors. Heads of 128, int8, bf16, group 4,
+// slowly and deals a batch in coarser parts; kv_attn_kernel reads the keys again for every 8 vectors. Heads of 128, int8, group 4,
 // 8 key / value heads, us of kv_attn_kernel / kv_attn_tc_kernel:
-//   vectors           40             56             80            112
-//   2 x 500      18.0 / 27.4    19.8 / 28.0    22.7 / 28.3    23.7 / 29.6
-//   2 x 4000     29.1 / 40.6    36.3 / 41.6    46.2 / 42.9    58.6 / 44.7
-//   16 x 500     43.1 / 36.1    50.4 / 36.5    67.1 / 37.4    85.3 / 37.9
-//   2 x 30000     119 / 110      161 / 111      224 / 112      306 / 115
-//   16 x 4000     142 / 117      191 / 118      267 / 122      362 / 124
-//   16 x 30000    929 / 638     1233 / 619     1949 / 626     2715 / 635
-// 32 vectors: 2 x 30000 98 / 108, 16 x 4000 117 / 115, 16 x 30000 702 / 605, with f32 queries 111 / 153, 131 / 164, 820 / 959. So: beyond
-// 64, and beyond 32 if the batch has 2^16 keys of all heads and requests (taken for as long as this one).
-constexpr int kKvFew = 32;
+//   bf16, vectors       32             40             56             80            112
+//   2 x 500      17.7 / 30.8    18.8 / 30.8    20.5 / 31.2    23.2 / 31.6    24.5 / 33.0
+//   2 x 4000     27.6 / 44.5    29.3 / 44.6    36.6 / 45.6    46.7 / 46.7    58.6 / 48.1
+//   16 x 500     37.6 / 42.2    43.8 / 41.9    51.2 / 42.3    68.2 / 43.4    86.9 / 44.1
+//   2 x 30000    98.1 / 121      117 / 121      159 / 122      219 / 123      300 / 125
+//   16 x 4000     118 / 131      140 / 132      188 / 134      262 / 138      356 / 140
+//   16 x 30000    686 / 718      853 / 723     1156 / 729     1699 / 738     2363 / 744
+//   f32
+//   2 x 4000     32.1 / 53.2    33.4 / 53.8    41.1 / 54.6    51.6 / 56.1    64.3 / 58.1
+//   16 x 500     42.1 / 48.2    49.5 / 48.7    58.0 / 49.1    77.4 / 50.6    97.2 / 51.9
+//   2 x 30000     109 / 171      129 / 171      175 / 172      243 / 173      329 / 173
+//   16 x 4000     131 / 184      156 / 185      208 / 187      291 / 190      393 / 192
+//   16 x 30000   748 / 1066     934 / 1068    1278 / 1069    1839 / 1077    2534 / 1080
+// So: beyond 64, and beyond 32 (48 where queries or outputs are f32) if the batch has 2^16 keys of all heads and requests (taken for
+// as long as this one).
+constexpr int kKvFew = 32, kKvFewF32 = 48, kKvAlways = 64;
 constexpr int64_t kKvManyKeys = 1 << 16;
 __device__ __forceinline__ bool kv_many(const KvAttn &a, const KvRequest &q) {
     const int64_t vecs = (int64_t)q.rows * a.group, keys = q.length - row_first(a, max(row_pos(q, 0), 0));
-    return vecs > 2 * (int64_t)a.few || (vecs > a.few && (float)keys * (float)a.kv_heads * (float)a.requests >= (float)kKvManyKeys);
+    return vecs > a.many || (vecs > a.few && (float)keys * (float)a.kv_heads * (float)a.requests >= (float)kKvManyKeys);
 }
 
 // Two f16 numbers of two codes that lie in the bytes of a 16-bit half each: int8 exactly, e4m3 times 2^-8 (its bits moved to their
