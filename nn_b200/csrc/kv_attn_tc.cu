@@ -12,11 +12,14 @@
 //   warps 16, 17:   (two more complete their group) a lane of each issues the MMAs of one softmax group: S(t + 1), then O += P(t) V(t). They
 //                   run in the order they are issued, so S(t + 1) may overwrite the weights of t - 1, whose product stands in front
 //                   of it. (One warp for both groups took 100 clocks an MMA beside the scheduler's other warps and set the pace.)
-// What bounds it is the softmax: some 6100 instructions of a scheduler's warps per tile of both groups, the exponentials among them (the
-// special function unit takes 16 a clock and SM), and the hand-over between softmax and MMA. Measured: 2000 rows behind 2100, e4m3, 8 key /
-// value heads of 4 bf16 query heads of 128, 215 us with the joining, 474 TFLOP/s of the 102 GFLOP that a causal prompt takes; counters of an
-// earlier form of 182 us: tensor pipe 30 % active, logic and FMA pipes 38 %, special functions 32 %. Slower were 128 keys a tile with both
-// MMA warps on each (217 us) and four converter warps in favour of more registers for the softmax (186 beside 182).
+// What bounds it are waits, not a unit: per 64 keys a softmax group goes through scores -> maxima -> weights -> hand-over, with two of its warps on a
+// scheduler. Measured: 2000 rows behind 2100, e4m3, 8 key / value heads of 4 bf16 query heads of 128, 215 us with the joining, 474 TFLOP/s of the
+// 102 GFLOP that a causal prompt takes: 7900 warp instructions of an SM per tile of both groups, issue slots 51 % used, tensor pipe 39 %, logic
+// pipe 38 %, special functions 28 %, FMA pipe 22 %; of the warps' waits four in ten for loads (of scores from tensor memory, of codes). f32 rows: 346 us, 34 %
+// and 32 %, with the records' sums beside them. Slower were 128 keys a tile with both
+// MMA warps on each (217 us where this form took 182) and four converter warps in favour of more registers for the softmax (186 beside 182).
+// The compiler spills (-Xptxas -v: 404 to 424 bytes of stores, 96 registers; it does not say in which role): 1.7 % of the instructions are loads and
+// stores of local memory.
 // Codes are exact in f16. A query vector is one f16 term under its power of two where that is exact (T = 1: bf16 queries and outputs), else two (T = 2); a
 // weight is always two, 22 bits (with one, 11 bits and 188 us for the prompt above, a bf16 output differed from the rounded exact one by 9e-4 in the
 // 2-norm, now by 2e-4).

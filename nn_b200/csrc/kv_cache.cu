@@ -12,9 +12,10 @@ namespace nnq {
 
 // One launch of one cluster: every CTA sums the counts of all requests, in portions of kTabChunk that lie in shared memory, and writes
 // its share of the tables: entry i of the portion's new blocks, row i of its rows, found by bisection of the sums. The cluster meets
-// between the reading of a portion and the writing, so lengths may be written where the old ones lie. What bounds it is latency:
-// the requests' loads, the sums, the bisection, one dependent load for a block that was there before. Measured: 8 single tokens 2.4 us,
-// 300 requests with some 32000 rows 10.2 us.
+// between the reading of a portion and the writing, so lengths may be written where the old ones lie. Single tokens are bound by latency:
+// the requests' loads, the sums, the bisection, one dependent load for a block that was there before (8 of them 2.4 us). Many rows are
+// bound by the threads of one cluster, which bisect for every row: 300 requests with some 32000 rows 10.2 us, half of the issue slots of its eight
+// SMs used (one CTA of 256 threads: 84 us).
 constexpr int kTabChunk = 2048;
 
 struct TableArgs {
@@ -137,7 +138,10 @@ __global__ void __launch_bounds__(1024) kv_tables_kernel(const TableArgs a) {
 // left out), the exponent byte, the codes; codes the block held before are rounded again where the exponent grew. The first pieces of
 // eight values of a lane stay in registers in between.
 // What bounds it is latency: the chain slot -> values -> codes, which a warp goes through alone (a CTA per run, with a barrier in it:
-// 12000 rows of 8 heads of 128, bf16, 43 us). Measured: those 32 us, 48 single f32 rows with the read behind them 4.4 us.
+// 12000 rows of 8 heads of 128, bf16, blocks of 32, 43 us). Measured: those 32 us, issue slots 44 % used, most waits for loads; 48 single f32 rows
+// with the read behind them 4.4 us. Large runs are slow, as one warp has them whole: 4000 rows of a prompt, 8 heads, in blocks of 16 / 64 / 256 tokens 5.7 /
+// 12.7 / 33.6 us (dim 64) and 15.9 / 45.9 / 136 us (dim 256); 48 single tokens that raise the scale of a full block 2.9 / 5 / 14 us and
+// 4.6 / 14 / 53 us, else 3 us.
 constexpr int kAppWarps = 8;
 
 struct AppendArgs {
@@ -329,8 +333,9 @@ struct ReadArgs {
     int *status;
 };
 
-// A thread has 16 values of a row: one load, two or four stores. Rows of no slot are zeros. Bound by the stores: 12000 rows of 8 heads of
-// 128 to bf16 16.6 us (4.4 TB/s both ways).
+// A thread has 16 values of a row: one load, two or four stores. Rows of no slot are zeros. 12000 rows of 8 heads of 128, e4m3, to bf16:
+// 16.6 us (4.4 TB/s both ways), bound by the conversions: issue slots 75 % used, logic pipe 65 %. (A warp's stores leave gaps of 16 bytes
+// that its next ones fill.)
 template <int FMT, bool F32>
 __global__ void __launch_bounds__(256) kv_read_kernel(const ReadArgs a) {
     pdl_prologue();
