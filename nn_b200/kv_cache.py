@@ -42,16 +42,25 @@ def _int32(t, name: str, shape, index: int):
     return t
 
 
-def _fixed(name: str):
-    """A tensor whose memory the calls rely on: filled in place (``copy_``), not replaced."""
-    return property(lambda self: getattr(self, "_" + name))
+class _InPlace:
+    """Tensors whose memory the calls rely on are filled in place (``copy_``), not replaced."""
+    _fixed = frozenset()
+
+    def __setattr__(self, name, value):
+        if name in self._fixed:
+            raise AttributeError(f"{type(self).__name__}.{name} is filled in place, not replaced")
+        object.__setattr__(self, name, value)
+
+    def _place(self, **tensors):
+        for name, value in tensors.items():
+            object.__setattr__(self, name, value)
 
 
-class KvBatch:
+class KvBatch(_InPlace):
     """Block tables [requests, max_blocks], lengths, packed rows (row_start), and slot and position of every row, on the device. The tensors
     are filled in place, not replaced."""
 
-    table, length, row_start, slot, position, used = map(_fixed, ("table", "length", "row_start", "slot", "position", "used"))
+    _fixed = frozenset(("table", "length", "row_start", "slot", "position", "used", "rows"))
 
     def __init__(self, requests: int, max_blocks: int, rows: int, block: int = 16, backend: Optional[api.Backend] = None):
         if requests < 1 or max_blocks < 1 or rows < 0:
@@ -61,8 +70,8 @@ class KvBatch:
         self.backend, self.block = b, int(block)
         self.device = torch.device("cuda", b.device)
         z = lambda *s: torch.zeros(s, dtype=torch.int32, device=self.device)  # noqa: E731
-        self._table = torch.full((requests, max_blocks), -1, dtype=torch.int32, device=self.device)
-        self._length, self._row_start, self._slot, self._position, self._used = z(requests), z(requests + 1), z(rows), z(rows), z(1)
+        self._place(table=torch.full((requests, max_blocks), -1, dtype=torch.int32, device=self.device), length=z(requests), row_start=z(requests + 1),
+                    slot=z(rows), position=z(rows), used=z(1), rows=int(rows))
 
     @classmethod
     def from_tensors(cls, table, length, row_start, block: int, slot=None, position=None, backend: Optional[api.Backend] = None) -> "KvBatch":
@@ -74,20 +83,16 @@ class KvBatch:
         if table.dim() != 2 or table.shape[0] < 1 or table.shape[1] < 1:
             raise api.ShapeMismatch(f"table: expected [requests, blocks], got {tuple(table.shape)}")
         n = table.shape[0]
-        self._table, self._length = _int32(table, "table", table.shape, b.device), _int32(length, "length", (n,), b.device)
-        self._row_start = _int32(row_start, "row_start", (n + 1,), b.device)
-        self._slot = None if slot is None else _int32(slot, "slot", (slot.numel(),), b.device)
-        self._position = None if position is None else _int32(position, "position", (position.numel() if slot is None else slot.numel(),), b.device)
-        self._used = torch.zeros(1, dtype=torch.int32, device=self.device)
+        rows = 0 if slot is None else slot.numel()
+        self._place(table=_int32(table, "table", table.shape, b.device), length=_int32(length, "length", (n,), b.device),
+                    row_start=_int32(row_start, "row_start", (n + 1,), b.device), slot=None if slot is None else _int32(slot, "slot", (rows,), b.device),
+                    position=None if position is None else _int32(position, "position", (position.numel() if slot is None else rows,), b.device),
+                    used=torch.zeros(1, dtype=torch.int32, device=self.device), rows=rows)
         return self
 
     @property
     def requests(self) -> int:
         return self.table.shape[0]
-
-    @property
-    def rows(self) -> int:
-        return 0 if self._slot is None else self._slot.numel()
 
     def build(self, past, count, free, skip=None):
         """Tables and slots for `count` new tokens behind `past` ones, int32 [requests] each. `free`: numbers of free blocks (int32), of which
@@ -96,7 +101,7 @@ class KvBatch:
         and so do tokens for whose block the list or the table had no room (``used`` then exceeds the list)."""
         if self.slot is None or self.position is None:
             raise api.InvalidArgument("a batch without slot and position tensors cannot be built")
-        n, b = self.requests, self.backend
+        n, b = self.table.shape[0], self.backend
         past, count = _int32(past, "past", (n,), b.device), _int32(count, "count", (n,), b.device)
         free = _int32(free, "free", (free.numel(),), b.device)
         if skip is not None:
@@ -109,11 +114,11 @@ class KvBatch:
         return self
 
 
-class KvCache:
+class KvCache(_InPlace):
     """One layer's keys and values: codes uint8 [blocks, kv_heads, block, dim] (``k``, ``v``) and exponent bytes uint8 [blocks, kv_heads]
     (``k_exp``, ``v_exp``); value = code * 2^(byte - 127). A saved cache is brought back with ``copy_`` into these tensors."""
 
-    k, v, k_exp, v_exp = map(_fixed, ("k", "v", "k_exp", "v_exp"))
+    _fixed = frozenset(("k", "v", "k_exp", "v_exp"))
 
     def __init__(self, blocks: int, kv_heads: int, dim: int, block: int = 16, fmt: int = INT8, backend: Optional[api.Backend] = None):
         torch = api._torch()
@@ -129,8 +134,8 @@ class KvCache:
         self.blocks, self.kv_heads, self.dim, self.block, self.fmt = int(blocks), int(kv_heads), int(dim), int(block), int(fmt)
         self.device = torch.device("cuda", b.device)
         z = lambda *s: torch.zeros(s, dtype=torch.uint8, device=self.device)  # noqa: E731
-        self._k, self._v = z(blocks, kv_heads, block, dim), z(blocks, kv_heads, block, dim)
-        self._k_exp, self._v_exp = z(blocks, kv_heads).fill_(127), z(blocks, kv_heads).fill_(127)
+        self._place(k=z(blocks, kv_heads, block, dim), v=z(blocks, kv_heads, block, dim), k_exp=z(blocks, kv_heads).fill_(127),
+                    v_exp=z(blocks, kv_heads).fill_(127))
         self._need = {}   # workspace by numbers of query heads and rows
         self._c = _Cache(self.fmt, self.kv_heads, self.dim, self.block, self.blocks, self.k.data_ptr(), self.v.data_ptr(), self.k_exp.data_ptr(), self.v_exp.data_ptr())
         self._ref = ctypes.byref(self._c)
@@ -209,7 +214,8 @@ class KvCache:
             raise api.InvalidArgument(f"a window of {window}")
         if batch.block != self.block or batch.backend.device != b.device:
             raise api.InvalidArgument(f"a batch of blocks of {batch.block} on {batch.device} for a cache of blocks of {self.block} on {self.device}")
-        c = _Batch(batch.length.data_ptr(), batch.row_start.data_ptr(), batch.table.data_ptr(), batch.requests, batch.table.shape[1], n, max(int(max_rows), 1))
+        table = batch.table
+        c = _Batch(batch.length.data_ptr(), batch.row_start.data_ptr(), table.data_ptr(), *table.shape, n, max(int(max_rows), 1))
         need = self._need.get((heads, c.max_rows))
         if need is None:
             size = ctypes.c_size_t()
