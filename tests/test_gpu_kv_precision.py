@@ -107,3 +107,29 @@ def test_outputs_in_bf16_are_the_exact_ones_rounded(fmt, rows, dim, window):
     wrong = ~((low <= y) & (y <= high))
     assert not wrong.any(), (int(wrong.sum()), wrong.numel())
     c.backend.device_status()
+
+
+@pytest.mark.parametrize("fmt,dim", [(kv_cache.INT8, 64), (kv_cache.E4M3, 128)])
+@pytest.mark.parametrize("window", [0, 20, 300])
+def test_chains_in_which_some_rows_see_nothing(fmt, dim, window):
+    """f32 prompts whose sums leave tensor memory on the way: rows that see their first key behind that, blocks whose scales are far apart, so that
+    the references move by much between two chains, rows in front of position 0, and a query that is not finite."""
+    rng = np.random.default_rng(window + dim)
+    lengths, rows = [700, 200], [300, 260]
+    c, table, start, q, b = serving(rng, fmt, lengths, rows, heads=2, kv=2, dim=dim, block=32)
+    for _ in range(2):
+        y = c.attend(q, b, window=window, max_rows=300)
+        want, mag, top = ref.attend(q.double().cpu().numpy(), *values_of(c), table, lengths, start, 32, dim ** -0.5, window)
+        lim = bound(mag, want, top, dim, min(window or 700, 700), torch.float32, np.abs(values_of(c)[1]).max())
+        off = np.abs(y.double().cpu().numpy() - want)
+        assert (off <= lim).all(), float((off / lim).max())
+        assert not y[300:360].any()
+        q2 = q.clone()
+        q2[280, 1, 3], q2[290, 0, 7] = float("nan"), float("inf")
+        got = c.attend(q2, b, window=window, max_rows=300)
+        assert got[280, 1].isnan().all() and got[290, 0].isnan().all()
+        got[280, 1], got[290, 0] = y[280, 1], y[290, 0]
+        off = np.abs(got.double().cpu().numpy() - want)
+        assert (off <= lim).all()
+        c.backend.device_status()
+        c.v_exp.copy_(torch.from_numpy(rng.integers(90, 150, c.v_exp.shape).astype(np.uint8)))
