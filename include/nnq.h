@@ -785,8 +785,8 @@ typedef struct nnq_kv_batch {
  * its own, with window > 0 the last `window` of them; query head h reads key / value head h / (heads / kv_heads).
  * q [rows, heads, dim] and y in the same layout, f32 or bf16, rows q_ld / y_ld elements apart, 16-byte aligned, apart from each
  * other. A row that sees nothing is zero; rows behind the last request are left as they were. Scores, softmax and sums are f32, codes exact, queries
- * and weights enter the products with 22 bits (bf16 queries exactly), weights below some 2^-10 of the largest of a vector with fewer: no weight
- * is off by more than 2^-32 of the largest. Sums of products are cut off towards zero inside the tensor core and join others in f32 after short chains: f32 outputs
+ * and weights enter the products with 22 bits (bf16 queries exactly), weights below some 2^-10 of the largest of a vector with fewer: each
+ * taken with its block's scale of values, none is off by more than 2^-32 of the largest. Sums of products are cut off towards zero inside the tensor core and join others in f32 after short chains: f32 outputs
  * lean by some 1e-6 of sum p |v| whatever the length, bf16 ones by 2e-5. Blocks that no row sees (behind every window, beyond the length) may have
  * any number. Of the others one outside the cache is not read: its positions
  * count as unseen, and nnq_device_status reports NNQ_ERR_INVALID_ARG. The workspace (nnq_kv_attention_workspace; 16-byte
