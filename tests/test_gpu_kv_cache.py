@@ -634,6 +634,24 @@ def test_blocks_behind_every_window_may_have_been_given_back(rows, window, block
     check_attend(c, table, lengths, start, q, b, window=window)
 
 
+@pytest.mark.parametrize("rows", [3, 90])
+def test_caches_beyond_32_bits_of_bytes(rows):
+    """The last blocks of a cache of 5 GB of codes, against a small cache with the same tokens."""
+    kv, dim, block, need = 2, 128, 64, 2
+    large, small = kv_cache.KvCache(320000, kv, dim, block), kv_cache.KvCache(need, kv, dim, block)
+    assert large.k.numel() > 1 << 32
+    k, v, q = torch.randn(rows, kv, dim, device=DEV), torch.randn(rows, kv, dim, device=DEV), torch.randn(rows, 8, dim, device=DEV)
+    out = []
+    for c, first in ((large, large.blocks - need), (small, 0)):
+        slots = first * block + torch.arange(rows, dtype=torch.int32, device=DEV)
+        c.append(k, v, slots)
+        b = kv_cache.KvBatch.from_tensors(i32([[first, first + 1]]), i32([rows]), i32([0, rows]), block)
+        out.append((*c.read(slots), c.attend(q, b, max_rows=rows)))
+    assert all(torch.equal(x, y) for x, y in zip(*out)) and out[0][2].any()
+    assert torch.equal(large.k[-need:], small.k) and torch.equal(large.v_exp[-need:], small.v_exp) and not large.k[:-need].any() and not large.v[:-need].any()
+    large.backend.device_status()
+
+
 @pytest.mark.parametrize("dtype,want", [(torch.float32, torch.float32), (torch.bfloat16, torch.bfloat16), (torch.float16, torch.float32), (torch.float64, torch.float32)])
 def test_types_of_queries_and_outputs(dtype, want):
     rng = np.random.default_rng(22)

@@ -231,3 +231,12 @@ def test_masked_rows_cost_what_others_do():
     plain, masked = shortest(x), shortest(few)
     print(f"{plain * 200:.1f} and {masked * 200:.1f} us")
     assert masked <= 3 * plain
+
+
+def test_logits_beyond_32_bits_of_bytes():
+    x = torch.zeros(9001, 128001, device="cuda:0")   # 4.6 GB
+    x[-1].normal_()
+    token = torch.full((9001,), 77, dtype=torch.int32, device="cuda:0")
+    r, one = token_logprobs(x, token, 3), token_logprobs(x[-1:].clone(), token[-1:], 3)
+    assert torch.equal(r.top_tokens[-1], one.top_tokens[0]) and float((r.logprob[-1] - one.logprob[0]).abs()) <= 1e-5
+    assert r.top_tokens[-2].tolist() == [0, 1, 2] and abs(float(r.logprob[0]) + np.log(128001)) <= 1e-5
